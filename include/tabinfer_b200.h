@@ -418,6 +418,81 @@ TB_API int tb_attn_decode_q8_batch(tb_ctx *ctx, float *out, const float *qr,
                                    const int32_t *dpos, int64_t S_max, int64_t nHq, int64_t nKv,
                                    int64_t hd, int nsplit);
 
+/* ---- paged int8 KV cache ---------------------------------------------------
+ * No counterpart in the reference, which keeps one contiguous cache a sequence.
+ * A page holds page_rows rows in the format of that cache (tb_attn_prep_q8):
+ * pools Kq/Vq int8 [n_pages][page_rows][nKv*hd], Ks/Vs f32
+ * [n_pages][page_rows][nKv*hd/32]; row r of sequence b is line r % page_rows of
+ * pool page table[b][r / page_rows] (sequences may share pages; entries behind a
+ * sequence's last row are not read).  An element stands for q / 127 * scale
+ * (bytes -127 .. 127, as every writer here leaves them).
+ * page_rows 16, 32, 64, 128 or 256; hd 64 or 128; nHq/nKv 1, 2, 4 or 8; n_pages *
+ * page_rows < 2^31; pools 16-byte aligned.
+ * What the host cannot see is checked on the device: a page number outside the
+ * pool sets the context's error word (tb_ctx_device_error) to 0x6c01 and its rows
+ * are neither read nor written; a length or row that the table cannot hold, or a
+ * chunk longer than its sequence, sets 0x6c02 and counts as empty.
+ * ws: device workspace of the size that the call's _ws query gives (it depends on
+ * the sizes in kv, nHq and T only), 256-byte aligned and not shared by calls that
+ * may overlap; NULL takes the context's scratch, which calls of one stream share
+ * and which grows on the first call at a size (before a capture).  */
+typedef struct tb_paged_kv {
+  int8_t *Kq;
+  float *Ks;
+  int8_t *Vq;
+  float *Vs;
+  const int32_t *table;   /* device [batch][max_pages] */
+  int64_t n_pages, page_rows, batch, max_pages, nKv, hd;
+} tb_paged_kv;
+
+/* attnPrepQ8 (models/qwen3.js:2297-2308) for T rows of any sequences at once:
+ * row t of q f32 [T][nHq*hd] and k, v f32 [T][nKv*hd] goes to cache row slot[t] of
+ * sequence seq[t] with rotary position pos[t] (all device i32 [T]; the (seq, slot)
+ * pairs of a call are distinct).  q -> per-head RMSNorm + RoPE -> qr f32; k the
+ * same and v as it is -> snorm int8 per 32 into the cache.  seq[t] < 0 marks a
+ * padding row: nothing is written for it.  Norm and rotation are formed in 64 bits
+ * and rounded to f32 once, so a cache byte does not depend on the call that wrote it. */
+TB_API int tb_attn_prep_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, const float *q, const float *k,
+                                 const float *v, const uint16_t *qw16, const uint16_t *kw16, float *qr,
+                                 int64_t nHq, int64_t T, const int32_t *seq, const int32_t *slot,
+                                 const int32_t *pos, float theta, float eps);
+
+/* Attention of one new token a sequence: qr, out f32 [batch][nHq*hd]; lens i32
+ * [batch] (device): the rows of each sequence, the new token's own (the last) among
+ * them; length 0 gives a row of zeros.  window > 0: the token sees the last
+ * `window` rows and the first `sinks` (0: all rows).  weights f32
+ * [batch][nKv][max_pages*page_rows] or NULL: the softmax weight of every row seen,
+ * summed over the kv head's q heads, is added to it (the input of
+ * tb_kv_evict_paged_q8).  Same math as tb_attn_decode_q8; results do not depend on
+ * timing. */
+TB_API int tb_attn_decode_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, int64_t nHq, int weights, size_t *bytes);
+TB_API int tb_attn_decode_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, float *out, const float *qr,
+                                   const int32_t *lens, int64_t nHq, int64_t window, int64_t sinks,
+                                   float *weights, void *ws, size_t ws_bytes);
+
+/* Attention of packed prompts or chunks of prompts: q f32 [T][nHq*hd] (after
+ * tb_attn_prep_paged_q8), out bf16 [T][nHq*hd] (the X that tb_gemm_int4_g32
+ * takes).  Rows cu[b] .. cu[b+1]-1 (device i32 [batch+1], ascending) are the last
+ * rows of sequence b's lens[b]; each sees the rows up to its own, under window and
+ * sinks as above.  Rows before cu[0] and from cu[batch] on are left as they were.
+ * Operands may be rounded to f16 (as in tb_attn_prefill_q8); sums in f32. */
+TB_API int tb_attn_prefill_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, int64_t nHq, int64_t T, size_t *bytes);
+TB_API int tb_attn_prefill_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, uint16_t *out_bf16, const float *q,
+                                    const int32_t *cu, const int32_t *lens, int64_t nHq, int64_t T,
+                                    int64_t window, int64_t sinks, void *ws, size_t ws_bytes);
+
+/* Shrinks every sequence to at most `budget` rows: its first `sinks` and last
+ * `recent` rows stay, then those with the largest score = sum over kv heads of
+ * weights[b][h][row] (formed in 64 bits; ties go to the lower row).  The rows that
+ * stay are copied in order into the pages of dst (its table; the pools of kv or
+ * others; none of its pages may be one that the call reads).  kept i32 [batch][budget]: the old row
+ * of each new one, -1 behind the last; new_lens i32 [batch]; new_weights f32
+ * [batch][nKv][dst max_pages*page_rows]: the kept rows' weights, then zeros. */
+TB_API int tb_kv_evict_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, size_t *bytes);
+TB_API int tb_kv_evict_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, const tb_paged_kv *dst, const int32_t *lens,
+                                const float *weights, int32_t *kept, int32_t *new_lens, float *new_weights,
+                                int64_t budget, int64_t sinks, int64_t recent, void *ws, size_t ws_bytes);
+
 /* ---- decode-step glue ------------------------------------------------------ */
 
 /* Argmax over `rows` rows of n logits -> out_idx[row*stride + offset]

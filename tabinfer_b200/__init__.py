@@ -18,6 +18,7 @@ from .ops import (  # noqa: F401
     quantize_tern_bf16, gemv_tern_wgsl, gemv_tern_wgsl_dp4a_multi, gate_up_silu_tern, gate_up_silu_tern_dp4a,
     gemm_tern, gemm_dp4, gemm_dp4_f16, linear_tern_wgsl,
     attn_prep_q8, kv_quant_write, attention_decode_q8, attention_prefill_q8, argmax,
+    attn_prep_paged_q8, attention_decode_paged_q8, attention_prefill_paged_q8, kv_evict_paged_q8,
     logit_mask, gumbel_noise, sample_argmax, GumbelSeeds, rmsnorm, embed_gather,
 )
 from .qwen3 import Qwen3, QWEN3_1_7B, QWEN3_0_6B  # noqa: F401,E402

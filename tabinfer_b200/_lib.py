@@ -79,6 +79,13 @@ SIGNATURES = {
     "tb_kv_quant_write": [P, P, P, P, P, P, P, I64, I64, I64, I64],
     "tb_attn_decode_q8": [P, P, P, P, P, P, P, I64, I64, I64, I64, I32],
     "tb_attn_decode_q8_noalloc": [P, P, P, P, P, P, P, I64, I64, I64, I64, I32],
+    "tb_attn_prep_paged_q8": [P, P, P, P, P, P, P, P, I64, I64, P, P, P, F32, F32],
+    "tb_attn_decode_paged_ws": [P, P, I64, I32, P],
+    "tb_attn_decode_paged_q8": [P, P, P, P, P, I64, I64, I64, P, P, ctypes.c_size_t],
+    "tb_attn_prefill_paged_ws": [P, P, I64, I64, P],
+    "tb_attn_prefill_paged_q8": [P, P, P, P, P, P, I64, I64, I64, I64, P, ctypes.c_size_t],
+    "tb_kv_evict_paged_ws": [P, P, P],
+    "tb_kv_evict_paged_q8": [P, P, P, P, P, P, P, P, I64, I64, I64, P, ctypes.c_size_t],
     "tb_argmax": [P, P, I64, I64, P, I64],
     "tb_rmsnorm": [P, P, P, P, I64, I64, F32],
     "tb_embed_gather": [P, P, I64, P, P, I64, I64],
@@ -152,6 +159,12 @@ class BinTensor(ctypes.Structure):
 
 
 BIN_TERN, BIN_EMBED_F16, BIN_F32 = 0, 1, 2
+
+
+class PagedKV(ctypes.Structure):
+    """tb_paged_kv (include/tabinfer_b200.h)"""
+    _fields_ = [("Kq", P), ("Ks", P), ("Vq", P), ("Vs", P), ("table", P), ("n_pages", I64), ("page_rows", I64),
+                ("batch", I64), ("max_pages", I64), ("nKv", I64), ("hd", I64)]
 
 
 def load(path=LIB_PATH):

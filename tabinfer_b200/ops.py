@@ -11,7 +11,7 @@ import threading
 
 import torch
 
-from ._lib import LIB, P
+from ._lib import LIB, P, PagedKV
 
 TB_ACT_F32, TB_ACT_Q8 = 0, 1
 CUDA_STREAM_LEGACY = 0x1   # cudaStreamLegacy
@@ -625,6 +625,132 @@ def attention_decode_q8(qr, kv, S, nHq, nKv, hd, nsplit=0, out=None):
     c.check(LIB.tb_attn_decode_q8(c.h, _p(out), _p(qr), _p(Kq), _p(Ks), _p(Vq), _p(Vs), int(S), nHq, nKv, hd,
                                   int(nsplit)), "attn_decode_q8")
     return out
+
+
+# --------------------------------------------------------------------------
+# paged int8 KV cache (no counterpart in the reference).  kv = (Kq, Ks, Vq, Vs):
+# pools int8 [n_pages, page_rows, nKv*hd] and f32 [n_pages, page_rows, nKv*hd/32];
+# table int32 [batch, max_pages]: row r of sequence b is line r % page_rows of pool
+# page table[b, r // page_rows].
+# --------------------------------------------------------------------------
+
+def _arg(t, what, dtype, shape, device):
+    """A dense device tensor of this type and shape (None: any extent) on `device` -> its address."""
+    if t.dtype != dtype or t.dim() != len(shape) or t.device != device or not t.is_contiguous():
+        raise TabInferError("%s must be a contiguous %s tensor of %d dimensions on %s" % (what, dtype, len(shape), device))
+    for have, want in zip(t.shape, shape):
+        if want is not None and have != want:
+            raise TabInferError("%s: shape %s does not fit %s" % (what, tuple(t.shape), tuple(shape)))
+    return t.data_ptr()
+
+
+def _paged(kv, table, nKv, hd, device, what="kv"):
+    """The cache's tb_paged_kv, its tensors checked."""
+    if device.type != "cuda":
+        raise TabInferError("tensor must be on a CUDA device")
+    Kq, Ks, Vq, Vs = kv
+    if Kq.dim() != 3:
+        raise TabInferError("%s: pools are [n_pages, page_rows, nKv*hd]" % what)
+    n, r, _ = Kq.shape
+    w = nKv * hd
+    kq = _arg(Kq, what + " Kq", torch.int8, (n, r, w), device)
+    ks = _arg(Ks, what + " Ks", torch.float32, (n, r, w // 32), device)
+    vq = _arg(Vq, what + " Vq", torch.int8, (n, r, w), device)
+    vs = _arg(Vs, what + " Vs", torch.float32, (n, r, w // 32), device)
+    tab = _arg(table, "table", torch.int32, (None, None), device)
+    return PagedKV(kq, ks, vq, vs, tab, n, r, table.shape[0], table.shape[1], nKv, hd)
+
+
+def _workspace(c, what, query, device, *sizes):
+    """Workspace of a paged call: a tensor of the current stream's allocator, so calls on other
+    streams and captured graphs have their own."""
+    n = ctypes.c_size_t(0)
+    c.check(query(c.h, *sizes, ctypes.byref(n)), what)
+    return torch.empty(max(n.value, 256), dtype=torch.uint8, device=device), n.value
+
+
+def attn_prep_paged_q8(q, k, v, qw16, kw16, kv, table, seq, slot, pos, nHq, nKv, hd, theta, eps, qr=None):
+    """attnPrepQ8 (qwen3.js:2297-2308) for T rows of any sequences: row t of q [T, nHq*hd] and
+    k, v [T, nKv*hd] -> cache row slot[t] of sequence seq[t] at rotary position pos[t] (int32 [T];
+    seq < 0: a padding row, nothing is written).  Returns qr f32 [T, nHq*hd]."""
+    d, T = q.device, q.shape[0]
+    s = _paged(kv, table, nKv, hd, d)
+    if qr is None:
+        qr = torch.empty((T, nHq * hd), dtype=torch.float32, device=d)
+    qp, op = _arg(q, "q", torch.float32, (T, nHq * hd), d), _arg(qr, "qr", torch.float32, (T, nHq * hd), d)
+    kp, vp = _arg(k, "k", torch.float32, (T, nKv * hd), d), _arg(v, "v", torch.float32, (T, nKv * hd), d)
+    i = [_arg(t, what, torch.int32, (T,), d) for t, what in ((seq, "seq"), (slot, "slot"), (pos, "pos"))]
+    w = [_arg(t.view(torch.int16), what, torch.int16, (hd,), d) for t, what in ((qw16, "qw16"), (kw16, "kw16"))]
+    c = _ctx(q)
+    c.check(LIB.tb_attn_prep_paged_q8(c.h, ctypes.byref(s), qp, kp, vp, w[0], w[1], op, nHq, T, *i, float(theta),
+                                      float(eps)), "attn_prep_paged_q8")
+    return qr
+
+
+def attention_decode_paged_q8(qr, kv, table, lens, nHq, nKv, hd, window=0, sinks=0, weights=None, out=None):
+    """Attention of one new token a sequence over its pages: qr [batch, nHq*hd], lens int32
+    [batch] (the new token's row included; 0 gives a row of zeros).  window > 0: the last
+    `window` rows and the first `sinks`.  weights f32 [batch, nKv, max_pages*page_rows]: each
+    row's attention weight, summed over the kv head's q heads, is added to it.  Returns f32
+    [batch, nHq*hd]."""
+    d, B = qr.device, table.shape[0]
+    s = _paged(kv, table, nKv, hd, d)
+    if out is None:
+        out = torch.empty((B, nHq * hd), dtype=torch.float32, device=d)
+    qp, op = _arg(qr, "qr", torch.float32, (B, nHq * hd), d), _arg(out, "out", torch.float32, (B, nHq * hd), d)
+    lp = _arg(lens, "lens", torch.int32, (B,), d)
+    wp = None if weights is None else _arg(weights, "weights", torch.float32, (B, nKv, s.max_pages * s.page_rows), d)
+    c = _ctx(qr)
+    ws, n = _workspace(c, "attn_decode_paged_ws", LIB.tb_attn_decode_paged_ws, d, ctypes.byref(s), nHq,
+                       0 if weights is None else 1)
+    c.check(LIB.tb_attn_decode_paged_q8(c.h, ctypes.byref(s), op, qp, lp, nHq, int(window), int(sinks), wp,
+                                        ws.data_ptr(), n), "attn_decode_paged_q8")
+    return out
+
+
+def attention_prefill_paged_q8(q, kv, table, cu, lens, nHq, nKv, hd, window=0, sinks=0, out=None):
+    """Causal attention of packed prompts or chunks: rows cu[b] .. cu[b+1]-1 (int32 [batch+1]) of
+    q [T, nHq*hd] are the last rows of sequence b, which holds lens[b] rows; window and sinks as
+    in attention_decode_paged_q8.  Returns bf16 [T, nHq*hd] (gemm_q's X); rows outside
+    cu[0] .. cu[batch] are left as they were."""
+    d, B, T = q.device, table.shape[0], q.shape[0]
+    s = _paged(kv, table, nKv, hd, d)
+    if out is None:
+        out = torch.empty((T, nHq * hd), dtype=torch.bfloat16, device=d)
+    qp, op = _arg(q, "q", torch.float32, (T, nHq * hd), d), _arg(out, "out", torch.bfloat16, (T, nHq * hd), d)
+    cp, lp = _arg(cu, "cu", torch.int32, (B + 1,), d), _arg(lens, "lens", torch.int32, (B,), d)
+    c = _ctx(q)
+    ws, n = _workspace(c, "attn_prefill_paged_ws", LIB.tb_attn_prefill_paged_ws, d, ctypes.byref(s), nHq, T)
+    c.check(LIB.tb_attn_prefill_paged_q8(c.h, ctypes.byref(s), op, qp, cp, lp, nHq, T, int(window), int(sinks),
+                                         ws.data_ptr(), n), "attn_prefill_paged_q8")
+    return out
+
+
+def kv_evict_paged_q8(kv, table, lens, weights, new_table, budget, sinks, recent, nKv, hd, kv_out=None):
+    """Shrinks every sequence to at most `budget` rows: the first `sinks`, the last `recent`, then
+    the rows with the largest weights summed over kv heads (weights f32 [batch, nKv,
+    max_pages*page_rows], as attention_decode_paged_q8 adds them up; ties go to the lower row).
+    The rows are copied in order into new_table's pages (of kv, or of the pools kv_out; none of
+    them a page that is read).  Returns (kept int32 [batch, budget], the old row of each new one, -1
+    behind the last; lens int32 [batch]; weights f32 [batch, nKv, new rows], zero behind the last)."""
+    d, B = table.device, table.shape[0]
+    s = _paged(kv, table, nKv, hd, d)
+    t = _paged(kv if kv_out is None else kv_out, new_table, nKv, hd, d, "kv_out")
+    lp = _arg(lens, "lens", torch.int32, (B,), d)
+    wp = _arg(weights, "weights", torch.float32, (B, nKv, s.max_pages * s.page_rows), d)
+    if t.batch != B:
+        raise TabInferError("new_table must have %d rows" % B)
+    if budget < 0:
+        raise TabInferError("budget must not be negative")
+    kept = torch.empty((B, int(budget)), dtype=torch.int32, device=d)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=d)
+    new_weights = torch.empty((B, nKv, t.max_pages * t.page_rows), dtype=torch.float32, device=d)
+    c = _ctx(table)
+    ws, n = _workspace(c, "kv_evict_paged_ws", LIB.tb_kv_evict_paged_ws, d, ctypes.byref(s))
+    c.check(LIB.tb_kv_evict_paged_q8(c.h, ctypes.byref(s), ctypes.byref(t), lp, wp, kept.data_ptr(),
+                                     new_lens.data_ptr(), new_weights.data_ptr(), int(budget), int(sinks),
+                                     int(recent), ws.data_ptr(), n), "kv_evict_paged_q8")
+    return kept, new_lens, new_weights
 
 
 # --------------------------------------------------------------------------
