@@ -15,6 +15,8 @@ namespace {
 // length or a row outside the table, a chunk longer than its sequence
 constexpr int ERR_PAGED_PAGE = 0x6c01;
 constexpr int ERR_PAGED_LEN = 0x6c02;
+// a bounded wait on a copy or an MMA of the CTA's own gave up
+constexpr int ERR_PAGED_WAIT = 0x6c03;
 
 constexpr int KT = 32;   // keys a tile: a tile starts on a multiple of KT rows
 
@@ -66,6 +68,44 @@ struct SeenTiles {
 __device__ __forceinline__ bool key_seen(int key, int pos, int window, int sinks)
 {
     return key <= pos && (window <= 0 || pos - key < window || key < sinks);
+}
+
+// ---- mbarriers and asynchronous copies -------------------------------------------
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint64_t* b, unsigned count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* b)
+{
+    asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}" ::"r"(smem_u32(b)) : "memory");
+}
+// Waits until the phase of this parity has completed; at most WAIT_TRIES tries of up to
+// 1 ms each, after which (or when *abort is up) it returns false.
+constexpr int WAIT_TRIES = 1000;
+__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, volatile int* abort = nullptr)
+{
+    const uint32_t a = smem_u32(b);
+    for (int it = 0; it < WAIT_TRIES; it++) {
+        uint32_t done;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+                     " selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done) : "r"(a), "r"(parity), "r"(1000000u) : "memory");
+        if (done) return true;
+        if (abort && *abort) return false;
+    }
+    return false;
+}
+// a box of a 2-D tensor map into shared memory (x: a multiple of 16 bytes)
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar)
+{
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+                 : "memory");
 }
 
 // makes a context's device the current one for a call's launches

@@ -19,6 +19,7 @@ namespace {
 constexpr int W = 4, NT = 32 * W;
 
 struct DecArgs {
+    CUtensorMap mk, mv;    // Kq / Vq as bytes [pool rows][nKv*HD], boxes of min(32, page_rows) rows x HD
     PagedArgs kv;
     const float* q;        // [B][nHq*HD]
     float* out;            // [B][nHq*HD]
@@ -29,7 +30,7 @@ struct DecArgs {
     float2* ML;            // [B][nHq] final (m, l), when weights are wanted
     float* weights;        // [B][nKv][cap]
     int nHq, window, sinks, grid;
-    float qscale;          // log2(e) / sqrt(HD)
+    float qscale;          // log2(e) / (127 sqrt(HD))
 };
 
 __device__ __forceinline__ SeenTiles seen_of(const DecArgs& a, int n) { return SeenTiles(n - 1, n - 1, a.window, a.sinks); }
@@ -38,153 +39,434 @@ __device__ __forceinline__ int chunks_of(const DecArgs& a, int b)
     return (seen_of(a, a.kv.checked_len(__ldg(a.lens + b))).count + W - 1) / W;
 }
 
-// Sums of the sequences' chunk counts, by all NT threads: returns the total; the thread
-// whose slice of sequences holds chunk index `at` (in units of one kv head's chunks when
-// nKv = 1) finds its sequence.  before(b) sums: pass find_b >= 0 to get the sum below
-// sequence find_b in *below, else the sequence holding unit `at` of the nKv-fold list.
+// Where a unit stands.  A unit is a chunk of a (sequence, kv head) pair; they are numbered by
+// sequence, then head, then chunk.
 struct Where {
     long long total;   // chunks of one kv head over all sequences
-    int b;             // the sequence found
-    long long below;   // chunks of one kv head in the sequences below b
+    long long below;   // those of the sequences before b
+    int b;
 };
-__device__ Where locate(const DecArgs& a, int find_b, long long per_of, long long cta)
+// By all NT threads: the sequence find_b (when >= 0), else the one that holds unit cta * per,
+// per = the units a CTA of `grid`.  buf: 8 * W + 32 bytes of shared memory.
+__device__ Where locate(const DecArgs& a, int find_b, long long cta, void* buf)
 {
-    __shared__ long long sums[NT];
-    __shared__ Where found;
+    long long* sums = static_cast<long long*>(buf);
+    Where* found = reinterpret_cast<Where*>(sums + W);
     const int tid = threadIdx.x, B = a.kv.batch, slice = (B + NT - 1) / NT;
     const int b0 = min(B, tid * slice), b1 = min(B, b0 + slice);
     long long mine = 0;
     for (int b = b0; b < b1; b++) mine += chunks_of(a, b);
-    sums[tid] = mine;
-    __syncthreads();
-    if (B > slice) {      // more than one slice in use: inclusive scan
-        for (int o = 1; o < NT; o <<= 1) {
-            const long long v = tid >= o ? sums[tid - o] : 0;
-            __syncthreads();
-            sums[tid] += v;
-            __syncthreads();
-        }
-    } else if (tid > 0) {
-        sums[tid] = sums[0];
+    // inclusive sums over the threads: within warps, then across
+    long long x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, x, o);
+        if ((tid & 31) >= o) x += v;
     }
+    if ((tid & 31) == 31) sums[tid >> 5] = x;
     __syncthreads();
-    const long long total = sums[NT - 1];
-    // the unit looked for, in chunks of the nKv-fold list
-    const long long all = total * a.kv.nKv;
-    const long long per = per_of > 0 ? (all + per_of - 1) / per_of : 0;
-    const long long at = cta * per;
-    if (tid == 0) found = Where{total, -1, 0};
-    __syncthreads();
-    long long below = sums[tid] - mine;
+    long long total = 0;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        if (i < (tid >> 5)) x += sums[i];
+        total += sums[i];
+    }
+    const long long all = total * a.kv.nKv, at = cta * ((all + a.grid - 1) / a.grid);
+    long long below = x - mine;
     if (find_b >= 0) {
         if (b0 <= find_b && find_b < b1) {
             for (int b = b0; b < find_b; b++) below += chunks_of(a, b);
-            found = Where{total, find_b, below};
+            *found = Where{total, below, find_b};
         }
-    } else if (at < all && below * a.kv.nKv <= at && at < (below + mine) * a.kv.nKv) {
+    } else if (at < all ? below * a.kv.nKv <= at && at < (below + mine) * a.kv.nKv : tid == 0) {
         int b = b0;
-        for (; b < b1; b++) {
+        for (; at < all && b < b1; b++) {
             const int n = chunks_of(a, b);
             if (at < (below + n) * a.kv.nKv) break;
             below += n;
         }
-        found = Where{total, b, below};
+        *found = Where{total, below, b};
     }
     __syncthreads();
-    return found;
+    const Where w = *found;
+    __syncthreads();       // buf may be written again
+    return w;
 }
 
+// Shared memory of a CTA: every warp has its own ring of NST tiles (K and V rows by TMA,
+// swizzled; the keys' scales behind them) and words through which scores and weights pass
+// between lanes, q's digits at a part's start and the outputs at its end.
 template <int HD, int GRP>
-__global__ void __launch_bounds__(NT) k_paged_decode(const DecArgs a)
+struct RingLayout {
+    static constexpr int NG = HD / 32, NN = (GRP * 4 + 7) / 8;   // 32-groups; 8-column tiles of (head, digit)
+    static constexpr int ROWS = KT * HD, SCALES = KT * NG * 4;
+    static constexpr int V = ROWS, KS = 2 * ROWS, VS = 2 * ROWS + SCALES;
+    static constexpr int STAGE = 2 * ROWS + 2 * SCALES;          // 9216 or 4608: whole swizzle atoms
+    static constexpr int NST = GRP <= 2 || HD == 64 ? 3 : 2;     // tiles in flight a warp
+    static constexpr int WORDS = GRP * HD * 4;                   // [GRP][NG][KT] words = [GRP][HD] floats
+    static constexpr int OFF_WORDS = W * NST * STAGE;
+    static constexpr int OFF_QF = OFF_WORDS + W * WORDS;         // float [GRP] steps of q's digits
+    static constexpr int OFF_M = (OFF_QF + GRP * 4 + 15) / 16 * 16;   // float [2][W][GRP] m and l
+    static constexpr int OFF_BAR = OFF_M + 2 * W * GRP * 4;      // mbarriers, then the tiles' masks
+    static constexpr int BYTES = OFF_BAR + W * NST * 12;
+    // CTAs an SM: 232448 bytes of shared memory, 1 KB of them a CTA the system's
+    static constexpr int OCC = 232448 / (BYTES + 1024) < 4 ? 232448 / (BYTES + 1024) : 4;
+    static_assert(OCC >= 2, "two CTAs an SM");
+    static_assert(GRP * 4 * HD <= W * WORDS, "q's digits fit in the words");
+    static_assert(W * WORDS >= W * 8 + 32, "the plan's sums fit in the words");
+    static_assert(STAGE % (HD == 128 ? 1024 : 512) == 0 && OFF_BAR % 8 == 0, "alignment");
+};
+
+// A warp's walk over its tiles, pair after pair of the CTA's range of units.
+struct Walk {
+    long long u, u1, base;     // first unit of the current part, end of the range, units below sequence b
+    int b, h, n, c0, c1, nc, i, t1;
+    SeenTiles seen;
+
+    __device__ Walk(const DecArgs& a, long long u0, long long u1_, int b_, long long base_, int wid)
+        : u(u0), u1(u1_), base(base_), b(b_), seen(-1, -1, 0, 0)
+    {
+        load(a);
+        enter(a, wid);
+    }
+    __device__ void load(const DecArgs& a)
+    {
+        n = a.kv.checked_len(__ldg(a.lens + b));
+        seen = seen_of(a, n);
+        nc = (seen.count + W - 1) / W;
+    }
+    __device__ void enter(const DecArgs& a, int wid)
+    {
+        if (u >= u1) return;
+        while (u >= base + (long long)nc * a.kv.nKv) {
+            base += (long long)nc * a.kv.nKv;
+            b++;
+            load(a);
+        }
+        h = (int)((u - base) / nc);
+        c0 = (int)((u - base) % nc);
+        c1 = (int)min((long long)nc, c0 + (u1 - u));
+        i = c0 * W + wid;
+        t1 = min(seen.count, c1 * W);
+    }
+    __device__ bool part() const { return u < u1; }
+    __device__ bool tile() const { return i < t1; }
+    __device__ void next_part(const DecArgs& a, int wid)
+    {
+        u += c1 - c0;
+        enter(a, wid);
+    }
+    // the warp's next tile, in this part or a later one
+    __device__ void advance(const DecArgs& a, int wid)
+    {
+        i += W;
+        settle(a, wid);
+    }
+    __device__ void settle(const DecArgs& a, int wid)
+    {
+        while (part() && !tile()) next_part(a, wid);
+    }
+};
+
+__device__ __forceinline__ float redux_max(float v)
 {
-    __shared__ float qs[GRP][HD];
-    __shared__ float wo[W][GRP][HD];
-    __shared__ float wm[W][GRP], wl[W][GRP];
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, make_float2(0.0f, 0.0f)); }
+
+// What bounds it is HBM, so the arithmetic on each byte has to be short.  Both products run
+// on the tensor cores with the cache's bytes as they are and exact int32 sums, 32 keys at a
+// time (mma m16n8k32, one 32-group of q . k or 32 keys of p . v an instruction):
+//   scores   A = K bytes (16 keys x 32 dims), B = q as four signed base-128 digits of one step
+//            a head (|error| < 2^-28 of the largest |q|), columns (head, digit);
+//   outputs  A = V bytes transposed (16 dims x 32 keys, ldmatrix.trans), B = the keys' weights
+//            p * vscale as three unsigned base-256 digits of a power-of-two step that the tile's
+//            largest weight sets (|error| <= 2^-22 of it), columns (head, digit).
+// The int32 sums stay below 2^22, so they are seeded with 1.5 * 2^23 and read as floats.
+// About 300 instructions a 32-key tile of 9.2 KB (hd 128, two q heads), against some 1600
+// issue slots that the tile's share of the HBM rate leaves an SM; the form that converts V
+// and K to f32 takes 1180.
+template <int HD, int GRP>
+__global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ DecArgs a)
+{
+    using L = RingLayout<HD, GRP>;
+    constexpr int NG = L::NG, NN = L::NN, NST = L::NST;
+    constexpr float MAGIC = 12582912.0f;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
+    uint8_t* ring = smem + wid * NST * L::STAGE;
+    uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_WORDS + wid * L::WORDS);
+    int8_t* qd = reinterpret_cast<int8_t*>(smem + L::OFF_WORDS);     // [GRP][4][HD]
+    float* qf = reinterpret_cast<float*>(smem + L::OFF_QF);
+    float* wo = reinterpret_cast<float*>(smem + L::OFF_WORDS);       // [W][GRP][HD]
+    float* wm = reinterpret_cast<float*>(smem + L::OFF_M);
+    float* wl = wm + W * GRP;
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + wid * NST;
+    uint32_t* okw = reinterpret_cast<uint32_t*>(smem + L::OFF_BAR + W * NST * 8) + wid * NST;
+    if (lane == 0) {
+        for (int s = 0; s < NST; s++) mbar_init(&full[s], 33);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
     tb_pdl_wait();
     tb_pdl_trigger();
-    constexpr int NG = HD / 32, DPL = HD / 32;
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const int nKv = a.kv.nKv, nHq = a.nHq, cta = blockIdx.x;
-    const Where w = locate(a, -1, a.grid, cta);
+    const Where w = locate(a, -1, cta, smem + L::OFF_WORDS);
     const long long all = w.total * nKv, per = (all + a.grid - 1) / a.grid;
     const long long u0 = cta * per, u1 = min(all, u0 + per);
     if (u0 >= u1) return;
-    int b = w.b;
-    long long base = w.below * nKv;          // units below sequence b
-    for (long long u = u0; u < u1;) {
-        const int n = a.kv.checked_len(__ldg(a.lens + b));
-        const SeenTiles seen = seen_of(a, n);
-        const int nc = (seen.count + W - 1) / W;
-        if (u >= base + (long long)nc * nKv) {
-            base += (long long)nc * nKv;
-            b++;
-            continue;
+
+    const int box = min(KT, 1 << a.kv.log_page);          // rows a copy
+    // the tile at the walk's place -> ring stage s
+    auto issue = [&](const Walk& p, int s) {
+        const int key = p.seen.tile(p.i) * KT + lane;
+        const bool see = key_seen(key, p.n - 1, a.window, a.sinks);
+        const unsigned any = __ballot_sync(0xffffffffu, see);
+        // a page is looked up when one of its rows in this tile is seen
+        const unsigned mine = box == KT ? any : any & (0xffffu << (lane & 16));
+        const int row = mine ? a.kv.row(p.b, key) : -1;
+        const int row16 = __shfl_sync(0xffffffffu, row, 16);
+        const unsigned ok = __ballot_sync(0xffffffffu, see && row >= 0);
+        uint8_t* st = ring + s * L::STAGE;
+        if (lane == 0) {
+            okw[s] = ok;
+            const bool second = box < KT && row16 >= 0;
+            mbar_expect_tx(&full[s], (uint32_t)(2 * HD * box * ((row >= 0) + second)));
+            if (row >= 0) {
+                tma_2d(st, &a.mk, p.h * HD, row, &full[s]);
+                tma_2d(st + L::V, &a.mv, p.h * HD, row, &full[s]);
+            }
+            if (second) {
+                tma_2d(st + 16 * HD, &a.mk, p.h * HD, row16, &full[s]);
+                tma_2d(st + L::V + 16 * HD, &a.mv, p.h * HD, row16, &full[s]);
+            }
         }
-        const int h = (int)((u - base) / nc), c0 = (int)((u - base) % nc);
-        const int c1 = (int)min((long long)nc, c0 + (u1 - u));
+        if (see && row >= 0) {
+            const long long at = ((long long)row * nKv + p.h) * NG;
+            if constexpr (NG == 4) {
+                cp_async16(st + L::KS + lane * 16, a.kv.Ks + at);
+                cp_async16(st + L::VS + lane * 16, a.kv.Vs + at);
+            } else {
+                cp_async8(st + L::KS + lane * 8, a.kv.Ks + at);
+                cp_async8(st + L::VS + lane * 8, a.kv.Vs + at);
+            }
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+    };
+    Walk c(a, u0, u1, w.b, w.below * nKv, wid), p = c;
+    p.settle(a, wid);
+    int issued = 0, used = 0;
+    bool alive = true;
+    for (; issued < NST && p.part(); issued++) {
+        issue(p, issued);
+        p.advance(a, wid);
+    }
+    const float f1 = (t4 & 1) ? 0.0f : 256.0f, f2 = (t4 & 1) ? 65536.0f : 1.0f;
+    const int lrow = (lane & 7) + (lane & 8), lchunk = lane >> 4;    // ldmatrix x4: 16 rows x two chunks
+    auto swz = [](int row, int chunk) {
+        return HD == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+    };
+
+    for (; c.part(); c.next_part(a, wid)) {
+        // ---- q of this pair: four signed digits, one step a head
+        __syncthreads();       // the last part's merge and digits are read
+        for (int g = wid; g < GRP; g += W) {
+            const float* src = a.q + (long long)c.b * nHq * HD + (c.h * GRP + g) * HD;
+            float r[NG], mx = 0.0f;
+            bool fine = true;
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                r[i] = __ldg(src + 32 * i + lane);
+                mx = fmaxf(mx, fabsf(r[i]));
+                fine = fine && fabsf(r[i]) <= 3.0e38f;
+            }
+            mx = warp_max(mx);
+            fine = __all_sync(0xffffffffu, fine);
+            float stp = mx > 1e-30f ? mx * (1.0f / 127.0f) : 1.0f;
+            if (lane == 0) qf[g] = fine ? stp * a.qscale : __int_as_float(0x7fc00000);
+            float inv = __frcp_rn(stp);
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    const int x = max(-127, min(127, __float2int_rn(r[i] * inv)));
+                    r[i] = fmaf(-stp, (float)x, r[i]);
+                    qd[(g * 4 + d) * HD + 32 * i + lane] = (int8_t)x;
+                }
+                stp *= 0.0078125f;
+                inv *= 128.0f;
+            }
+        }
         __syncthreads();
-        for (int i = tid; i < GRP * HD; i += NT)
-            qs[i / HD][i % HD] = a.q[(long long)b * nHq * HD + h * GRP * HD + i] * a.qscale;
-        __syncthreads();
-        float m[GRP], l[GRP], o[GRP][DPL];
+        uint32_t qb[NN][NG][2];
+        float qs[NN];
+#pragma unroll
+        for (int nt = 0; nt < NN; nt++) {
+            const int col = 8 * nt + g8, hd_ = 2 * nt + (t4 >> 1);
+#pragma unroll
+            for (int G = 0; G < NG; G++) {
+                const int8_t* src = qd + col * HD + 32 * G + 4 * t4;
+                qb[nt][G][0] = col < 4 * GRP ? *reinterpret_cast<const uint32_t*>(src) : 0u;
+                qb[nt][G][1] = col < 4 * GRP ? *reinterpret_cast<const uint32_t*>(src + 16) : 0u;
+            }
+            qs[nt] = hd_ < GRP ? qf[hd_] * ((t4 & 1) ? 1.0f / 16384.0f : 1.0f) : 0.0f;
+        }
+        __syncthreads();       // the digits are read: their words take scores and weights
+        float m[GRP], l[GRP];
+        float2 o[2 * NG][NN];      // (dims 16 mt + g8, + 8) of head 2 nt + t4 / 2, digits of this lane
 #pragma unroll
         for (int g = 0; g < GRP; g++) {
             m[g] = NEG_BIG;
             l[g] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < DPL; i++) o[g][i] = 0.0f;
         }
-        const int t1 = min(seen.count, c1 * W);
-        for (int i = c0 * W + wid; i < t1; i += W) {
-            const int key = seen.tile(i) * KT + lane;
-            bool ok = key_seen(key, n - 1, a.window, a.sinks);
-            int row = ok ? a.kv.row(b, key) : -1;
-            ok = row >= 0;
-            const long long at = (long long)(ok ? row : 0) * nKv * HD + h * HD;
-            float s[GRP];
 #pragma unroll
-            for (int g = 0; g < GRP; g++) s[g] = 0.0f;
-            if (ok) {
+        for (int i = 0; i < 2 * NG; i++)
+#pragma unroll
+            for (int nt = 0; nt < NN; nt++) o[i][nt] = make_float2(0.0f, 0.0f);
+
+        for (; c.tile() && alive; c.i += W, used++) {
+            const int s = used % NST;
+            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (used / NST) & 1))) {
+                if (lane == 0) atomicExch(a.kv.err, ERR_PAGED_WAIT);
+                alive = false;
+                break;
+            }
+            const uint8_t* st = ring + s * L::STAGE;
+            const uint32_t kb = smem_u32(st), vb = kb + L::V;
+            const bool ok = (okw[s] >> lane) & 1;
+            const float* ks = reinterpret_cast<const float*>(st + L::KS);
+            float* scs = reinterpret_cast<float*>(words);
+            // ---- scores
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++) {
+                float2 part[NN];
+#pragma unroll
+                for (int nt = 0; nt < NN; nt++) part[nt] = make_float2(0.0f, 0.0f);
+                float k0[NG], k1[NG];
+#pragma unroll
+                for (int i = 0; i < NG; i += 2) {
+                    *reinterpret_cast<float2*>(k0 + i) = *reinterpret_cast<const float2*>(ks + (16 * mt + g8) * NG + i);
+                    *reinterpret_cast<float2*>(k1 + i) = *reinterpret_cast<const float2*>(ks + (16 * mt + g8 + 8) * NG + i);
+                }
+#pragma unroll
                 for (int G = 0; G < NG; G++) {
-                    float part[GRP];
+                    uint32_t af[4];
+                    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(af[0]), "=r"(af[1]), "=r"(af[2]), "=r"(af[3])
+                                 : "r"(kb + swz(16 * mt + lrow, 2 * G + lchunk)));
 #pragma unroll
-                    for (int g = 0; g < GRP; g++) part[g] = 0.0f;
-                    for (int d = 0; d < 32; d++) {
-                        const float x = (float)a.kv.Kq[at + 32 * G + d];
-#pragma unroll
-                        for (int g = 0; g < GRP; g++) part[g] = fmaf(x, qs[g][32 * G + d], part[g]);
+                    for (int nt = 0; nt < NN; nt++) {
+                        int d[4];
+                        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                            "{%8,%9}, {%10,%10,%10,%10};"
+                            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                            : "r"(af[0]), "r"(af[1]), "r"(af[2]), "r"(af[3]), "r"(qb[nt][G][0]), "r"(qb[nt][G][1]),
+                              "r"(0x4B400000));
+                        const float2 hi = fadd2(make_float2(__int_as_float(d[0]), __int_as_float(d[2])),
+                                                make_float2(-MAGIC, -MAGIC));
+                        const float2 lo = fadd2(make_float2(__int_as_float(d[1]), __int_as_float(d[3])),
+                                                make_float2(-MAGIC, -MAGIC));
+                        part[nt] = ffma2(ffma2(lo, make_float2(0.0078125f, 0.0078125f), hi), make_float2(k0[G], k1[G]),
+                                         part[nt]);
                     }
-                    const float sc = a.kv.Ks[at / 32 + G] * (1.0f / 127.0f);
+                }
 #pragma unroll
-                    for (int g = 0; g < GRP; g++) s[g] = fmaf(part[g], sc, s[g]);
+                for (int nt = 0; nt < NN; nt++) {
+                    float x = part[nt].x * qs[nt], y = part[nt].y * qs[nt];
+                    x += __shfl_xor_sync(0xffffffffu, x, 1);
+                    y += __shfl_xor_sync(0xffffffffu, y, 1);
+                    const int hd_ = 2 * nt + (t4 >> 1);
+                    if ((t4 & 1) == 0 && hd_ < GRP) {
+                        scs[hd_ * KT + 16 * mt + g8] = x;
+                        scs[hd_ * KT + 16 * mt + g8 + 8] = y;
+                    }
                 }
             }
-            float p[GRP];
+            __syncwarp();
+            float pr[GRP], corr[GRP];
+#pragma unroll
+            for (int g = 0; g < GRP; g++) pr[g] = ok ? scs[g * KT + lane] : NEG_BIG;
+            __syncwarp();
+            if (a.SC) {
+                const int key = c.seen.tile(c.i) * KT + lane;
+                if (key < a.kv.cap()) {
+                    float* dst = a.SC + (((long long)c.b * nKv + c.h) * a.kv.cap() + key) * GRP;
+#pragma unroll
+                    for (int g = 0; g < GRP; g++) dst[g] = ok ? pr[g] : -INFINITY;
+                }
+            }
+            // ---- running maximum and sum (m the same in every lane, l per lane)
 #pragma unroll
             for (int g = 0; g < GRP; g++) {
-                const float x = ok ? s[g] : NEG_BIG;
-                const float mn = fmaxf(m[g], warp_max(x)), corr = exp2f(m[g] - mn);
-                p[g] = ok ? exp2f(x - mn) : 0.0f;
-                l[g] = fmaf(l[g], corr, p[g]);
+                const float mn = fmaxf(m[g], redux_max(pr[g]));
+                corr[g] = exp2f(m[g] - mn);
+                pr[g] = ok ? exp2f(pr[g] - mn) : 0.0f;
+                l[g] = fmaf(l[g], corr[g], pr[g]);
                 m[g] = mn;
-#pragma unroll
-                for (int j = 0; j < DPL; j++) o[g][j] *= corr;
-                if (a.SC && key < a.kv.cap())
-                    a.SC[(((long long)b * nKv + h) * a.kv.cap() + key) * GRP + g] = ok ? x : -INFINITY;
             }
-            for (int k = 0; k < KT; k++) {
-                const int r = __shfl_sync(0xffffffffu, row, k);
-                float pk[GRP];
+            // ---- the keys' weights a V group, as integers of a power-of-two step
+            float sc[GRP][NG];
+            {
+                float vs[NG];
 #pragma unroll
-                for (int g = 0; g < GRP; g++) pk[g] = __shfl_sync(0xffffffffu, p[g], k);
-                if (r < 0) continue;
-                const long long va = (long long)r * nKv * HD + h * HD;
+                for (int i = 0; i < NG; i += 2)
+                    *reinterpret_cast<float2*>(vs + i) =
+                        *reinterpret_cast<const float2*>(st + L::VS + (lane * NG + i) * 4);
 #pragma unroll
-                for (int j = 0; j < DPL; j++) {      // lane holds dims 32 j + lane
-                    const float v = (float)a.kv.Vq[va + 32 * j + lane] * (a.kv.Vs[va / 32 + j] * (1.0f / 127.0f));
+                for (int G = 0; G < NG; G++)
 #pragma unroll
-                    for (int g = 0; g < GRP; g++) o[g][j] = fmaf(pk[g], v, o[g][j]);
+                    for (int g = 0; g < GRP; g++) {
+                        const float x = ok ? pr[g] * vs[G] : 0.0f;
+                        const int e = max(24, (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(x)) >> 23));
+                        sc[g][G] = e > 250 ? __int_as_float(0x7fc00000) : __int_as_float((e - 21) << 23);   // 2^(e - 127 - 21)
+                        words[(g * NG + G) * KT + lane] =
+                            __float_as_uint(fmaf(x, __int_as_float((275 - min(e, 250)) << 23), 8388608.0f));
+                    }
+            }
+            __syncwarp();
+            // ---- outputs
+#pragma unroll
+            for (int nt = 0; nt < NN; nt++) {
+                const int hb = 2 * nt + (g8 >> 2), sel = (g8 & 3) | ((4 + (g8 & 3)) << 4);
+                // this lane's output columns belong to head 2 nt + t4 / 2
+                const float cr = 2 * nt + 1 < GRP && (t4 >> 1) ? corr[(2 * nt + 1) % GRP] : corr[2 * nt];
+                const float2 cr2 = make_float2(cr, cr);
+#pragma unroll
+                for (int G = 0; G < NG; G++) {
+                    uint32_t b0 = 0, b1 = 0;
+                    if (hb < GRP) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(words + (hb * NG + G) * KT + 4 * t4);
+                        const uint4 y = *reinterpret_cast<const uint4*>(words + (hb * NG + G) * KT + 16 + 4 * t4);
+                        b0 = __byte_perm(__byte_perm(x.x, x.y, sel), __byte_perm(x.z, x.w, sel), 0x5410);
+                        b1 = __byte_perm(__byte_perm(y.x, y.y, sel), __byte_perm(y.z, y.w, sel), 0x5410);
+                    }
+                    const float so = (2 * nt + 1 < GRP && (t4 >> 1) ? sc[(2 * nt + 1) % GRP][G] : sc[2 * nt][G]) * f2;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        const int mt = 2 * G + k;
+                        uint32_t af[4];
+                        int d[4];
+                        asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(af[0]), "=r"(af[1]), "=r"(af[2]), "=r"(af[3]) : "r"(vb + swz(lane, mt)));
+                        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+                            "{%8,%9}, {%10,%10,%10,%10};"
+                            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+                            : "r"(af[0]), "r"(af[1]), "r"(af[2]), "r"(af[3]), "r"(b0), "r"(b1), "r"(0x4B400000));
+                        const float2 lo = fadd2(make_float2(__int_as_float(d[0]), __int_as_float(d[2])),
+                                                make_float2(-MAGIC, -MAGIC));
+                        const float2 hi = fadd2(make_float2(__int_as_float(d[1]), __int_as_float(d[3])),
+                                                make_float2(-MAGIC, -MAGIC));
+                        o[mt][nt] = ffma2(ffma2(hi, make_float2(f1, f1), lo), make_float2(so, so), mul2(o[mt][nt], cr2));
+                    }
                 }
+            }
+            __syncwarp();          // the stage and the words are read
+            if (p.part()) {
+                issue(p, s);
+                issued++;
+                p.advance(a, wid);
             }
         }
         // ---- the warps' states meet
@@ -192,46 +474,60 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const DecArgs a)
         for (int g = 0; g < GRP; g++) {
             const float lt = warp_sum(l[g]);
             if (lane == 0) {
-                wm[wid][g] = m[g];
-                wl[wid][g] = lt;
+                wm[wid * GRP + g] = m[g];
+                wl[wid * GRP + g] = lt;
             }
-#pragma unroll
-            for (int j = 0; j < DPL; j++) wo[wid][g][32 * j + lane] = o[g][j];
         }
+#pragma unroll
+        for (int nt = 0; nt < NN; nt++)
+#pragma unroll
+            for (int mt = 0; mt < 2 * NG; mt++) {
+                const float x = o[mt][nt].x + __shfl_xor_sync(0xffffffffu, o[mt][nt].x, 1);
+                const float y = o[mt][nt].y + __shfl_xor_sync(0xffffffffu, o[mt][nt].y, 1);
+                const int hd_ = 2 * nt + (t4 >> 1);
+                if ((t4 & 1) == 0 && hd_ < GRP) {
+                    wo[(wid * GRP + hd_) * HD + 16 * mt + g8] = x;
+                    wo[(wid * GRP + hd_) * HD + 16 * mt + g8 + 8] = y;
+                }
+            }
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == nc;
-        const long long slot = 2LL * cta + (u == u0 ? 0 : 1);
+        const bool whole = c.c0 == 0 && c.c1 == c.nc;
+        const long long slot = 2LL * cta + (c.u == u0 ? 0 : 1);
         for (int i = tid; i < GRP * HD; i += NT) {
             const int g = i / HD, d = i % HD;
-            float M = NEG_BIG, L = 0.0f, O = 0.0f;
+            float M = NEG_BIG, Ls = 0.0f, O = 0.0f;
 #pragma unroll
-            for (int k = 0; k < W; k++) M = fmaxf(M, wm[k][g]);
+            for (int k = 0; k < W; k++) M = fmaxf(M, wm[k * GRP + g]);
 #pragma unroll
             for (int k = 0; k < W; k++) {
-                const float e = exp2f(wm[k][g] - M);
-                L = fmaf(wl[k][g], e, L);
-                O = fmaf(wo[k][g][d], e, O);
+                const float e = exp2f(wm[k * GRP + g] - M);
+                Ls = fmaf(wl[k * GRP + g], e, Ls);
+                O = fmaf(wo[(k * GRP + g) * HD + d], e, O);
             }
+            O *= 1.0f / 127.0f;
             if (whole) {
-                a.out[(long long)b * nHq * HD + (h * GRP + g) * HD + d] = L > 0.0f ? O / L : 0.0f;
-                if (d == 0 && a.ML) a.ML[(long long)b * nHq + h * GRP + g] = make_float2(M, L);
+                a.out[(long long)c.b * nHq * HD + (c.h * GRP + g) * HD + d] = Ls > 0.0f || Ls != Ls ? O / Ls : 0.0f;
+                if (d == 0 && a.ML) a.ML[(long long)c.b * nHq + c.h * GRP + g] = make_float2(M, Ls);
             } else {
                 a.PO[(slot * GRP + g) * HD + d] = O;
-                if (d == 0) a.PML[slot * GRP + g] = make_float2(M, L);
+                if (d == 0) a.PML[slot * GRP + g] = make_float2(M, Ls);
             }
         }
-        u += c1 - c0;
     }
+    // after a wait that gave up: no copy may land once the CTA has left
+    if (!alive)
+        for (int i = used; i < issued; i++) mbar_wait(&full[i % NST], (i / NST) & 1);
 }
 
 // joins the parts of pair (kv head x, sequence y); pairs that one CTA held are done
 template <int HD, int GRP>
-__global__ void __launch_bounds__(NT) k_paged_combine(const DecArgs a)
+__global__ void __launch_bounds__(NT) k_paged_combine(const __grid_constant__ DecArgs a)
 {
     tb_pdl_wait();
     tb_pdl_trigger();
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, nKv = a.kv.nKv;
-    const Where w = locate(a, b, a.grid, 0);
+    __shared__ __align__(16) uint8_t plan[W * 8 + 32];
+    const Where w = locate(a, b, 0, plan);
     const int nc = chunks_of(a, b);
     float* out = a.out + (long long)b * a.nHq * HD + h * GRP * HD;
     if (nc == 0) {
@@ -255,14 +551,14 @@ __global__ void __launch_bounds__(NT) k_paged_combine(const DecArgs a)
             L = fmaf(ml.y, e, L);
             O = fmaf(a.PO[(s * GRP + g) * HD + d], e, O);
         }
-        out[i] = L > 0.0f ? O / L : 0.0f;
+        out[i] = L > 0.0f || L != L ? O / L : 0.0f;
         if (d == 0 && a.ML) a.ML[(long long)b * a.nHq + h * GRP + g] = make_float2(M, L);
     }
 }
 
 // weights[b][h][j] += sum over the group of 2^(s - m) / l, for the keys seen
 template <int GRP>
-__global__ void __launch_bounds__(256) k_paged_weights(const DecArgs a)
+__global__ void __launch_bounds__(256) k_paged_weights(const __grid_constant__ DecArgs a)
 {
     tb_pdl_wait();
     tb_pdl_trigger();
@@ -294,12 +590,19 @@ struct DecWs {
     size_t bytes() const { return po + pml + ml + sc; }
 };
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+int dec_occ(int64_t hd, int64_t grp)
+{
+    if (hd == 64) return grp <= 2 ? (grp == 1 ? RingLayout<64, 1>::OCC : RingLayout<64, 2>::OCC)
+                                  : (grp == 4 ? RingLayout<64, 4>::OCC : RingLayout<64, 8>::OCC);
+    return grp <= 2 ? (grp == 1 ? RingLayout<128, 1>::OCC : RingLayout<128, 2>::OCC)
+                    : (grp == 4 ? RingLayout<128, 4>::OCC : RingLayout<128, 8>::OCC);
+}
 DecWs dec_ws(const tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, bool weights)
 {
     const int64_t cap = kv->max_pages * kv->page_rows, grp = nHq / kv->nKv;
     const int64_t chunks = kv->batch * kv->nKv * ((cap + KT * W - 1) / (KT * W));
     DecWs w{};
-    w.grid = (int)std::min<int64_t>(chunks, 4LL * ctx->num_sms);
+    w.grid = (int)std::min<int64_t>(chunks, (int64_t)dec_occ(kv->hd, grp) * ctx->num_sms);
     w.po = up256((size_t)w.grid * 2 * grp * kv->hd * sizeof(float));
     w.pml = up256((size_t)w.grid * 2 * grp * sizeof(float2));
     if (weights) {
@@ -312,7 +615,15 @@ DecWs dec_ws(const tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, bool weights
 template <int HD, int GRP>
 int launch_decode(tb_ctx* ctx, const DecArgs& a)
 {
-    cudaError_t e = tb_launch(ctx, k_paged_decode<HD, GRP>, dim3(a.grid), dim3(NT), 0, a);
+    auto kern = k_paged_decode<HD, GRP>;
+    constexpr int smem = RingLayout<HD, GRP>::BYTES;
+    static bool attr_set[64] = {};   // per device and instantiation; setting it twice is harmless
+    cudaError_t e = cudaSuccess;
+    if (ctx->device >= 64 || !attr_set[ctx->device]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess && ctx->device < 64) attr_set[ctx->device] = true;
+    }
+    if (e == cudaSuccess) e = tb_launch(ctx, kern, dim3(a.grid), dim3(NT), (size_t)smem, a);
     if (e == cudaSuccess) e = tb_launch(ctx, k_paged_combine<HD, GRP>, dim3(a.kv.nKv, a.kv.batch), dim3(NT), 0, a);
     if (e == cudaSuccess && a.weights)
         e = tb_launch(ctx, k_paged_weights<GRP>,
@@ -372,7 +683,13 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, float* ou
     a.window = (int)std::min<int64_t>(window, 1LL << 30);
     a.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
     a.grid = w.grid;
-    a.qscale = 1.4426950408889634f / sqrtf((float)kv->hd);
+    a.qscale = 1.4426950408889634f / (127.0f * sqrtf((float)kv->hd));
+    const int64_t cols = kv->nKv * kv->hd, rows = kv->n_pages * kv->page_rows;
+    const int box = (int)std::min<int64_t>(KT, kv->page_rows);
+    const CUtensorMapSwizzle swz = kv->hd == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    rc = tb_encode_2d(ctx, &a.mk, kv->Kq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, cols, rows, (int)kv->hd, box, swz);
+    if (!rc) rc = tb_encode_2d(ctx, &a.mv, kv->Vq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, cols, rows, (int)kv->hd, box, swz);
+    if (rc) return rc;
     switch ((int)(kv->hd * 10 + nHq / kv->nKv)) {
     case 641: return launch_decode<64, 1>(ctx, a);
     case 642: return launch_decode<64, 2>(ctx, a);
