@@ -5,18 +5,23 @@
 //   s_j = q . k_j / sqrt(hd) over the keys seen;  p = softmax(s);  out = sum_j p_j v_j
 //   weights[b][kv head][j] += sum over the head's group of p_j
 //
-// The keys seen are a list of 32-key tiles; W consecutive tiles are a chunk, and the
-// chunks of all (sequence, kv head) pairs in order are dealt out evenly to the CTAs, so
-// ragged batches and long single sequences fill the machine alike.  A CTA whose range
-// holds only a part of a pair's chunks writes (m, l, o) for it (at most two such parts a
-// CTA: its first and its last pair); k_paged_combine joins a pair's parts in order, so
-// results do not depend on timing.
+// The keys seen are a list of 32-key tiles.  The W warps of a CTA take HG neighbouring kv
+// heads of W / HG consecutive tiles (a chunk), HG = 4, 2 or 1, the most that divides the
+// heads: a cache row holds its heads side by side, so the CTA reads 512 contiguous bytes a
+// row (one head a CTA left 128-byte pieces, and the 16-byte pieces of the scales, to CTAs
+// that came by at other times: 505 MB from DRAM for a cache of 302 MB).  The chunks of all
+// (sequence, head group) pairs in order are dealt out evenly to the CTAs, so ragged batches
+// and long single sequences fill the machine alike.  A CTA whose range holds only a part of
+// a pair's chunks writes (m, l, o) for it (at most two such parts a CTA: its first and its
+// last pair); k_paged_combine joins a pair's parts in order, so results do not depend on
+// timing.
 #include "tb_attn_dev.cuh"
 #include "tb_paged.cuh"
 
 namespace {
 
 constexpr int W = 4, NT = 32 * W;
+constexpr int CT = 512;    // threads of a joining CTA
 
 struct DecArgs {
     CUtensorMap mk, mv;    // Kq / Vq as bytes [pool rows][nKv*HD], boxes of min(32, page_rows) rows x HD
@@ -24,72 +29,84 @@ struct DecArgs {
     const float* q;        // [B][nHq*HD]
     float* out;            // [B][nHq*HD]
     const int* lens;       // [B]
-    float* PO;             // [grid][2][GRP][HD]
-    float2* PML;           // [grid][2][GRP]
+    float* PO;             // [grid][2][HG][GRP][HD]
+    float2* PML;           // [grid][2][HG][GRP]
     float* SC;             // [B][nKv][cap][GRP] scores (log2), when weights are wanted
     float2* ML;            // [B][nHq] final (m, l), when weights are wanted
     float* weights;        // [B][nKv][cap]
     int nHq, window, sinks, grid;
+    int log_hg;            // heads a group
     float qscale;          // log2(e) / (127 sqrt(HD))
 };
 
 __device__ __forceinline__ SeenTiles seen_of(const DecArgs& a, int n) { return SeenTiles(n - 1, n - 1, a.window, a.sinks); }
 __device__ __forceinline__ int chunks_of(const DecArgs& a, int b)
 {
-    return (seen_of(a, a.kv.checked_len(__ldg(a.lens + b))).count + W - 1) / W;
+    const int tw = W >> a.log_hg;      // tiles a chunk
+    return (seen_of(a, a.kv.checked_len(__ldg(a.lens + b))).count + tw - 1) / tw;
 }
 
-// Where a unit stands.  A unit is a chunk of a (sequence, kv head) pair; they are numbered by
-// sequence, then head, then chunk.
+// Where a unit stands.  A unit is a chunk of a (sequence, head group) pair; they are numbered
+// by sequence, then group, then chunk (below 2^31 in all).
 struct Where {
-    long long total;   // chunks of one kv head over all sequences
-    long long below;   // those of the sequences before b
+    int total;   // chunks of one group over all sequences
+    int below;   // those of the sequences before b
     int b;
 };
-// By all NT threads: the sequence find_b (when >= 0), else the one that holds unit cta * per,
-// per = the units a CTA of `grid`.  buf: 8 * W + 32 bytes of shared memory.
-__device__ Where locate(const DecArgs& a, int find_b, long long cta, void* buf)
+// The sequence find_b (when >= 0), else the one that holds unit cta * per, per = the units a
+// CTA of `grid`.  Up to 32 sequences every warp finds it by itself; more take all threads and
+// buf, (NT / 32 + 3) words of shared memory.
+__device__ Where locate(const DecArgs& a, int find_b, int cta, int* buf)
 {
-    long long* sums = static_cast<long long*>(buf);
-    Where* found = reinterpret_cast<Where*>(sums + W);
-    const int tid = threadIdx.x, B = a.kv.batch, slice = (B + NT - 1) / NT;
-    const int b0 = min(B, tid * slice), b1 = min(B, b0 + slice);
-    long long mine = 0;
+    const int B = a.kv.batch, groups = a.kv.nKv >> a.log_hg;
+    if (B == 1) return Where{chunks_of(a, 0), 0, 0};
+    const int nt = B <= 32 ? 32 : (int)blockDim.x, tid = B <= 32 ? threadIdx.x & 31 : threadIdx.x;
+    const int slice = (B + nt - 1) / nt, b0 = min(B, tid * slice), b1 = min(B, b0 + slice);
+    int mine = 0;
     for (int b = b0; b < b1; b++) mine += chunks_of(a, b);
-    // inclusive sums over the threads: within warps, then across
-    long long x = mine;
+    int x = mine;                                   // inclusive sums over the threads
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, x, o);
+        const int v = __shfl_up_sync(0xffffffffu, x, o);
         if ((tid & 31) >= o) x += v;
     }
-    if ((tid & 31) == 31) sums[tid >> 5] = x;
-    __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int i = 0; i < W; i++) {
-        if (i < (tid >> 5)) x += sums[i];
-        total += sums[i];
+    int total = __shfl_sync(0xffffffffu, x, 31);
+    if (nt > 32) {
+        if ((tid & 31) == 31) buf[tid >> 5] = x;
+        __syncthreads();
+        total = 0;
+        for (int i = 0; i < nt / 32; i++) {
+            if (i < (tid >> 5)) x += buf[i];
+            total += buf[i];
+        }
     }
-    const long long all = total * a.kv.nKv, at = cta * ((all + a.grid - 1) / a.grid);
-    long long below = x - mine;
+    const int all = total * groups, at = cta * ((all + a.grid - 1) / a.grid);
+    Where w{total, x - mine, b0};
+    bool here;
     if (find_b >= 0) {
-        if (b0 <= find_b && find_b < b1) {
-            for (int b = b0; b < find_b; b++) below += chunks_of(a, b);
-            *found = Where{total, below, find_b};
-        }
-    } else if (at < all ? below * a.kv.nKv <= at && at < (below + mine) * a.kv.nKv : tid == 0) {
-        int b = b0;
-        for (; at < all && b < b1; b++) {
-            const int n = chunks_of(a, b);
-            if (at < (below + n) * a.kv.nKv) break;
-            below += n;
-        }
-        *found = Where{total, below, b};
+        here = b0 <= find_b && find_b < b1;
+        if (here)
+            for (; w.b < find_b; w.b++) w.below += chunks_of(a, w.b);
+    } else {
+        here = at < all && w.below * groups <= at && at < (w.below + mine) * groups;
+        if (here)
+            for (int n; at >= (w.below + (n = chunks_of(a, w.b))) * groups; w.b++) w.below += n;
+    }
+    if (nt == 32) {
+        const int src = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+        w.below = __shfl_sync(0xffffffffu, w.below, max(src, 0));
+        w.b = __shfl_sync(0xffffffffu, w.b, max(src, 0));
+        return w;
+    }
+    int* out = buf + nt / 32;
+    if (here) {
+        out[0] = w.below;
+        out[1] = w.b;
     }
     __syncthreads();
-    const Where w = *found;
-    __syncthreads();       // buf may be written again
+    w.below = out[0];                               // not read where no unit is left
+    w.b = out[1];
+    __syncthreads();                                // buf may be written again
     return w;
 }
 
@@ -105,25 +122,24 @@ struct RingLayout {
     static constexpr int NST = GRP <= 2 || HD == 64 ? 3 : 2;     // tiles in flight a warp
     static constexpr int WORDS = GRP * HD * 4;                   // [GRP][NG][KT] words = [GRP][HD] floats
     static constexpr int OFF_WORDS = W * NST * STAGE;
-    static constexpr int OFF_QF = OFF_WORDS + W * WORDS;         // float [GRP] steps of q's digits
-    static constexpr int OFF_M = (OFF_QF + GRP * 4 + 15) / 16 * 16;   // float [2][W][GRP] m and l
+    static constexpr int OFF_M = OFF_WORDS + W * WORDS;          // float [2][W][GRP] m and l
     static constexpr int OFF_BAR = OFF_M + 2 * W * GRP * 4;      // mbarriers, then the tiles' masks
     static constexpr int BYTES = OFF_BAR + W * NST * 12;
     // CTAs an SM: 232448 bytes of shared memory, 1 KB of them a CTA the system's
     static constexpr int OCC = 232448 / (BYTES + 1024) < 4 ? 232448 / (BYTES + 1024) : 4;
     static_assert(OCC >= 2, "two CTAs an SM");
-    static_assert(GRP * 4 * HD <= W * WORDS, "q's digits fit in the words");
-    static_assert(W * WORDS >= W * 8 + 32, "the plan's sums fit in the words");
+    static_assert(GRP * 4 * HD <= WORDS, "q's digits fit in the words");
+    static_assert(W * WORDS >= (W + 3) * 4, "the plan's sums fit in the words");
     static_assert(STAGE % (HD == 128 ? 1024 : 512) == 0 && OFF_BAR % 8 == 0, "alignment");
 };
 
 // A warp's walk over its tiles, pair after pair of the CTA's range of units.
 struct Walk {
-    long long u, u1, base;     // first unit of the current part, end of the range, units below sequence b
-    int b, h, n, c0, c1, nc, i, t1;
+    int u, u1, base;           // first unit of the current part, end of the range, units below sequence b
+    int b, grp, n, c0, c1, nc, i, t1;
     SeenTiles seen;
 
-    __device__ Walk(const DecArgs& a, long long u0, long long u1_, int b_, long long base_, int wid)
+    __device__ Walk(const DecArgs& a, int u0, int u1_, int b_, int base_, int wid)
         : u(u0), u1(u1_), base(base_), b(b_), seen(-1, -1, 0, 0)
     {
         load(a);
@@ -131,26 +147,29 @@ struct Walk {
     }
     __device__ void load(const DecArgs& a)
     {
+        const int tw = W >> a.log_hg;
         n = a.kv.checked_len(__ldg(a.lens + b));
         seen = seen_of(a, n);
-        nc = (seen.count + W - 1) / W;
+        nc = (seen.count + tw - 1) / tw;
     }
     __device__ void enter(const DecArgs& a, int wid)
     {
         if (u >= u1) return;
-        while (u >= base + (long long)nc * a.kv.nKv) {
-            base += (long long)nc * a.kv.nKv;
+        const int groups = a.kv.nKv >> a.log_hg, tw = W >> a.log_hg;
+        while (u >= base + nc * groups) {
+            base += nc * groups;
             b++;
             load(a);
         }
-        h = (int)((u - base) / nc);
-        c0 = (int)((u - base) % nc);
-        c1 = (int)min((long long)nc, c0 + (u1 - u));
-        i = c0 * W + wid;
-        t1 = min(seen.count, c1 * W);
+        grp = (u - base) / nc;
+        c0 = (u - base) - grp * nc;
+        c1 = min(nc, c0 + (u1 - u));
+        i = c0 * tw + (wid >> a.log_hg);
+        t1 = min(seen.count, c1 * tw);
     }
     __device__ bool part() const { return u < u1; }
     __device__ bool tile() const { return i < t1; }
+    __device__ int head(const DecArgs& a, int wid) const { return (grp << a.log_hg) + (wid & ((1 << a.log_hg) - 1)); }
     __device__ void next_part(const DecArgs& a, int wid)
     {
         u += c1 - c0;
@@ -159,7 +178,7 @@ struct Walk {
     // the warp's next tile, in this part or a later one
     __device__ void advance(const DecArgs& a, int wid)
     {
-        i += W;
+        i += W >> a.log_hg;
         settle(a, wid);
     }
     __device__ void settle(const DecArgs& a, int wid)
@@ -198,8 +217,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5, g8 = lane >> 2, t4 = lane & 3;
     uint8_t* ring = smem + wid * NST * L::STAGE;
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_WORDS + wid * L::WORDS);
-    int8_t* qd = reinterpret_cast<int8_t*>(smem + L::OFF_WORDS);     // [GRP][4][HD]
-    float* qf = reinterpret_cast<float*>(smem + L::OFF_QF);
+    int8_t* qd = reinterpret_cast<int8_t*>(words);                   // [GRP][4][HD]
     float* wo = reinterpret_cast<float*>(smem + L::OFF_WORDS);       // [W][GRP][HD]
     float* wm = reinterpret_cast<float*>(smem + L::OFF_M);
     float* wl = wm + W * GRP;
@@ -212,16 +230,16 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     __syncwarp();
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int nKv = a.kv.nKv, nHq = a.nHq, cta = blockIdx.x;
-    const Where w = locate(a, -1, cta, smem + L::OFF_WORDS);
-    const long long all = w.total * nKv, per = (all + a.grid - 1) / a.grid;
-    const long long u0 = cta * per, u1 = min(all, u0 + per);
+    const int nKv = a.kv.nKv, nHq = a.nHq, cta = blockIdx.x, hg = 1 << a.log_hg, tw = W >> a.log_hg;
+    const Where w = locate(a, -1, cta, reinterpret_cast<int*>(smem + L::OFF_WORDS));
+    const int all = w.total * (nKv >> a.log_hg), per = (all + a.grid - 1) / a.grid;
+    const int u0 = cta * per, u1 = min(all, u0 + per);
     if (u0 >= u1) return;
 
     const int box = min(KT, 1 << a.kv.log_page);          // rows a copy
     // the tile at the walk's place -> ring stage s
     auto issue = [&](const Walk& p, int s) {
-        const int key = p.seen.tile(p.i) * KT + lane;
+        const int key = p.seen.tile(p.i) * KT + lane, ph = p.head(a, wid);
         const bool see = key_seen(key, p.n - 1, a.window, a.sinks);
         const unsigned any = __ballot_sync(0xffffffffu, see);
         // a page is looked up when one of its rows in this tile is seen
@@ -235,16 +253,16 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
             const bool second = box < KT && row16 >= 0;
             mbar_expect_tx(&full[s], (uint32_t)(2 * HD * box * ((row >= 0) + second)));
             if (row >= 0) {
-                tma_2d(st, &a.mk, p.h * HD, row, &full[s]);
-                tma_2d(st + L::V, &a.mv, p.h * HD, row, &full[s]);
+                tma_2d(st, &a.mk, ph * HD, row, &full[s]);
+                tma_2d(st + L::V, &a.mv, ph * HD, row, &full[s]);
             }
             if (second) {
-                tma_2d(st + 16 * HD, &a.mk, p.h * HD, row16, &full[s]);
-                tma_2d(st + L::V + 16 * HD, &a.mv, p.h * HD, row16, &full[s]);
+                tma_2d(st + 16 * HD, &a.mk, ph * HD, row16, &full[s]);
+                tma_2d(st + L::V + 16 * HD, &a.mv, ph * HD, row16, &full[s]);
             }
         }
         if (see && row >= 0) {
-            const long long at = ((long long)row * nKv + p.h) * NG;
+            const long long at = ((long long)row * nKv + ph) * NG;
             if constexpr (NG == 4) {
                 cp_async16(st + L::KS + lane * 16, a.kv.Ks + at);
                 cp_async16(st + L::VS + lane * 16, a.kv.Vs + at);
@@ -255,7 +273,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
     };
-    Walk c(a, u0, u1, w.b, w.below * nKv, wid), p = c;
+    Walk c(a, u0, u1, w.b, w.below * (nKv >> a.log_hg), wid), p = c;
     p.settle(a, wid);
     int issued = 0, used = 0;
     bool alive = true;
@@ -270,10 +288,13 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     };
 
     for (; c.part(); c.next_part(a, wid)) {
-        // ---- q of this pair: four signed digits, one step a head
-        __syncthreads();       // the last part's merge and digits are read
-        for (int g = wid; g < GRP; g += W) {
-            const float* src = a.q + (long long)c.b * nHq * HD + (c.h * GRP + g) * HD;
+        // ---- q of this warp's head: four signed digits, one step a q head
+        const int h = c.head(a, wid);
+        if (tw > 1) __syncthreads();       // the last part's merge has read the words
+        float qf[GRP];
+#pragma unroll
+        for (int g = 0; g < GRP; g++) {
+            const float* src = a.q + (long long)c.b * nHq * HD + (h * GRP + g) * HD;
             float r[NG], mx = 0.0f;
             bool fine = true;
 #pragma unroll
@@ -282,10 +303,10 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
                 mx = fmaxf(mx, fabsf(r[i]));
                 fine = fine && fabsf(r[i]) <= 3.0e38f;
             }
-            mx = warp_max(mx);
+            mx = redux_max(mx);
             fine = __all_sync(0xffffffffu, fine);
             float stp = mx > 1e-30f ? mx * (1.0f / 127.0f) : 1.0f;
-            if (lane == 0) qf[g] = fine ? stp * a.qscale : __int_as_float(0x7fc00000);
+            qf[g] = fine ? stp * a.qscale : __int_as_float(0x7fc00000);
             float inv = __frcp_rn(stp);
 #pragma unroll
             for (int d = 0; d < 4; d++) {
@@ -299,21 +320,21 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
                 inv *= 128.0f;
             }
         }
-        __syncthreads();
+        __syncwarp();
         uint32_t qb[NN][NG][2];
         float qs[NN];
 #pragma unroll
         for (int nt = 0; nt < NN; nt++) {
-            const int col = 8 * nt + g8, hd_ = 2 * nt + (t4 >> 1);
+            const int col = 8 * nt + g8;
 #pragma unroll
             for (int G = 0; G < NG; G++) {
                 const int8_t* src = qd + col * HD + 32 * G + 4 * t4;
                 qb[nt][G][0] = col < 4 * GRP ? *reinterpret_cast<const uint32_t*>(src) : 0u;
                 qb[nt][G][1] = col < 4 * GRP ? *reinterpret_cast<const uint32_t*>(src + 16) : 0u;
             }
-            qs[nt] = hd_ < GRP ? qf[hd_] * ((t4 & 1) ? 1.0f / 16384.0f : 1.0f) : 0.0f;
+            qs[nt] = (2 * nt + 1 < GRP && (t4 >> 1) ? qf[(2 * nt + 1) % GRP] : qf[2 * nt]) * ((t4 & 1) ? 1.0f / 16384.0f : 1.0f);
         }
-        __syncthreads();       // the digits are read: their words take scores and weights
+        __syncwarp();          // the digits are read: their words take scores and weights
         float m[GRP], l[GRP];
         float2 o[2 * NG][NN];      // (dims 16 mt + g8, + 8) of head 2 nt + t4 / 2, digits of this lane
 #pragma unroll
@@ -326,7 +347,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
 #pragma unroll
             for (int nt = 0; nt < NN; nt++) o[i][nt] = make_float2(0.0f, 0.0f);
 
-        for (; c.tile() && alive; c.i += W, used++) {
+        for (; c.tile() && alive; c.i += tw, used++) {
             const int s = used % NST;
             if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (used / NST) & 1))) {
                 if (lane == 0) atomicExch(a.kv.err, ERR_PAGED_WAIT);
@@ -392,7 +413,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
             if (a.SC) {
                 const int key = c.seen.tile(c.i) * KT + lane;
                 if (key < a.kv.cap()) {
-                    float* dst = a.SC + (((long long)c.b * nKv + c.h) * a.kv.cap() + key) * GRP;
+                    float* dst = a.SC + (((long long)c.b * nKv + h) * a.kv.cap() + key) * GRP;
 #pragma unroll
                     for (int g = 0; g < GRP; g++) dst[g] = ok ? pr[g] : -INFINITY;
                 }
@@ -469,7 +490,8 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
                 p.advance(a, wid);
             }
         }
-        // ---- the warps' states meet
+        // ---- the states of a head's warps meet
+        __syncwarp();
 #pragma unroll
         for (int g = 0; g < GRP; g++) {
             const float lt = warp_sum(l[g]);
@@ -490,69 +512,115 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
                     wo[(wid * GRP + hd_) * HD + 16 * mt + g8 + 8] = y;
                 }
             }
-        __syncthreads();
+        if (tw > 1) __syncthreads();
+        else __syncwarp();
         const bool whole = c.c0 == 0 && c.c1 == c.nc;
-        const long long slot = 2LL * cta + (c.u == u0 ? 0 : 1);
-        for (int i = tid; i < GRP * HD; i += NT) {
+        const long long slot = ((2LL * cta + (c.u == u0 ? 0 : 1)) << a.log_hg) + (wid & (hg - 1));
+        // the tw warps of a head share its outputs
+        for (int i = (wid >> a.log_hg) * 32 + lane; i < GRP * HD; i += 32 * tw) {
             const int g = i / HD, d = i % HD;
             float M = NEG_BIG, Ls = 0.0f, O = 0.0f;
-#pragma unroll
-            for (int k = 0; k < W; k++) M = fmaxf(M, wm[k * GRP + g]);
-#pragma unroll
-            for (int k = 0; k < W; k++) {
+            for (int k = wid & (hg - 1); k < W; k += hg) M = fmaxf(M, wm[k * GRP + g]);
+            for (int k = wid & (hg - 1); k < W; k += hg) {
                 const float e = exp2f(wm[k * GRP + g] - M);
                 Ls = fmaf(wl[k * GRP + g], e, Ls);
                 O = fmaf(wo[(k * GRP + g) * HD + d], e, O);
             }
             O *= 1.0f / 127.0f;
             if (whole) {
-                a.out[(long long)c.b * nHq * HD + (c.h * GRP + g) * HD + d] = Ls > 0.0f || Ls != Ls ? O / Ls : 0.0f;
-                if (d == 0 && a.ML) a.ML[(long long)c.b * nHq + c.h * GRP + g] = make_float2(M, Ls);
+                a.out[(long long)c.b * nHq * HD + (h * GRP + g) * HD + d] = Ls > 0.0f || Ls != Ls ? O / Ls : 0.0f;
+                if (d == 0 && a.ML) a.ML[(long long)c.b * nHq + h * GRP + g] = make_float2(M, Ls);
             } else {
                 a.PO[(slot * GRP + g) * HD + d] = O;
                 if (d == 0) a.PML[slot * GRP + g] = make_float2(M, Ls);
             }
         }
+        __syncwarp();
     }
     // after a wait that gave up: no copy may land once the CTA has left
     if (!alive)
         for (int i = used; i < issued; i++) mbar_wait(&full[i % NST], (i / NST) & 1);
 }
 
-// joins the parts of pair (kv head x, sequence y); pairs that one CTA held are done
+// Joins the parts of kv head x of sequence y; those that one CTA held are done.  The parts'
+// factors 2^(m - M) come first (in shared memory), then each thread sums a float4 column of
+// every CT-th part, eight loads in flight, and the CT sums are added in order.
 template <int HD, int GRP>
-__global__ void __launch_bounds__(NT) k_paged_combine(const __grid_constant__ DecArgs a)
+__global__ void __launch_bounds__(CT) k_paged_combine(const __grid_constant__ DecArgs a)
 {
+    constexpr int COLS = GRP * HD / 4, P = CT / COLS;
+    static_assert(CT % COLS == 0 && CT / 32 >= GRP, "whole columns, a warp a q head");
+    extern __shared__ __align__(16) float fac[];     // [np][GRP]
+    __shared__ float4 part[P][COLS];
+    __shared__ float sl[GRP];
+    __shared__ int plan[CT / 32 + 3];
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, nKv = a.kv.nKv;
-    __shared__ __align__(16) uint8_t plan[W * 8 + 32];
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
     const Where w = locate(a, b, 0, plan);
-    const int nc = chunks_of(a, b);
-    float* out = a.out + (long long)b * a.nHq * HD + h * GRP * HD;
+    const int nc = chunks_of(a, b), groups = a.kv.nKv >> a.log_hg, hg = 1 << a.log_hg;
+    float4* out = reinterpret_cast<float4*>(a.out + (long long)b * a.nHq * HD + h * GRP * HD);
     if (nc == 0) {
-        for (int i = tid; i < GRP * HD; i += NT) out[i] = 0.0f;
+        if (tid < COLS) out[tid] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         return;
     }
-    const long long all = w.total * nKv, per = (all + a.grid - 1) / a.grid;
-    const long long u0 = w.below * nKv + (long long)h * nc, u1 = u0 + nc;
-    const long long c0 = u0 / per, c1 = (u1 - 1) / per;
+    const int all = w.total * groups, per = (all + a.grid - 1) / a.grid;
+    const int u0 = w.below * groups + (h >> a.log_hg) * nc, u1 = u0 + nc;
+    const int c0 = u0 / per, c1 = (u1 - 1) / per;
     if (c0 == c1) return;
-    const long long s0 = 2 * c0 + (u0 == c0 * per ? 0 : 1);
-    for (int i = tid; i < GRP * HD; i += NT) {
-        const int g = i / HD, d = i % HD;
-        float M = a.PML[s0 * GRP + g].x;
-        for (long long c = c0 + 1; c <= c1; c++) M = fmaxf(M, a.PML[2 * c * GRP + g].x);
-        float L = 0.0f, O = 0.0f;
-        for (long long c = c0; c <= c1; c++) {
-            const long long s = c == c0 ? s0 : 2 * c;
-            const float2 ml = a.PML[s * GRP + g];
-            const float e = exp2f(ml.x - M);
-            L = fmaf(ml.y, e, L);
-            O = fmaf(a.PO[(s * GRP + g) * HD + d], e, O);
+    // part k is CTA c0 + k's: its first part, but for a pair that starts inside CTA c0's range
+    const int first = u0 == c0 * per ? 0 : 1, np = c1 - c0 + 1;
+    auto slot = [&](int k) { return (size_t)((2 * (c0 + k) + (k == 0 ? first : 0)) * hg + (h & (hg - 1))) * GRP; };
+    if (wid < GRP) {
+        float x = NEG_BIG;
+        for (int k = lane; k < np; k += 32) x = fmaxf(x, a.PML[slot(k) + wid].x);
+        x = warp_max(x);
+        float l = 0.0f;
+        for (int k = lane; k < np; k += 32) {
+            const float2 ml = a.PML[slot(k) + wid];
+            const float e = exp2f(ml.x - x);
+            fac[k * GRP + wid] = e;
+            l = fmaf(ml.y, e, l);
         }
-        out[i] = L > 0.0f || L != L ? O / L : 0.0f;
-        if (d == 0 && a.ML) a.ML[(long long)b * a.nHq + h * GRP + g] = make_float2(M, L);
+        l = warp_sum(l);
+        if (lane == 0) {
+            sl[wid] = l;
+            if (a.ML) a.ML[(long long)b * a.nHq + h * GRP + wid] = make_float2(x, l);
+        }
+    }
+    __syncthreads();
+    const int col = tid % COLS, pp = tid / COLS, g = col / (HD / 4);
+    const float4* po = reinterpret_cast<const float4*>(a.PO) + col;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = pp; k < np; k += 8 * P) {
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (k + i * P < np) v[i] = po[slot(k + i * P) * (HD / 4)];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            if (k + i * P < np) {
+                const float e = fac[(k + i * P) * GRP + g];
+                o.x = fmaf(v[i].x, e, o.x);
+                o.y = fmaf(v[i].y, e, o.y);
+                o.z = fmaf(v[i].z, e, o.z);
+                o.w = fmaf(v[i].w, e, o.w);
+            }
+    }
+    part[pp][col] = o;
+    __syncthreads();
+    if (tid < COLS) {
+        o = part[0][tid];
+#pragma unroll
+        for (int i = 1; i < P; i++) {
+            const float4 v = part[i][tid];
+            o.x += v.x;
+            o.y += v.y;
+            o.z += v.z;
+            o.w += v.w;
+        }
+        const float l = sl[g];
+        out[tid] = l > 0.0f || l != l ? make_float4(o.x / l, o.y / l, o.z / l, o.w / l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
 }
 
@@ -590,6 +658,8 @@ struct DecWs {
     size_t bytes() const { return po + pml + ml + sc; }
 };
 size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+// heads a CTA reads side by side
+int log_group(int64_t nKv) { return nKv % 4 == 0 ? 2 : (nKv % 2 == 0 ? 1 : 0); }
 int dec_occ(int64_t hd, int64_t grp)
 {
     if (hd == 64) return grp <= 2 ? (grp == 1 ? RingLayout<64, 1>::OCC : RingLayout<64, 2>::OCC)
@@ -600,11 +670,12 @@ int dec_occ(int64_t hd, int64_t grp)
 DecWs dec_ws(const tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, bool weights)
 {
     const int64_t cap = kv->max_pages * kv->page_rows, grp = nHq / kv->nKv;
-    const int64_t chunks = kv->batch * kv->nKv * ((cap + KT * W - 1) / (KT * W));
+    const int lhg = log_group(kv->nKv), tw = W >> lhg;
+    const int64_t chunks = kv->batch * (kv->nKv >> lhg) * ((cap + KT * tw - 1) / (KT * tw));
     DecWs w{};
     w.grid = (int)std::min<int64_t>(chunks, (int64_t)dec_occ(kv->hd, grp) * ctx->num_sms);
-    w.po = up256((size_t)w.grid * 2 * grp * kv->hd * sizeof(float));
-    w.pml = up256((size_t)w.grid * 2 * grp * sizeof(float2));
+    w.po = up256(((size_t)w.grid * 2 * grp * kv->hd * sizeof(float)) << lhg);
+    w.pml = up256(((size_t)w.grid * 2 * grp * sizeof(float2)) << lhg);
     if (weights) {
         w.ml = up256((size_t)kv->batch * nHq * sizeof(float2));
         w.sc = up256((size_t)kv->batch * nHq * cap * sizeof(float));
@@ -624,7 +695,7 @@ int launch_decode(tb_ctx* ctx, const DecArgs& a)
         if (e == cudaSuccess && ctx->device < 64) attr_set[ctx->device] = true;
     }
     if (e == cudaSuccess) e = tb_launch(ctx, kern, dim3(a.grid), dim3(NT), (size_t)smem, a);
-    if (e == cudaSuccess) e = tb_launch(ctx, k_paged_combine<HD, GRP>, dim3(a.kv.nKv, a.kv.batch), dim3(NT), 0, a);
+    if (e == cudaSuccess) e = tb_launch(ctx, k_paged_combine<HD, GRP>, dim3(a.kv.nKv, a.kv.batch), dim3(CT), (size_t)a.grid * GRP * 4, a);
     if (e == cudaSuccess && a.weights)
         e = tb_launch(ctx, k_paged_weights<GRP>,
                       dim3(tb_cdiv((long long)a.kv.max_pages << a.kv.log_page, 1024), a.kv.nKv, a.kv.batch), dim3(256), 0, a);
@@ -657,6 +728,8 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, float* ou
     TB_REQUIRE(ctx, out && qr && lens, "null pointer");
     TB_REQUIRE(ctx, TB_ALIGNED(out, 16) && TB_ALIGNED(qr, 16), "q and out must be 16-byte aligned");
     TB_REQUIRE(ctx, window >= 0 && sinks >= 0, "window and sinks must not be negative");
+    TB_REQUIRE(ctx, kv->batch * kv->nKv * (kv->max_pages * kv->page_rows / KT + 1) < (1LL << 31),
+               "batch x heads x rows too large");
     DeviceGuard dev(ctx->device);
     const DecWs w = dec_ws(ctx, kv, nHq, weights != nullptr);
     if (!ws) {
@@ -683,6 +756,7 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, float* ou
     a.window = (int)std::min<int64_t>(window, 1LL << 30);
     a.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
     a.grid = w.grid;
+    a.log_hg = log_group(kv->nKv);
     a.qscale = 1.4426950408889634f / (127.0f * sqrtf((float)kv->hd));
     const int64_t cols = kv->nKv * kv->hd, rows = kv->n_pages * kv->page_rows;
     const int box = (int)std::min<int64_t>(KT, kv->page_rows);
