@@ -50,16 +50,16 @@ struct PagedArgs {
 };
 
 // The keys that the queries at rows p0 .. p1 see between them (key j <= p, and with a
-// window p - j < window or j < sinks): rows [0, sinks) and [lo, p1], as 32-key tiles.
+// window p - j < window or j < sinks): rows [0, sinks) and [lo, p1], as tiles of kt keys.
 struct SeenTiles {
     int first, from, count;   // tiles 0 .. first-1, then from .. from+count-first-1
 
-    __device__ __forceinline__ SeenTiles(int p0, int p1, int window, int sinks)
+    __device__ __forceinline__ SeenTiles(int p0, int p1, int window, int sinks, int kt = KT)
     {
-        const int end = p1 < 0 ? 0 : p1 / KT + 1;
+        const int end = p1 < 0 ? 0 : p1 / kt + 1;
         const int lo = window > 0 && p0 >= window ? p0 - window + 1 : 0;
-        from = lo / KT;
-        first = min(from, (min(sinks, lo) + KT - 1) / KT);
+        from = lo / kt;
+        first = min(from, (min(sinks, lo) + kt - 1) / kt);
         count = first + max(0, end - from);
     }
     __device__ __forceinline__ int tile(int i) const { return i < first ? i : from + i - first; }

@@ -1,17 +1,54 @@
 // tb_paged_prefill.cu -- attention of packed prompts or chunks of prompts over the paged
-// int8 KV cache: causal, GQA, a sliding window with first tokens kept.
+// int8 KV cache on the 5th-generation tensor cores: causal, GQA, a sliding window with
+// first tokens kept.
 //
 // Rows cu[b] .. cu[b+1]-1 of q are the last t_b = cu[b+1]-cu[b] rows of sequence b; query i
-// stands at row n_b - t_b + i.  One CTA a (query, kv head): each warp takes 32-key tiles
-// with its own running maximum and sum, and the warps meet at the end.
+// stands at row n_b - t_b + i.
+//
+// An item is 256 / GRP consecutive queries of a sequence and one kv head: with the group's
+// q heads that is two 128-row tiles of S = Q K^T, so a dequantized K / V tile serves 256
+// rows.  The 128-key tiles that an item's queries see are its work; items with more than
+// their share (all tiles / SMs) are cut into parts, whose (m, l, O) a joining kernel merges
+// in order.  k_prefill_plan (one CTA) lists the parts by length; the persistent CTAs (one an
+// SM) take them in boustrophedon order.
+//
+// Warp roles of k_paged_prefill (512 threads):
+//   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread a row: S from TMEM, P (f16) back
+//                    over it; the reference maximum is raised (and O rescaled in TMEM) only
+//                    when a score passes it by 2^8, so O is hardly ever touched; Q of the
+//                    next part into shared memory, then the part's outputs
+//   warps 8-11       K / V tiles: 16-byte loads a tile ahead, bytes -> f16 (one exact step,
+//                    one multiplication by the group's scale) into swizzled tiles
+//   warp 12          TMEM and the MMAs: S_t = Q_t K^T (both K-major), O_t += P_t V (P from
+//                    TMEM, V MN-major as it lies in the cache), row tile 0 and 1 in turn so
+//                    that one's softmax runs under the other's MMAs
+// Roundings: Q, dequantized K and V (and their scales) and P to f16, relative 2^-11 each; S,
+// the statistics and O in f32.
+// Every wait is bounded: one that gives up sets the error word and the CTA's abort flag, all
+// roles leave, the MMA thread waits for its last commit and TMEM is freed.
 #include <cuda_bf16.h>
 
-#include "tb_attn_dev.cuh"
 #include "tb_paged.cuh"
 
 namespace {
 
-constexpr int W = 4, NT = 32 * W;
+constexpr int PK = 128;                  // keys a tile
+constexpr int ROWS = 256;                // rows an item: two tiles of 128
+constexpr int THREADS = 512;
+constexpr int KV_STAGES = 2;
+constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps their sums in shared memory)
+constexpr int MIN_TILES = 2;             // an item is not cut below this many tiles a part
+constexpr float RAISE = 8.0f;            // log2 by which a score may pass the reference maximum
+
+struct Part {
+    int b, row0, nq, p0;                 // sequence, first packed row, queries, row of the first in the sequence
+    int t0, t1;                          // its tiles in the item's list
+    int slot;                            // partial slot, -1: the item whole
+    int pad;
+};
+struct Item {
+    int row0, nq, slot0, parts;
+};
 
 struct PrefillArgs {
     PagedArgs kv;
@@ -19,123 +56,766 @@ struct PrefillArgs {
     __nv_bfloat16* out;     // [T][nHq*HD]
     const int* cu;          // [B+1]
     const int* lens;        // [B]
-    int T, nHq, window, sinks;
-    float qscale;
+    int* head;              // parts, items
+    Part* parts;
+    Item* items;
+    float* PO;              // [slot][nKv][ROWS][HD]
+    float2* PML;            // [slot][nKv][ROWS]
+    int T, nHq, grp, window, sinks, sms, max_items, max_parts, max_slots;
+    float sl2;              // log2(e) / sqrt(HD)
 };
 
-template <int HD, int GRP>
-__global__ void __launch_bounds__(NT) k_paged_prefill(const PrefillArgs a)
+// ---- the plan: one CTA ---------------------------------------------------------------
+// Items of a sequence and the sum over all threads of a value
+constexpr int PT = 1024;
+
+__device__ int block_scan(int x, int* buf, int* total)      // inclusive; buf: PT / 32 words
 {
-    __shared__ float qs[GRP][HD];
-    __shared__ float wo[W][GRP][HD];
-    __shared__ float wm[W][GRP], wl[W][GRP];
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += v;
+    }
+    __syncthreads();
+    if (lane == 31) buf[wid] = x;
+    __syncthreads();
+    int all = 0;
+    for (int i = 0; i < PT / 32; i++) {
+        if (i < wid) x += buf[i];
+        all += buf[i];
+    }
+    *total = all;
+    return x;
+}
+
+__global__ void __launch_bounds__(PT) k_prefill_plan(const PrefillArgs a)
+{
+    __shared__ int first[MAX_BATCH + 1];      // items below each sequence
+    __shared__ int buf[PT / 32], hist[PT];
+    __shared__ unsigned long long all_tiles;
     tb_pdl_wait();
     tb_pdl_trigger();
-    constexpr int NG = HD / 32, DPL = HD / 32;
-    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const int nKv = a.kv.nKv, nHq = a.nHq, t = blockIdx.x, h = blockIdx.y;
-    int lo = 0, hi = a.kv.batch;             // the sequence with cu[b] <= t < cu[b+1]
-    if (t < __ldg(a.cu) || t >= __ldg(a.cu + hi)) return;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (__ldg(a.cu + mid) <= t) lo = mid;
-        else hi = mid;
+    const int tid = threadIdx.x, B = a.kv.batch, qb = ROWS / a.grp;
+    int items = 0;
+    for (int b0 = 0; b0 < B; b0 += PT) {
+        const int b = b0 + tid;
+        int n = 0;
+        if (b < B) {
+            const int c0 = a.cu[b], c1 = a.cu[b + 1];
+            if (c0 >= 0 && c1 <= a.T && c1 >= c0) n = (c1 - c0 + qb - 1) / qb;
+            else atomicExch(a.kv.err, ERR_PAGED_LEN);
+        }
+        int all;
+        const int x = block_scan(n, buf, &all);
+        if (b < B) first[b] = items + x - n;
+        items += all;
     }
-    const int b = lo, first = __ldg(a.cu + b), rows = __ldg(a.cu + b + 1) - first;
-    const int n = a.kv.checked_len(__ldg(a.lens + b)), pos = n - rows + t - first;
-    if (pos < 0 && tid == 0) atomicExch(a.kv.err, ERR_PAGED_LEN);
-    for (int i = tid; i < GRP * HD; i += NT)
-        qs[i / HD][i % HD] = a.q[(long long)t * nHq * HD + h * GRP * HD + i] * a.qscale;
+    if (tid == 0) first[B] = items;
+    hist[tid] = 0;
     __syncthreads();
-    float m[GRP], l[GRP], o[GRP][DPL];
-#pragma unroll
-    for (int g = 0; g < GRP; g++) {
-        m[g] = NEG_BIG;
-        l[g] = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DPL; i++) o[g][i] = 0.0f;
+    if (items > a.max_items) {                // overlapping sequences: more rows than q has
+        if (tid == 0) {
+            a.head[0] = a.head[1] = 0;
+            atomicExch(a.kv.err, ERR_PAGED_LEN);
+        }
+        return;
     }
-    const SeenTiles seen(pos, pos, a.window, a.sinks);
-    for (int i = wid; i < seen.count; i += W) {
-        const int key = seen.tile(i) * KT + lane;
-        bool ok = key_seen(key, pos, a.window, a.sinks);
-        const int row = ok ? a.kv.row(b, key) : -1;
-        ok = row >= 0;
-        const long long at = (long long)(ok ? row : 0) * nKv * HD + h * HD;
-        float s[GRP], p[GRP];
+    // the item's queries and tiles
+    auto item = [&](int i, int& b, int& row0, int& nq, int& p0, int& nt) {
+        int lo = 0, hi = B;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= i) lo = mid;
+            else hi = mid;
+        }
+        b = lo;
+        const int c0 = a.cu[b], rows = a.cu[b + 1] - c0, at = (i - first[b]) * qb;
+        const int n = a.kv.checked_len(a.lens[b]);
+        row0 = c0 + at;
+        nq = min(qb, rows - at);
+        p0 = n - rows + at;
+        nt = SeenTiles(max(p0, 0), p0 + nq - 1, a.window, a.sinks, PK).count;
+        if (p0 < 0) atomicExch(a.kv.err, ERR_PAGED_LEN);
+    };
+    unsigned long long tiles = 0;
+    for (int i = tid; i < items; i += PT) {
+        int b, row0, nq, p0, nt;
+        item(i, b, row0, nq, p0, nt);
+        tiles += nt;
+    }
+    if (tid == 0) all_tiles = 0;
+    __syncthreads();
+    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    if ((tid & 31) == 0) atomicAdd(&all_tiles, tiles);
+    __syncthreads();
+    // the longest part: a CTA's share of all heads' tiles
+    const int share = (int)min(1ull << 24, max((unsigned long long)MIN_TILES, (all_tiles * a.kv.nKv + a.sms - 1) / a.sms));
+    const int shift = max(0, 32 - __clz(share) - 10);          // part lengths as at most PT classes
+    for (int i = tid; i < items; i += PT) {
+        int b, row0, nq, p0, nt;
+        item(i, b, row0, nq, p0, nt);
+        const int np = max(1, (nt + share - 1) / share);
+        for (int k = 0; k < np; k++)
+            atomicAdd(&hist[((k + 1) * nt / np - k * nt / np) >> shift], 1);
+    }
+    __syncthreads();
+    // places from the longest class down
+    const int mine = hist[PT - 1 - tid];
+    int parts;
+    const int place = block_scan(mine, buf, &parts) - mine;
+    __syncthreads();
+    hist[PT - 1 - tid] = place;
+    __syncthreads();
+    int slots = 0;
+    for (int i0 = 0; i0 < items; i0 += PT) {
+        const int i = i0 + tid;
+        int b = 0, row0 = 0, nq = 0, p0 = 0, nt = 0, np = 0;
+        if (i < items) {
+            item(i, b, row0, nq, p0, nt);
+            np = max(1, (nt + share - 1) / share);
+        }
+        int all;
+        const int mine_slots = np > 1 ? np : 0;
+        const int s0 = slots + block_scan(mine_slots, buf, &all) - mine_slots;
+        slots += all;
+        if (i >= items) continue;
+        a.items[i] = Item{row0, nq, s0, np};
+        for (int k = 0; k < np; k++) {
+            const int t0 = k * nt / np, t1 = (k + 1) * nt / np;
+            const int at = atomicAdd(&hist[(t1 - t0) >> shift], 1);
+            if (at < a.max_parts) a.parts[at] = Part{b, row0, nq, p0, t0, t1, np > 1 ? s0 + k : -1, 0};
+        }
+    }
+    if (tid == 0) {
+        a.head[0] = min(parts, a.max_parts);
+        a.head[1] = items;
+    }
+}
+
+// ---- the products ---------------------------------------------------------------------
+template <int HD>
+struct PrefillLayout {
+    static constexpr int HALF = 128 * 128;                     // 128 rows x 64 f16, 128-byte swizzle
+    static constexpr int TILE = HALF * (HD / 64);
+    static constexpr int OFF_Q = 0;                            // [2]
+    static constexpr int OFF_K = 2 * TILE;                     // [KV_STAGES]
+    static constexpr int OFF_V = OFF_K + KV_STAGES * TILE;
+    static constexpr int OFF_ROW = OFF_V + KV_STAGES * TILE;   // int [3][PK] pool rows
+    static constexpr int OFF_SC = OFF_ROW + 3 * PK * 4;        // f16 [3][2][PK][4] scales of K and V
+    static constexpr int OFF_BAD = OFF_SC + 3 * 2 * PK * 8;   // uint [8][PK / 32]: keys of pages outside the pool
+    static constexpr int OFF_BAR = OFF_BAD + 8 * PK / 8;
+    static constexpr int BYTES = 1024 + OFF_BAR + 256;
+    static_assert(BYTES <= 227 * 1024, "shared memory");
+};
+// byte offset of 16-byte chunk c (0..7) of row r in a half tile
+__device__ __forceinline__ uint32_t sw128(int r, int c)
+{
+    return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4));
+}
+// K-major operand: 8-row atoms 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr)
+{
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// MN-major operand: atoms of 64 columns x 8 keys, 1024 bytes apart along the keys and HALF
+// bytes along the columns
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr)
+{
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(16384 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16: D f32, A and B f16; B MN-major at bit 16; N >> 3 at bit 17, M >> 4 at bit 24
+constexpr uint32_t idesc(int n, bool bmn)
+{
+    return (1u << 4) | ((bmn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+
+#define TB_R32(r) \
+    "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7]), \
+        "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]), "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]), \
+        "=r"((r)[15]), "=r"((r)[16]), "=r"((r)[17]), "=r"((r)[18]), "=r"((r)[19]), "=r"((r)[20]), "=r"((r)[21]), \
+        "=r"((r)[22]), "=r"((r)[23]), "=r"((r)[24]), "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]), \
+        "=r"((r)[29]), "=r"((r)[30]), "=r"((r)[31])
+// 32 columns of this warp's 32 TMEM lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+                 "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : TB_R32(r) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+                 "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+                   "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+                   "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t* bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                 ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// the k-th (part, head) of CTA c: rounds over the list, every other one backwards
+__device__ __forceinline__ int nth(int k, int c, int grid) { return k * grid + ((k & 1) ? grid - 1 - c : c); }
+
+template <int HD, int GRP>
+__global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_constant__ PrefillArgs a)
+{
+    using L = PrefillLayout<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);     // [2] Q of the part staged
+    uint64_t* k_full = q_full + 2;                                          // [KV_STAGES]
+    uint64_t* k_empty = k_full + KV_STAGES;
+    uint64_t* v_full = k_empty + KV_STAGES;
+    uint64_t* v_empty = v_full + KV_STAGES;
+    uint64_t* s_full = v_empty + KV_STAGES;                                 // [2] S written
+    uint64_t* p_full = s_full + 2;                                          // [2] P written, O rescaled
+    uint64_t* o_done = p_full + 2;                                          // [2] O += P V completed
+    uint64_t* done = o_done + 2;                                            // every MMA completed
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(done + 2);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nKv = a.kv.nKv;
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&q_full[i], 4);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_done[i], 1);
+        }
+        for (int i = 0; i < KV_STAGES; i++) {
+            mbar_init(&k_full[i], 4);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_full[i], 4);
+            mbar_init(&v_empty[i], 1);
+        }
+        mbar_init(done, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32((const void*)tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = *tmem_slot;      // S 0, S 1 (128 columns each), O 0, O 1
+    tb_pdl_wait();
+    tb_pdl_trigger();
+    const int total = a.head[0] * nKv, grid = gridDim.x, cta = blockIdx.x;
+    auto give_up = [&]() {
+        *abort_flag = 1;
+        atomicExch(a.kv.err, ERR_PAGED_WAIT);
+    };
+    // one outcome for the warp: its lanes then run the .aligned instructions together
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+        if (!ok && lane == 0) give_up();
+        __syncwarp();
+        return ok;
+    };
+
+    if (warp < 8) {
+        // =============================== softmax ======================================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        const int t = warp >> 2, wq = warp & 3, row = 32 * wq + lane;      // row of the tile
+        const uint32_t ts = tmem + ((uint32_t)(32 * wq) << 16) + 128 * t;
+        const uint32_t to = tmem + ((uint32_t)(32 * wq) << 16) + 256 + HD * t;
+        uint8_t* qs = smem + L::OFF_Q + t * L::TILE;
+        // Q rows of this warp: row r of the item = query r / GRP, head r % GRP
+        auto load_q = [&](const Part& p, int h) {
+            constexpr int C4 = HD / 4;                          // float4 columns a row
+#pragma unroll 4
+            for (int i = lane; i < 32 * C4; i += 32) {
+                const int r = 32 * wq + i / C4, c = i % C4, ir = 128 * t + r, qi = ir / GRP;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (qi < p.nq)
+                    v = __ldg(reinterpret_cast<const float4*>(a.q + ((long long)(p.row0 + qi) * a.nHq + h * GRP + ir % GRP) * HD) + c);
+                *reinterpret_cast<uint2*>(qs + (c >> 4) * L::HALF + sw128(r, (c & 15) >> 1) + (c & 1) * 8) =
+                    make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[t]);
+        };
+        // the CTA's next part that has rows in this tile
+        const uint4* bad = reinterpret_cast<const uint4*>(smem + L::OFF_BAD);
+        int tile = 0;                                            // tiles of the CTA so far (the masks' ring)
+        auto find = [&](int k, Part& p, int& h) {
+            for (;; k++) {
+                if (k * grid >= total) return -1;
+                const int i = nth(k, cta, grid);
+                if (i >= total) continue;
+                p = a.parts[i / nKv];
+                h = i % nKv;
+                if (p.t1 > p.t0 && (t == 0 || p.nq * GRP > 128)) return k;
+                tile += p.t1 - p.t0;
+                // a part that sees nothing: zeros (its rows lie before the sequence)
+                if (p.t1 <= p.t0 && t == 0 && p.slot < 0)
+                    for (int j = tid; j < p.nq * GRP * HD; j += 128)
+                        a.out[((long long)(p.row0 + j / (GRP * HD)) * a.nHq + h * GRP) * HD + j % (GRP * HD)] =
+                            __float2bfloat16_rn(0.0f);
+            }
+        };
+        Part p;
+        int h = 0, k = find(0, p, h), seq = 0;                   // seq: tiles of this row tile so far
+        if (k >= 0) load_q(p, h);
+        while (k >= 0) {
+            const int qi = (128 * t + row) / GRP;
+            const int pos = p.p0 + min(qi, p.nq - 1), pmin = max(p.p0, 0), pmax = p.p0 + p.nq - 1;
+            const SeenTiles seen(pmin, pmax, a.window, a.sinks, PK);
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = p.t0; j < p.t1; j++, seq++, tile++) {
+                if (!(ok = wait_warp(&s_full[t], seq & 1))) break;
+                tc_after();
+                float s[PK];
 #pragma unroll
-        for (int g = 0; g < GRP; g++) s[g] = 0.0f;
-        if (ok) {
-            for (int G = 0; G < NG; G++) {
-                float part[GRP];
+                for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(s) + 32 * c);
+                tmem_wait_ld();
+                const int k0 = seen.tile(j) * PK;
+                const uint4 out = bad[tile & 7];
+                if (out.x | out.y | out.z | out.w) {
+                    const uint32_t w[4] = {out.x, out.y, out.z, out.w};
 #pragma unroll
-                for (int g = 0; g < GRP; g++) part[g] = 0.0f;
-                for (int d = 0; d < 32; d++) {
-                    const float x = (float)a.kv.Kq[at + 32 * G + d];
-#pragma unroll
-                    for (int g = 0; g < GRP; g++) part[g] = fmaf(x, qs[g][32 * G + d], part[g]);
+                    for (int c = 0; c < PK; c++)
+                        if ((w[c >> 5] >> (c & 31)) & 1) s[c] = -INFINITY;
                 }
-                const float sc = a.kv.Ks[at / 32 + G] * (1.0f / 127.0f);
+                // a tile that some row sees only in part
+                if (k0 + PK - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window && k0 + PK > a.sinks)) {
+                    const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
 #pragma unroll
-                for (int g = 0; g < GRP; g++) s[g] = fmaf(part[g], sc, s[g]);
+                    for (int c = 0; c < PK; c++) s[c] = c <= hi && (c > lo || c < sk) ? s[c] : -INFINITY;
+                }
+                float mx = s[0];
+#pragma unroll
+                for (int c = 1; c < PK; c++) mx = fmaxf(mx, s[c]);
+                mx *= a.sl2;
+                // raise the reference only when a score would pass it by 2^RAISE (or none was seen yet)
+                const bool up = mx > m + RAISE || (m == -INFINITY && mx > m);
+                if (__any_sync(0xffffffffu, up && l > 0.0f)) {
+                    // every column of O so far, once the last product is in
+                    if (!(ok = wait_warp(&o_done[t], (seq - 1) & 1))) break;
+                    tc_after();
+                    const float f = up ? ex2(m - mx) : 1.0f;
+#pragma unroll
+                    for (int c = 0; c < HD / 32; c++) {
+                        uint32_t o[32];
+                        tmem_ld32(to + 32 * c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st32(to + 32 * c, o);
+                    }
+                    l *= f;
+                }
+                if (up) m = mx;
+                const float off = m == -INFINITY ? 0.0f : -m;
+                float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const float2 x = ffma2(make_float2(s[64 * c + 2 * i], s[64 * c + 2 * i + 1]),
+                                               make_float2(a.sl2, a.sl2), make_float2(off, off));
+                        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                        sum = fadd2(sum, e);
+                        pk[i] = pack_h2(e.x, e.y);
+                    }
+                    tmem_st32(ts + 32 * c, pk);
+                }
+                l += sum.x + sum.y;
+                tmem_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+            }
+            if (!ok) break;
+            // the next part's Q goes in under this part's last product
+            Part pn;
+            int hn = 0;
+            const int kn = find(k + 1, pn, hn);
+            if (kn >= 0) load_q(pn, hn);
+            if (!wait_warp(&o_done[t], (seq - 1) & 1)) break;
+            tc_after();
+            const bool live = qi < p.nq;
+            const long long slot = p.slot < 0 ? 0 : (long long)p.slot * nKv + h;
+            if (p.slot >= 0) a.PML[slot * ROWS + 128 * t + row] = make_float2(m, l);
+            const float r = p.slot >= 0 ? 1.0f : (l > 0.0f || l != l ? 1.0f / l : 0.0f);
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                uint32_t o[32];
+                tmem_ld32(to + 32 * c, o);
+                tmem_wait_ld();
+                if (p.slot >= 0) {
+                    float4* dst = reinterpret_cast<float4*>(a.PO + (slot * ROWS + 128 * t + row) * HD + 32 * c);
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                             __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                } else if (live) {
+                    uint4* dst = reinterpret_cast<uint4*>(
+                        a.out + ((long long)(p.row0 + qi) * a.nHq + h * GRP + (128 * t + row) % GRP) * HD + 32 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(o[8 * i + 2 * x]) * r,
+                                                                           __uint_as_float(o[8 * i + 2 * x + 1]) * r);
+                            w[x] = *reinterpret_cast<const uint32_t*>(&v);
+                        }
+                        dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+            tc_before();       // O is read before the p_full that lets the next part's product write it
+            p = pn;
+            h = hn;
+            k = kn;
+        }
+    } else if (warp < 12) {
+        // ============================ K / V tiles ======================================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
+        int* rows = reinterpret_cast<int*>(smem + L::OFF_ROW);
+        uint2* scs = reinterpret_cast<uint2*>(smem + L::OFF_SC);    // [3][2][PK] four f16 scales
+        constexpr int NG = HD / 32, CPR = HD / 16, NCH = PK * CPR / 128;   // 16-byte chunks: a row, a thread
+        // the walk over the tiles of the CTA's parts
+        int wk = -1, wj = 0, wt1 = 0, wb = 0, wh = 0, pmin = 0, pmax = 0, steps = 0;
+        uint32_t* bads = reinterpret_cast<uint32_t*>(smem + L::OFF_BAD);
+        SeenTiles seen(-1, -1, 0, 0, PK);
+        auto step = [&](int& row, int& hh) {                        // the thread's pool row of the next tile
+            while (wj >= wt1) {
+                wk++;
+                if (wk * grid >= total) return false;
+                const int i = nth(wk, cta, grid);
+                if (i >= total) continue;
+                const Part p = a.parts[i / nKv];
+                wh = i % nKv;
+                wb = p.b;
+                wj = p.t0;
+                wt1 = p.t1;
+                pmin = max(p.p0, 0);
+                pmax = p.p0 + p.nq - 1;
+                seen = SeenTiles(pmin, pmax, a.window, a.sinks, PK);
+            }
+            const int key = seen.tile(wj++) * PK + pt;
+            // a row that no query of the part sees stays zero
+            const bool see = key <= pmax && (a.window <= 0 || key > pmin - a.window || key < a.sinks);
+            row = see ? a.kv.row(wb, key) : -1;
+            // A key on a page outside the pool: the softmax leaves it out.  This runs up to three tiles ahead of
+            // the tile being stored, whose stage the product of two tiles before has left, so of the eight
+            // masks the one written here was last read five tiles ago.
+            const unsigned miss = __ballot_sync(0xffffffffu, see && row < 0);
+            if (lane == 0) bads[(steps & 7) * 4 + (pt >> 5)] = miss;
+            steps++;
+            hh = wh;
+            return true;
+        };
+        auto load_scales = [&](int row, int hh, float (&ks)[4], float (&vs)[4]) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) ks[i] = vs[i] = 0.0f;
+            if (row >= 0) {
+                const long long at = ((long long)row * nKv + hh) * NG;
+                if constexpr (NG == 4) {
+                    const float4 x = __ldg(reinterpret_cast<const float4*>(a.kv.Ks + at));
+                    const float4 y = __ldg(reinterpret_cast<const float4*>(a.kv.Vs + at));
+                    ks[0] = x.x; ks[1] = x.y; ks[2] = x.z; ks[3] = x.w;
+                    vs[0] = y.x; vs[1] = y.y; vs[2] = y.z; vs[3] = y.w;
+                } else {
+                    const float2 x = __ldg(reinterpret_cast<const float2*>(a.kv.Ks + at));
+                    const float2 y = __ldg(reinterpret_cast<const float2*>(a.kv.Vs + at));
+                    ks[0] = x.x; ks[1] = x.y;
+                    vs[0] = y.x; vs[1] = y.y;
+                }
+            }
+        };
+        auto publish = [&](int buf, int row, const float (&ks)[4], const float (&vs)[4]) {
+            constexpr float S = 128.0f / 127.0f;                    // bytes become q / 128
+            rows[buf * PK + pt] = row;
+            scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * S, ks[1] * S), pack_h2(ks[2] * S, ks[3] * S));
+            scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(vs[0] * S, vs[1] * S), pack_h2(vs[2] * S, vs[3] * S));
+        };
+        const int ch = pt % CPR, r0 = pt / CPR;                     // chunk of a row; rows r0 + i * 128 / CPR
+        auto load = [&](const int8_t* pool, int buf, int hh, uint4 (&x)[NCH]) {
+#pragma unroll
+            for (int i = 0; i < NCH; i++) {
+                const int row = rows[buf * PK + r0 + i * (128 / CPR)];
+                x[i] = row >= 0 ? ldg_stream_v4(pool + ((long long)row * nKv + hh) * HD + 16 * ch) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto store = [&](uint8_t* tile, int buf, int which, const uint4 (&x)[NCH]) {
+            const __half* sc = reinterpret_cast<const __half*>(scs + (2 * buf + which) * PK) + (ch >> 1);
+            uint8_t* half = tile + (ch >> 2) * L::HALF;
+            const int c0 = (ch & 3) * 2, swap = (ch >> 2) & 1;      // the halves' chunks go to other banks
+#pragma unroll
+            for (int i = 0; i < NCH; i++) {
+                const int r = r0 + i * (128 / CPR);
+                const __half2 s2 = __half2half2(sc[4 * r]);
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                uint32_t o[8];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const uint32_t u = w[y] ^ 0x80808080u;          // byte + 128 -> 1024 + u -> (u - 128) / 128
+                    const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+                    const __half2 k = __float2half2_rn(0.0078125f), m9 = __float2half2_rn(-9.0f);
+                    const __half2 f0 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&lo), k, m9), s2);
+                    const __half2 f1 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&hi), k, m9), s2);
+                    o[2 * y] = *reinterpret_cast<const uint32_t*>(&f0);
+                    o[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&f1);
+                }
+                uint4 lo4 = make_uint4(o[0], o[1], o[2], o[3]), hi4 = make_uint4(o[4], o[5], o[6], o[7]);
+                *reinterpret_cast<uint4*>(half + sw128(r, c0 + swap)) = swap ? hi4 : lo4;
+                *reinterpret_cast<uint4*>(half + sw128(r, c0 + 1 - swap)) = swap ? lo4 : hi4;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+        };
+        // a barrier of the four warps; true when one of them has given up
+        auto sync = [](bool dead) {
+            uint32_t any;
+            asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n"
+                         " selp.u32 %0, 1, 0, q;\n}" : "=r"(any) : "r"((uint32_t)dead) : "memory");
+            return any != 0;
+        };
+        int row1 = -1, row2 = -1, h0 = 0, h1 = 0, h2 = 0;
+        float ks[4], vs[4];
+        uint4 xk[NCH], xv[NCH];
+        bool more0 = step(row1, h0), more1 = false, more2 = false;
+        if (more0) {
+            load_scales(row1, h0, ks, vs);
+            publish(0, row1, ks, vs);
+            sync(false);
+            load(a.kv.Kq, 0, h0, xk);
+            load(a.kv.Vq, 0, h0, xv);
+            more1 = step(row1, h1);
+            if (more1) {
+                load_scales(row1, h1, ks, vs);
+                more2 = step(row2, h2);
             }
         }
-#pragma unroll
-        for (int g = 0; g < GRP; g++) {
-            const float x = ok ? s[g] : NEG_BIG;
-            const float mn = fmaxf(m[g], warp_max(x)), corr = exp2f(m[g] - mn);
-            p[g] = ok ? exp2f(x - mn) : 0.0f;
-            l[g] = fmaf(l[g], corr, p[g]);
-            m[g] = mn;
-#pragma unroll
-            for (int j = 0; j < DPL; j++) o[g][j] *= corr;
+        bool dead = false;
+        for (int it = 0; more0; it++) {
+            const int s = it % KV_STAGES, buf = it % 3, nb = (it + 1) % 3;
+            const uint32_t par = ((it / KV_STAGES) & 1) ^ 1;
+            // rows and scales of the next tile (their buffer was last read two tiles ago)
+            if (more1) publish(nb, row1, ks, vs);
+            if (sync(dead)) break;
+            if (more2) load_scales(row2, h2, ks, vs);
+            if ((dead = !wait_warp(&k_empty[s], par))) continue;    // all leave at the next barrier
+            store(smem + L::OFF_K + s * L::TILE, buf, 0, xk);
+            if (lane == 0) mbar_arrive(&k_full[s]);
+            if (more1) load(a.kv.Kq, nb, h1, xk);
+            if ((dead = !wait_warp(&v_empty[s], par))) continue;
+            store(smem + L::OFF_V + s * L::TILE, buf, 1, xv);
+            if (lane == 0) mbar_arrive(&v_full[s]);
+            if (more1) load(a.kv.Vq, nb, h1, xv);
+            more0 = more1;
+            h0 = h1;
+            more1 = more2;
+            h1 = h2;
+            row1 = row2;
+            if (more2) more2 = step(row2, h2);
         }
-        for (int k = 0; k < KT; k++) {
-            const int r = __shfl_sync(0xffffffffu, row, k);
-            float pk[GRP];
+    } else {
+        // ================================ MMAs ==========================================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 12 && lane == 0) {
+            constexpr uint32_t I1 = idesc(PK, false), I2 = idesc(HD, true);
+            const uint32_t base = smem_u32(smem);
+            int it = 0;
+            uint32_t ph = 0;                               // parities of q_full (bits 0, 1) and p_full (2, 3)
+            bool ok = true;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                if (ok && !mbar_wait(bar, parity, abort_flag)) {
+                    give_up();
+                    ok = false;
+                }
+                return ok;
+            };
+            auto scores = [&](int t, int s) {          // S_t = Q_t K^T
+                const uint32_t qa = base + L::OFF_Q + t * L::TILE, kb = base + L::OFF_K + s * L::TILE;
 #pragma unroll
-            for (int g = 0; g < GRP; g++) pk[g] = __shfl_sync(0xffffffffu, p[g], k);
-            if (r < 0) continue;
-            const long long va = (long long)r * nKv * HD + h * HD;
+                for (int c = 0; c < HD / 16; c++) {
+                    const uint32_t at = (uint32_t)((c >> 2) * L::HALF + (c & 3) * 32);
+                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
+                                 ::"r"(tmem + 128 * t), "l"(desc_k(qa + at)), "l"(desc_k(kb + at)), "r"(I1),
+                                   "r"(c > 0 ? 1u : 0u), "r"(0u) : "memory");
+                }
+                tc_commit(&s_full[t]);
+            };
+            auto output = [&](int t, int s, bool add) {   // O_t (+)= P_t V
+                const uint32_t vb = base + L::OFF_V + s * L::TILE;
 #pragma unroll
-            for (int j = 0; j < DPL; j++) {
-                const float v = (float)a.kv.Vq[va + 32 * j + lane] * (a.kv.Vs[va / 32 + j] * (1.0f / 127.0f));
-#pragma unroll
-                for (int g = 0; g < GRP; g++) o[g][j] = fmaf(pk[g], v, o[g][j]);
+                for (int c = 0; c < PK / 16; c++)
+                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
+                                 ::"r"(tmem + 256 + HD * t), "r"(tmem + 128 * t + 8 * c), "l"(desc_mn(vb + 2048 * c)),
+                                   "r"(I2), "r"(add || c > 0 ? 1u : 0u), "r"(0u) : "memory");
+                tc_commit(&o_done[t]);
+            };
+            for (int k = 0; ok && k * grid < total; k++) {
+                const int i = nth(k, cta, grid);
+                if (i >= total) continue;
+                const Part p = a.parts[i / nKv];
+                const int nt = p.t1 - p.t0, tiles = p.nq * GRP > 128 ? 2 : 1;
+                if (nt <= 0) continue;
+                if (!wait(&k_full[it % KV_STAGES], (it / KV_STAGES) & 1)) break;
+                for (int t = 0; t < tiles && ok; t++) {
+                    if (!wait(&q_full[t], (ph >> t) & 1)) break;
+                    ph ^= 1u << t;
+                    tc_after();
+                    scores(t, it % KV_STAGES);
+                }
+                if (!ok) break;
+                tc_commit(&k_empty[it % KV_STAGES]);
+                for (int j = 0; j < nt && ok; j++, it++) {
+                    const int s = it % KV_STAGES, sn = (it + 1) % KV_STAGES;
+                    if (!wait(&v_full[s], (it / KV_STAGES) & 1)) break;
+                    for (int t = 0; t < tiles; t++) {
+                        if (!wait(&p_full[t], (ph >> (2 + t)) & 1)) break;
+                        ph ^= 4u << t;
+                        tc_after();
+                        output(t, s, j > 0);
+                        if (j + 1 < nt) {
+                            if (t == 0) {
+                                if (!wait(&k_full[sn], ((it + 1) / KV_STAGES) & 1)) break;
+                                tc_after();
+                            }
+                            scores(t, sn);
+                        }
+                    }
+                    if (!ok) break;
+                    tc_commit(&v_empty[s]);
+                    if (j + 1 < nt) tc_commit(&k_empty[sn]);
+                }
             }
+            tc_commit(done);
+            if (!mbar_wait(done, 0)) give_up();            // no MMA in flight past here
         }
+        __syncwarp();
     }
-#pragma unroll
-    for (int g = 0; g < GRP; g++) {
-        const float lt = warp_sum(l[g]);
-        if (lane == 0) {
-            wm[wid][g] = m[g];
-            wl[wid][g] = lt;
-        }
-#pragma unroll
-        for (int j = 0; j < DPL; j++) wo[wid][g][32 * j + lane] = o[g][j];
-    }
+    tc_before();
     __syncthreads();
-    for (int i = tid; i < GRP * HD; i += NT) {
-        const int g = i / HD, d = i % HD;
-        float M = NEG_BIG, L = 0.0f, O = 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; k++) M = fmaxf(M, wm[k][g]);
-#pragma unroll
-        for (int k = 0; k < W; k++) {
-            const float e = exp2f(wm[k][g] - M);
-            L = fmaf(wl[k][g], e, L);
-            O = fmaf(wo[k][g][d], e, O);
-        }
-        a.out[(long long)t * nHq * HD + (h * GRP + g) * HD + d] = __float2bfloat16_rn(L > 0.0f ? O / L : 0.0f);
+    if (warp == 12) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }
+}
+
+// joins the parts of item x, kv head y, rows 32 z ..: a warp four rows at a time
+template <int HD, int GRP>
+__global__ void __launch_bounds__(256) k_prefill_join(const __grid_constant__ PrefillArgs a)
+{
+    tb_pdl_wait();
+    tb_pdl_trigger();
+    const int i = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nKv = a.kv.nKv;
+    if (i >= a.head[1]) return;
+    const Item it = a.items[i];
+    if (it.parts < 2) return;
+    for (int k = 0; k < 4; k++) {
+        const int row = 32 * blockIdx.z + 4 * wid + k, qi = row / GRP;
+        if (qi >= it.nq) return;
+        float M = -INFINITY;
+        for (int p = 0; p < it.parts; p++)
+            M = fmaxf(M, a.PML[((long long)(it.slot0 + p) * nKv + h) * ROWS + row].x);
+        const float off = M == -INFINITY ? 0.0f : M;
+        float l = 0.0f, o[HD / 32];
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) o[c] = 0.0f;
+#pragma unroll 4
+        for (int p = 0; p < it.parts; p++) {
+            const long long s = ((long long)(it.slot0 + p) * nKv + h) * ROWS + row;
+            const float2 ml = a.PML[s];
+            const float e = exp2f(ml.x - off);
+            l = fmaf(ml.y, e, l);
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) o[c] = fmaf(a.PO[s * HD + 32 * c + lane], e, o[c]);
+        }
+        const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        __nv_bfloat16* dst = a.out + ((long long)(it.row0 + qi) * a.nHq + h * GRP + row % GRP) * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) dst[32 * c + lane] = __float2bfloat16_rn(o[c] * r);
+    }
+}
+
+// device workspace: head, parts, items, PML, PO
+struct PrefillWs {
+    int items, parts, slots;
+    size_t o_parts, o_items, o_pml, o_po, bytes;
+};
+PrefillWs prefill_ws(const tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, int64_t T)
+{
+    const int64_t qb = ROWS / (nHq / kv->nKv), extra = ctx->num_sms / kv->nKv + 2;
+    PrefillWs w{};
+    // each sequence with rows has at most one item that is not full; an item of n tiles has at most
+    // 1 + n / share parts, and all n / share add up to at most SMs / heads
+    w.items = (int)(T / qb + std::min<int64_t>(kv->batch, T));
+    w.parts = (int)(w.items + extra);
+    w.slots = (int)(2 * extra);
+    auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+    w.o_parts = 256;
+    w.o_items = w.o_parts + up((size_t)w.parts * sizeof(Part));
+    w.o_pml = w.o_items + up((size_t)w.items * sizeof(Item));
+    w.o_po = w.o_pml + up((size_t)w.slots * kv->nKv * ROWS * sizeof(float2));
+    w.bytes = w.o_po + up((size_t)w.slots * kv->nKv * ROWS * kv->hd * sizeof(float));
+    return w;
 }
 
 template <int HD, int GRP>
 int launch_prefill(tb_ctx* ctx, const PrefillArgs& a)
 {
-    cudaError_t e = tb_launch(ctx, k_paged_prefill<HD, GRP>, dim3(a.T, a.kv.nKv), dim3(NT), 0, a);
+    auto kern = k_paged_prefill<HD, GRP>;
+    constexpr int smem = PrefillLayout<HD>::BYTES;
+    static bool attr_set[64] = {};   // per device and instantiation; setting it twice is harmless
+    cudaError_t e = cudaSuccess;
+    if (ctx->device >= 64 || !attr_set[ctx->device]) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess && ctx->device < 64) attr_set[ctx->device] = true;
+    }
+    if (e == cudaSuccess) e = tb_launch(ctx, k_prefill_plan, dim3(1), dim3(PT), 0, a);
+    const int grid = (int)std::min<long long>(a.sms, (long long)a.max_parts * a.kv.nKv);
+    if (e == cudaSuccess) e = tb_launch(ctx, kern, dim3(grid), dim3(THREADS), (size_t)smem, a);
+    if (e == cudaSuccess) e = tb_launch(ctx, k_prefill_join<HD, GRP>, dim3(a.max_items, a.kv.nKv, ROWS / 32), dim3(256), 0, a);
     if (e != cudaSuccess) return tb_fail(ctx, TB_ERR_CUDA, "attn_prefill_paged launch: %s", cudaGetErrorString(e));
+    return TB_OK;
+}
+
+int prefill_check(tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, int64_t T)
+{
+    int rc = paged_check(ctx, kv);
+    if (!rc) rc = paged_check_heads(ctx, kv, nHq);
+    if (rc) return rc;
+    TB_REQUIRE(ctx, T >= 0 && T < (1LL << 24), "row count must be below 2^24 (got %lld)", (long long)T);
+    TB_REQUIRE(ctx, kv->batch <= MAX_BATCH, "at most %d sequences a prefill (got %lld)", MAX_BATCH, (long long)kv->batch);
     return TB_OK;
 }
 
@@ -146,11 +826,9 @@ extern "C" {
 TB_API int tb_attn_prefill_paged_ws(tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, int64_t T, size_t* bytes)
 {
     if (!ctx || !bytes) return TB_ERR_INVALID;
-    int rc = paged_check(ctx, kv);
-    if (!rc) rc = paged_check_heads(ctx, kv, nHq);
+    const int rc = prefill_check(ctx, kv, nHq, T);
     if (rc) return rc;
-    TB_REQUIRE(ctx, T >= 0 && T < (1LL << 31), "bad row count %lld", (long long)T);
-    *bytes = 0;
+    *bytes = T ? prefill_ws(ctx, kv, nHq, T).bytes : 0;
     return TB_OK;
 }
 
@@ -159,28 +837,43 @@ TB_API int tb_attn_prefill_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, uint16_t
                                     int64_t sinks, void* ws, size_t ws_bytes)
 {
     if (!ctx) return TB_ERR_INVALID;
-    int rc = paged_check(ctx, kv);
-    if (!rc) rc = paged_check_heads(ctx, kv, nHq);
+    const int rc = prefill_check(ctx, kv, nHq, T);
     if (rc) return rc;
-    TB_REQUIRE(ctx, T >= 0 && T < (1LL << 31), "bad row count %lld", (long long)T);
     TB_REQUIRE(ctx, window >= 0 && sinks >= 0, "window and sinks must not be negative");
     if (T == 0) return TB_OK;
     TB_REQUIRE(ctx, out_bf16 && q && cu && lens, "null pointer");
     TB_REQUIRE(ctx, TB_ALIGNED(out_bf16, 16) && TB_ALIGNED(q, 16), "q and out must be 16-byte aligned");
     DeviceGuard dev(ctx->device);
-    (void)ws;
-    (void)ws_bytes;
+    const PrefillWs w = prefill_ws(ctx, kv, nHq, T);
+    if (!ws) {
+        ws = tb_ctx_scratch(ctx, w.bytes);
+        if (!ws) return TB_ERR_NOMEM;
+    } else {
+        TB_REQUIRE(ctx, TB_ALIGNED(ws, 256) && ws_bytes >= w.bytes, "workspace: %zu bytes, 256-byte aligned, are needed",
+                   w.bytes);
+    }
+    char* p = static_cast<char*>(ws);
     PrefillArgs a{};
     a.kv = paged_args(ctx, kv);
     a.q = q;
     a.out = reinterpret_cast<__nv_bfloat16*>(out_bf16);
     a.cu = cu;
     a.lens = lens;
+    a.head = reinterpret_cast<int*>(p);
+    a.parts = reinterpret_cast<Part*>(p + w.o_parts);
+    a.items = reinterpret_cast<Item*>(p + w.o_items);
+    a.PML = reinterpret_cast<float2*>(p + w.o_pml);
+    a.PO = reinterpret_cast<float*>(p + w.o_po);
     a.T = (int)T;
     a.nHq = (int)nHq;
+    a.grp = (int)(nHq / kv->nKv);
     a.window = (int)std::min<int64_t>(window, 1LL << 30);
     a.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
-    a.qscale = 1.4426950408889634f / sqrtf((float)kv->hd);
+    a.sms = ctx->num_sms;
+    a.max_items = w.items;
+    a.max_parts = w.parts;
+    a.max_slots = w.slots;
+    a.sl2 = 1.4426950408889634f / sqrtf((float)kv->hd);
     switch ((int)(kv->hd * 10 + nHq / kv->nKv)) {
     case 641: return launch_prefill<64, 1>(ctx, a);
     case 642: return launch_prefill<64, 2>(ctx, a);
