@@ -255,6 +255,14 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r)
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                  : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+                 "%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -342,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
 
     if (warp < 8) {
         // =============================== softmax ======================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int t = warp >> 2, wq = warp & 3, row = 32 * wq + lane;      // row of the tile
         const uint32_t ts = tmem + ((uint32_t)(32 * wq) << 16) + 128 * t;
         const uint32_t to = tmem + ((uint32_t)(32 * wq) << 16) + 256 + HD * t;
@@ -394,27 +402,33 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             for (int j = p.t0; j < p.t1; j++, seq++, tile++) {
                 if (!(ok = wait_warp(&s_full[t], seq & 1))) break;
                 tc_after();
-                float s[PK];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(s) + 32 * c);
-                tmem_wait_ld();
                 const int k0 = seen.tile(j) * PK;
-                const uint4 out = bad[tile & 7];
-                if (out.x | out.y | out.z | out.w) {
-                    const uint32_t w[4] = {out.x, out.y, out.z, out.w};
+                const uint4 bw = bad[tile & 7];
+                // a tile that some row sees only in part, or with keys on bad pages
+                const bool cut = k0 + PK - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window && k0 + PK > a.sinks) ||
+                                 (bw.x | bw.y | bw.z | bw.w);
+                const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
+                auto mask = [&](int c0, float* s) {
+                    const uint32_t w = c0 == 0 ? bw.x : c0 == 32 ? bw.y : c0 == 64 ? bw.z : bw.w;
 #pragma unroll
-                    for (int c = 0; c < PK; c++)
-                        if ((w[c >> 5] >> (c & 31)) & 1) s[c] = -INFINITY;
+                    for (int c = 0; c < 32; c++)
+                        if (!(c0 + c <= hi && (c0 + c > lo || c0 + c < sk)) || ((w >> c) & 1)) s[c] = -INFINITY;
+                };
+                // the scores are read twice (once for the maximum), so that a thread holds 64 of them at most
+                float mx = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < 4; c += 2) {
+                    float s[64];
+                    tmem_ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(s));
+                    tmem_ld32(ts + 32 * c + 32, reinterpret_cast<uint32_t*>(s) + 32);
+                    tmem_wait_ld();
+                    if (cut) {
+                        mask(32 * c, s);
+                        mask(32 * c + 32, s + 32);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 64; i++) mx = fmaxf(mx, s[i]);
                 }
-                // a tile that some row sees only in part
-                if (k0 + PK - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window && k0 + PK > a.sinks)) {
-                    const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
-#pragma unroll
-                    for (int c = 0; c < PK; c++) s[c] = c <= hi && (c > lo || c < sk) ? s[c] : -INFINITY;
-                }
-                float mx = s[0];
-#pragma unroll
-                for (int c = 1; c < PK; c++) mx = fmaxf(mx, s[c]);
                 mx *= a.sl2;
                 // raise the reference only when a score would pass it by 2^RAISE (or none was seen yet)
                 const bool up = mx > m + RAISE || (m == -INFINITY && mx > m);
@@ -437,18 +451,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 if (up) m = mx;
                 const float off = m == -INFINITY ? 0.0f : -m;
                 float2 sum = make_float2(0.0f, 0.0f);
+                float sc[2][32];
+                tmem_ld32(ts, reinterpret_cast<uint32_t*>(sc[0]));
+                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    uint32_t pk[32];
+                for (int c = 0; c < 4; c++) {
+                    float* x = sc[c & 1];
+                    if (c < 3) tmem_ld32(ts + 32 * (c + 1), reinterpret_cast<uint32_t*>(sc[(c + 1) & 1]));
+                    if (cut) mask(32 * c, x);
+                    uint32_t pk[16];
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const float2 x = ffma2(make_float2(s[64 * c + 2 * i], s[64 * c + 2 * i + 1]),
-                                               make_float2(a.sl2, a.sl2), make_float2(off, off));
-                        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                    for (int i = 0; i < 16; i++) {
+                        const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2),
+                                               make_float2(off, off));
+                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
                         sum = fadd2(sum, e);
                         pk[i] = pack_h2(e.x, e.y);
                     }
-                    tmem_st32(ts + 32 * c, pk);
+                    tmem_st16(ts + 16 * c, pk);     // over scores that are read
+                    if (c < 3) tmem_wait_ld();
                 }
                 l += sum.x + sum.y;
                 tmem_wait_st();
@@ -502,16 +523,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         }
     } else if (warp < 12) {
         // ============================ K / V tiles ======================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
         int* rows = reinterpret_cast<int*>(smem + L::OFF_ROW);
         uint2* scs = reinterpret_cast<uint2*>(smem + L::OFF_SC);    // [3][2][PK] four f16 scales
         constexpr int NG = HD / 32, CPR = HD / 16, NCH = PK * CPR / 128;   // 16-byte chunks: a row, a thread
         // the walk over the tiles of the CTA's parts
-        int wk = -1, wj = 0, wt1 = 0, wb = 0, wh = 0, pmin = 0, pmax = 0, steps = 0;
+        int wk = -1, wj = 0, wt1 = 0, wb = 0, wh = 0, pmin = 0, pmax = 0, published = 0;
         uint32_t* bads = reinterpret_cast<uint32_t*>(smem + L::OFF_BAD);
         SeenTiles seen(-1, -1, 0, 0, PK);
-        auto step = [&](int& row, int& hh) {                        // the thread's pool row of the next tile
+        // The thread's key of the next tile: its page number (requested here, looked at a tile later) and line;
+        // a row that no query of the part sees is line -1 and stays zero.
+        auto step = [&](int& page, int& line, int& hh) {
             while (wj >= wt1) {
                 wk++;
                 if (wk * grid >= total) return false;
@@ -527,17 +550,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 seen = SeenTiles(pmin, pmax, a.window, a.sinks, PK);
             }
             const int key = seen.tile(wj++) * PK + pt;
-            // a row that no query of the part sees stays zero
             const bool see = key <= pmax && (a.window <= 0 || key > pmin - a.window || key < a.sinks);
-            row = see ? a.kv.row(wb, key) : -1;
-            // A key on a page outside the pool: the softmax leaves it out.  This runs up to three tiles ahead of
-            // the tile being stored, whose stage the product of two tiles before has left, so of the eight
-            // masks the one written here was last read five tiles ago.
-            const unsigned miss = __ballot_sync(0xffffffffu, see && row < 0);
-            if (lane == 0) bads[(steps & 7) * 4 + (pt >> 5)] = miss;
-            steps++;
+            page = see ? __ldg(a.kv.table + (long long)wb * a.kv.max_pages + (key >> a.kv.log_page)) : 0;
+            line = see ? key & ((1 << a.kv.log_page) - 1) : -1;
             hh = wh;
             return true;
+        };
+        // the pool row: -1 not seen, -2 a page outside the pool
+        auto finish = [&](int page, int line) {
+            if (line < 0) return -1;
+            if ((unsigned)page < (unsigned)a.kv.n_pages) return (page << a.kv.log_page) | line;
+            atomicExch(a.kv.err, ERR_PAGED_PAGE);
+            return -2;
         };
         auto load_scales = [&](int row, int hh, float (&ks)[4], float (&vs)[4]) {
 #pragma unroll
@@ -559,7 +583,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         };
         auto publish = [&](int buf, int row, const float (&ks)[4], const float (&vs)[4]) {
             constexpr float S = 128.0f / 127.0f;                    // bytes become q / 128
-            rows[buf * PK + pt] = row;
+            // a row that is not there: any bytes, of scale zero
+            rows[buf * PK + pt] = max(row, 0);
+            // its key, on a page outside the pool, is left out by the softmax; of the eight masks the one
+            // written here was last read seven tiles ago, four more than the stages hold
+            const unsigned miss = __ballot_sync(0xffffffffu, row == -2);
+            if (lane == 0) bads[(published & 7) * 4 + (pt >> 5)] = miss;
+            published++;
             scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * S, ks[1] * S), pack_h2(ks[2] * S, ks[3] * S));
             scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(vs[0] * S, vs[1] * S), pack_h2(vs[2] * S, vs[3] * S));
         };
@@ -568,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
 #pragma unroll
             for (int i = 0; i < NCH; i++) {
                 const int row = rows[buf * PK + r0 + i * (128 / CPR)];
-                x[i] = row >= 0 ? ldg_stream_v4(pool + ((long long)row * nKv + hh) * HD + 16 * ch) : make_uint4(0, 0, 0, 0);
+                x[i] = ldg_stream_v4(pool + ((long long)row * nKv + hh) * HD + 16 * ch);
             }
         };
         auto store = [&](uint8_t* tile, int buf, int which, const uint4 (&x)[NCH]) {
@@ -605,44 +635,52 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                          " selp.u32 %0, 1, 0, q;\n}" : "=r"(any) : "r"((uint32_t)dead) : "memory");
             return any != 0;
         };
-        int row1 = -1, row2 = -1, h0 = 0, h1 = 0, h2 = 0;
+        // tile it is stored, it + 1's bytes are loaded, it + 2's scales and it + 3's page numbers requested
+        int row = -1, page = 0, line = -1, h0 = 0, h1 = 0, h2 = 0, h3 = 0;
         float ks[4], vs[4];
         uint4 xk[NCH], xv[NCH];
-        bool more0 = step(row1, h0), more1 = false, more2 = false;
+        bool more0 = step(page, line, h0), more1 = false, more2 = false, more3 = false, dead = false;
         if (more0) {
-            load_scales(row1, h0, ks, vs);
-            publish(0, row1, ks, vs);
+            row = finish(page, line);
+            load_scales(row, h0, ks, vs);
+            publish(0, row, ks, vs);
             sync(false);
             load(a.kv.Kq, 0, h0, xk);
             load(a.kv.Vq, 0, h0, xv);
-            more1 = step(row1, h1);
-            if (more1) {
-                load_scales(row1, h1, ks, vs);
-                more2 = step(row2, h2);
+            if ((more1 = step(page, line, h1))) {
+                row = finish(page, line);
+                load_scales(row, h1, ks, vs);
+                more2 = step(page, line, h2);
             }
         }
-        bool dead = false;
         for (int it = 0; more0; it++) {
             const int s = it % KV_STAGES, buf = it % 3, nb = (it + 1) % 3;
             const uint32_t par = ((it / KV_STAGES) & 1) ^ 1;
             // rows and scales of the next tile (their buffer was last read two tiles ago)
-            if (more1) publish(nb, row1, ks, vs);
+            if (more1) publish(nb, row, ks, vs);
             if (sync(dead)) break;
-            if (more2) load_scales(row2, h2, ks, vs);
-            if ((dead = !wait_warp(&k_empty[s], par))) continue;    // all leave at the next barrier
+            if (more2) {
+                row = finish(page, line);
+                load_scales(row, h2, ks, vs);
+                more3 = step(page, line, h3);
+            }
+            dead = !wait_warp(&k_empty[s], par);
+            if (dead) continue;                                     // all leave at the next barrier
             store(smem + L::OFF_K + s * L::TILE, buf, 0, xk);
             if (lane == 0) mbar_arrive(&k_full[s]);
             if (more1) load(a.kv.Kq, nb, h1, xk);
-            if ((dead = !wait_warp(&v_empty[s], par))) continue;
+            dead = !wait_warp(&v_empty[s], par);
+            if (dead) continue;
             store(smem + L::OFF_V + s * L::TILE, buf, 1, xv);
             if (lane == 0) mbar_arrive(&v_full[s]);
             if (more1) load(a.kv.Vq, nb, h1, xv);
             more0 = more1;
-            h0 = h1;
             more1 = more2;
+            more2 = more3;
+            more3 = false;
+            h0 = h1;
             h1 = h2;
-            row1 = row2;
-            if (more2) more2 = step(row2, h2);
+            h2 = h3;
         }
     } else {
         // ================================ MMAs ==========================================
