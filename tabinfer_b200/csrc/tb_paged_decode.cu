@@ -15,13 +15,13 @@
 // a pair's chunks writes (m, l, o) for it (at most two such parts a CTA: its first and its
 // last pair); k_paged_combine joins a pair's parts in order, so results do not depend on
 // timing.
-#include "tb_attn_dev.cuh"
 #include "tb_paged.cuh"
 
 namespace {
 
 constexpr int W = 4, NT = 32 * W;
 constexpr int CT = 512;    // threads of a joining CTA
+constexpr float NEG_BIG = -3.0e38f;
 
 struct DecArgs {
     CUtensorMap mk, mv;    // Kq / Vq as bytes [pool rows][nKv*HD], boxes of min(32, page_rows) rows x HD

@@ -12,13 +12,14 @@
 // in order.  k_prefill_plan (one CTA) lists the parts by length; the persistent CTAs (one an
 // SM) take them in boustrophedon order.
 //
-// Warp roles of k_paged_prefill (512 threads):
+// Warp roles of k_paged_prefill:
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread a row: S from TMEM, P (f16) back
 //                    over it; the reference maximum is raised (and O rescaled in TMEM) only
 //                    when a score passes it by 2^8, so O is hardly ever touched; Q of the
 //                    next part into shared memory, then the part's outputs
-//   warps 8-11       K / V tiles: 16-byte loads a tile ahead, bytes -> f16 (one exact step,
-//                    one multiplication by the group's scale) into swizzled tiles
+//   warps 8-11       K / V tiles: 16-byte copies ahead into thread-private shared memory, bytes
+//                    -> f16 (one exact step, one multiplication by the group's scale) into
+//                    swizzled tiles
 //   warp 12          TMEM and the MMAs: S_t = Q_t K^T (both K-major), O_t += P_t V (P from
 //                    TMEM, V MN-major as it lies in the cache), row tile 0 and 1 in turn so
 //                    that one's softmax runs under the other's MMAs
@@ -34,7 +35,9 @@ namespace {
 
 constexpr int PK = 128;                  // keys a tile
 constexpr int ROWS = 256;                // rows an item: two tiles of 128
-constexpr int THREADS = 512;
+constexpr int THREADS = 512;               // 2 x 4 softmax and 4 producer warps, the MMA warp and three idle ones
+constexpr int PROD = 128, W_MMA = 12;
+constexpr int NC = 4;                      // 16-byte chunks a producer thread takes at a time
 constexpr int KV_STAGES = 2;
 constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps their sums in shared memory)
 constexpr int MIN_TILES = 2;             // an item is not cut below this many tiles a part
@@ -204,7 +207,10 @@ struct PrefillLayout {
     static constexpr int OFF_ROW = OFF_V + KV_STAGES * TILE;   // int [3][PK] pool rows
     static constexpr int OFF_SC = OFF_ROW + 3 * PK * 4;        // f16 [3][2][PK][4] scales of K and V
     static constexpr int OFF_BAD = OFF_SC + 3 * 2 * PK * 8;   // uint [8][PK / 32]: keys of pages outside the pool
-    static constexpr int OFF_BAR = OFF_BAD + 8 * PK / 8;
+    // the producers' raw bytes: units of NC x 16 bytes a thread, thread-private (cp.async), NU in flight
+    static constexpr int UNITS = HD / 64, NU = HD == 128 ? 3 : 2;
+    static constexpr int OFF_RAW = OFF_BAD + 8 * PK / 8;
+    static constexpr int OFF_BAR = OFF_RAW + NU * NC * 16 * PROD;
     static constexpr int BYTES = 1024 + OFF_BAR + 256;
     static_assert(BYTES <= 227 * 1024, "shared memory");
 };
@@ -245,6 +251,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r)
                  "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : TB_R32(r) : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr));
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
@@ -255,22 +268,40 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r)
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r)
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-                 "%14,%15,%16};"
-                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// The MMA warp runs these with all lanes and warp-uniform operands and elects the issuing
+// thread inside: addresses then stay in uniform registers and an MMA costs one instruction
+// (issued from a branch on one lane, 128 x 128 x 16 took 115 cycles against 68 here).
 __device__ __forceinline__ void tc_commit(uint64_t* bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}"
                  ::"r"(smem_u32(bar)) : "memory");
+}
+// D (+)= A B^T over 64 k of f16: A and B K-major in shared memory, four steps of 32 bytes
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t id, uint32_t add)
+{
+#define TB_SS(i, pr)                                                                              \
+    " add.u64 a, %1, " #i ";\n add.u64 b, %2, " #i ";\n"                                          \
+    " @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, " #pr ";\n"
+    asm volatile("{\n .reg .pred e, p, t;\n .reg .b64 a, b;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+                 " elect.sync _|e, 0xffffffff;\n" TB_SS(0, p) TB_SS(2, t) TB_SS(4, t) TB_SS(6, t) "}"
+                 ::"r"(d), "l"(da), "l"(db), "r"(id), "r"(add) : "memory");
+#undef TB_SS
+}
+// D (+)= A B over 64 k: A f16 in TMEM (8 columns a step), B MN-major (2048 bytes a step)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t id, uint32_t add)
+{
+#define TB_TS(i, j, pr)                                                                           \
+    " add.u32 a, %1, " #i ";\n add.u64 b, %2, " #j ";\n"                                          \
+    " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, " #pr ";\n"
+    asm volatile("{\n .reg .pred e, p, t;\n .reg .b32 a;\n .reg .b64 b;\n setp.ne.b32 p, %4, 0;\n setp.eq.b32 t, 0, 0;\n"
+                 " elect.sync _|e, 0xffffffff;\n" TB_TS(0, 0, p) TB_TS(8, 128, t) TB_TS(16, 256, t) TB_TS(24, 384, t) "}"
+                 ::"r"(d), "r"(ta), "l"(db), "r"(id), "r"(add) : "memory");
+#undef TB_TS
 }
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi)
 {
@@ -315,16 +346,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             mbar_init(&o_done[i], 1);
         }
         for (int i = 0; i < KV_STAGES; i++) {
-            mbar_init(&k_full[i], 4);
+            mbar_init(&k_full[i], PROD / 32);
             mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], 4);
+            mbar_init(&v_full[i], PROD / 32);
             mbar_init(&v_empty[i], 1);
         }
         mbar_init(done, 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == W_MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                      ::"r"(smem_u32((const void*)tmem_slot)), "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -350,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
 
     if (warp < 8) {
         // =============================== softmax ======================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");      // 256 x 152 + 128 x 128 + 128 x 80 = 65536
         const int t = warp >> 2, wq = warp & 3, row = 32 * wq + lane;      // row of the tile
         const uint32_t ts = tmem + ((uint32_t)(32 * wq) << 16) + 128 * t;
         const uint32_t to = tmem + ((uint32_t)(32 * wq) << 16) + 256 + HD * t;
@@ -409,68 +440,79 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                                  (bw.x | bw.y | bw.z | bw.w);
                 const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
                 auto mask = [&](int c0, float* s) {
-                    const uint32_t w = c0 == 0 ? bw.x : c0 == 32 ? bw.y : c0 == 64 ? bw.z : bw.w;
+                    const uint32_t w = (c0 < 32 ? bw.x : c0 < 64 ? bw.y : c0 < 96 ? bw.z : bw.w) >> (c0 & 31);
 #pragma unroll
-                    for (int c = 0; c < 32; c++)
+                    for (int c = 0; c < 16; c++)
                         if (!(c0 + c <= hi && (c0 + c > lo || c0 + c < sk)) || ((w >> c) & 1)) s[c] = -INFINITY;
                 };
-                // the scores are read twice (once for the maximum), so that a thread holds 64 of them at most
-                float mx = -INFINITY;
+                // One pass over the scores against the reference maximum as it stands; a score that passes it
+                // by 2^RAISE raises it, rescales O (every column, once the last product is in) and repeats
+                // the pass.  The first tile's maximum comes first.
+                if (j == p.t0) {
+                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < 4; c += 2) {
-                    float s[64];
-                    tmem_ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(s));
-                    tmem_ld32(ts + 32 * c + 32, reinterpret_cast<uint32_t*>(s) + 32);
-                    tmem_wait_ld();
-                    if (cut) {
-                        mask(32 * c, s);
-                        mask(32 * c + 32, s + 32);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 64; i++) mx = fmaxf(mx, s[i]);
-                }
-                mx *= a.sl2;
-                // raise the reference only when a score would pass it by 2^RAISE (or none was seen yet)
-                const bool up = mx > m + RAISE || (m == -INFINITY && mx > m);
-                if (__any_sync(0xffffffffu, up && l > 0.0f)) {
-                    // every column of O so far, once the last product is in
-                    if (!(ok = wait_warp(&o_done[t], (seq - 1) & 1))) break;
-                    tc_after();
-                    const float f = up ? ex2(m - mx) : 1.0f;
-#pragma unroll
-                    for (int c = 0; c < HD / 32; c++) {
-                        uint32_t o[32];
-                        tmem_ld32(to + 32 * c, o);
+                    for (int c = 0; c < 4; c++) {
+                        float s[32];
+                        tmem_ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(s));
                         tmem_wait_ld();
+                        if (cut) {
+                            mask(32 * c, s);
+                            mask(32 * c + 16, s + 16);
+                        }
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tmem_st32(to + 32 * c, o);
+                        for (int i = 0; i < 32; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
                     }
-                    l *= f;
+                    m = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.sl2;
                 }
-                if (up) m = mx;
-                const float off = m == -INFINITY ? 0.0f : -m;
-                float2 sum = make_float2(0.0f, 0.0f);
-                float sc[2][32];
-                tmem_ld32(ts, reinterpret_cast<uint32_t*>(sc[0]));
-                tmem_wait_ld();
+                uint32_t pk[64];
+                float2 sum;
+                for (;;) {
+                    const float off = m == -INFINITY ? 0.0f : -m;
+                    float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                    float t2[2] = {-INFINITY, -INFINITY};
+                    float sc[2][16];
+                    tmem_ld16(ts, reinterpret_cast<uint32_t*>(sc[0]));
+                    tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    float* x = sc[c & 1];
-                    if (c < 3) tmem_ld32(ts + 32 * (c + 1), reinterpret_cast<uint32_t*>(sc[(c + 1) & 1]));
-                    if (cut) mask(32 * c, x);
-                    uint32_t pk[16];
+                    for (int c = 0; c < 8; c++) {
+                        float* x = sc[c & 1];
+                        if (c < 7) tmem_ld16(ts + 16 * (c + 1), reinterpret_cast<uint32_t*>(sc[(c + 1) & 1]));
+                        if (cut) mask(16 * c, x);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2),
-                                               make_float2(off, off));
-                        const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                        sum = fadd2(sum, e);
-                        pk[i] = pack_h2(e.x, e.y);
+                        for (int i = 0; i < 8; i++) {
+                            const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2),
+                                                   make_float2(off, off));
+                            t2[i & 1] = fmaxf(t2[i & 1], fmaxf(y.x, y.y));
+                            const float2 e = make_float2(ex2(y.x), ex2(y.y));
+                            s2[i & 1] = fadd2(s2[i & 1], e);
+                            pk[8 * c + i] = pack_h2(e.x, e.y);
+                        }
+                        if (c < 7) tmem_wait_ld();
                     }
-                    tmem_st16(ts + 16 * c, pk);     // over scores that are read
-                    if (c < 3) tmem_wait_ld();
+                    sum = fadd2(s2[0], s2[1]);
+                    const float top = fmaxf(t2[0], t2[1]);           // the maximum, from the reference
+                    const bool up = top > (m == -INFINITY ? -INFINITY : RAISE);
+                    if (!__any_sync(0xffffffffu, up)) break;
+                    if (j > p.t0) {
+                        if (!(ok = wait_warp(&o_done[t], (seq - 1) & 1))) break;
+                        tc_after();
+                        const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(-top);
+#pragma unroll
+                        for (int c = 0; c < HD / 32; c++) {
+                            uint32_t o[32];
+                            tmem_ld32(to + 32 * c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_st32(to + 32 * c, o);
+                        }
+                        l *= f;
+                    }
+                    if (up) m = m == -INFINITY ? top : m + top;
                 }
+                if (!ok) break;
+                tmem_st32(ts, pk);
+                tmem_st32(ts + 32, pk + 32);
                 l += sum.x + sum.y;
                 tmem_wait_st();
                 tc_before();
@@ -521,13 +563,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             h = hn;
             k = kn;
         }
-    } else if (warp < 12) {
+    } else if (warp < W_MMA) {
         // ============================ K / V tiles ======================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-        const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
+                const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
         int* rows = reinterpret_cast<int*>(smem + L::OFF_ROW);
         uint2* scs = reinterpret_cast<uint2*>(smem + L::OFF_SC);    // [3][2][PK] four f16 scales
-        constexpr int NG = HD / 32, CPR = HD / 16, NCH = PK * CPR / 128;   // 16-byte chunks: a row, a thread
+        constexpr int NG = HD / 32, CPR = HD / 16, RPU = NC * PROD / CPR;   // 16-byte chunks a row, rows a unit
         // the walk over the tiles of the CTA's parts
         int wk = -1, wj = 0, wt1 = 0, wb = 0, wh = 0, pmin = 0, pmax = 0, published = 0;
         uint32_t* bads = reinterpret_cast<uint32_t*>(smem + L::OFF_BAD);
@@ -593,42 +634,51 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * S, ks[1] * S), pack_h2(ks[2] * S, ks[3] * S));
             scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(vs[0] * S, vs[1] * S), pack_h2(vs[2] * S, vs[3] * S));
         };
-        const int ch = pt % CPR, r0 = pt / CPR;                     // chunk of a row; rows r0 + i * 128 / CPR
-        auto load = [&](const int8_t* pool, int buf, int hh, uint4 (&x)[NCH]) {
+        const int ch = pt % CPR, r0 = pt / CPR;                     // chunk of a row; rows r0 + i * PROD / CPR
+        uint4* raw = reinterpret_cast<uint4*>(smem + L::OFF_RAW) + pt;
+        // unit x of a tile (K: 0 .. UNITS - 1, then V): this thread's chunk of four of its rows, into ring slot n
+        auto load = [&](int x, int buf, int hh, int n) {
+            const int8_t* pool = (x < L::UNITS ? a.kv.Kq : a.kv.Vq) + hh * HD + 16 * ch;
+            const int* rr = rows + buf * PK + (x % L::UNITS) * RPU + r0;
+            int at[NC];
 #pragma unroll
-            for (int i = 0; i < NCH; i++) {
-                const int row = rows[buf * PK + r0 + i * (128 / CPR)];
-                x[i] = ldg_stream_v4(pool + ((long long)row * nKv + hh) * HD + 16 * ch);
-            }
+            for (int i = 0; i < NC; i++) at[i] = rr[i * (PROD / CPR)];
+#pragma unroll
+            for (int i = 0; i < NC; i++) cp_async16(raw + (NC * n + i) * PROD, pool + (long long)at[i] * (nKv * HD));
         };
-        auto store = [&](uint8_t* tile, int buf, int which, const uint4 (&x)[NCH]) {
-            const __half* sc = reinterpret_cast<const __half*>(scs + (2 * buf + which) * PK) + (ch >> 1);
+        auto store = [&](int x, uint8_t* tile, int buf, int n) {
+            const __half* sc = reinterpret_cast<const __half*>(scs + (2 * buf + x / L::UNITS) * PK) + (ch >> 1);
             uint8_t* half = tile + (ch >> 2) * L::HALF;
             const int c0 = (ch & 3) * 2, swap = (ch >> 2) & 1;      // the halves' chunks go to other banks
+            const int r = (x % L::UNITS) * RPU + r0;
+            uint4 v[NC];                                            // all loads before the first store
+            __half2 s2[NC];
 #pragma unroll
-            for (int i = 0; i < NCH; i++) {
-                const int r = r0 + i * (128 / CPR);
-                const __half2 s2 = __half2half2(sc[4 * r]);
-                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            for (int i = 0; i < NC; i++) {
+                v[i] = raw[(NC * n + i) * PROD];
+                s2[i] = __half2half2(sc[4 * (r + i * (PROD / CPR))]);
+            }
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int ri = r + i * (PROD / CPR);
+                const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
                 uint32_t o[8];
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
                     const uint32_t u = w[y] ^ 0x80808080u;          // byte + 128 -> 1024 + u -> (u - 128) / 128
                     const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
                     const __half2 k = __float2half2_rn(0.0078125f), m9 = __float2half2_rn(-9.0f);
-                    const __half2 f0 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&lo), k, m9), s2);
-                    const __half2 f1 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&hi), k, m9), s2);
+                    const __half2 f0 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&lo), k, m9), s2[i]);
+                    const __half2 f1 = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&hi), k, m9), s2[i]);
                     o[2 * y] = *reinterpret_cast<const uint32_t*>(&f0);
                     o[2 * y + 1] = *reinterpret_cast<const uint32_t*>(&f1);
                 }
-                uint4 lo4 = make_uint4(o[0], o[1], o[2], o[3]), hi4 = make_uint4(o[4], o[5], o[6], o[7]);
-                *reinterpret_cast<uint4*>(half + sw128(r, c0 + swap)) = swap ? hi4 : lo4;
-                *reinterpret_cast<uint4*>(half + sw128(r, c0 + 1 - swap)) = swap ? lo4 : hi4;
+                const uint4 lo4 = make_uint4(o[0], o[1], o[2], o[3]), hi4 = make_uint4(o[4], o[5], o[6], o[7]);
+                *reinterpret_cast<uint4*>(half + sw128(ri, c0 + swap)) = swap ? hi4 : lo4;
+                *reinterpret_cast<uint4*>(half + sw128(ri, c0 + 1 - swap)) = swap ? lo4 : hi4;
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
         };
-        // a barrier of the four warps; true when one of them has given up
+        // a barrier of the producers; true when one of them has given up
         auto sync = [](bool dead) {
             uint32_t any;
             asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n"
@@ -636,17 +686,19 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             return any != 0;
         };
         // tile it is stored, it + 1's bytes are loaded, it + 2's scales and it + 3's page numbers requested
-        int row = -1, page = 0, line = -1, h0 = 0, h1 = 0, h2 = 0, h3 = 0;
+        int ring = 0, row = -1, page = 0, line = -1, h0 = 0, h1 = 0, h2 = 0, h3 = 0;
         float ks[4], vs[4];
-        uint4 xk[NCH], xv[NCH];
         bool more0 = step(page, line, h0), more1 = false, more2 = false, more3 = false, dead = false;
         if (more0) {
             row = finish(page, line);
             load_scales(row, h0, ks, vs);
             publish(0, row, ks, vs);
             sync(false);
-            load(a.kv.Kq, 0, h0, xk);
-            load(a.kv.Vq, 0, h0, xv);
+#pragma unroll
+            for (int x = 0; x < L::NU; x++) {                       // the ring, from unit 0 on
+                load(x, 0, h0, x);
+                cp_async_commit();
+            }
             if ((more1 = step(page, line, h1))) {
                 row = finish(page, line);
                 load_scales(row, h1, ks, vs);
@@ -664,16 +716,26 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 load_scales(row, h2, ks, vs);
                 more3 = step(page, line, h3);
             }
-            dead = !wait_warp(&k_empty[s], par);
+#pragma unroll
+            for (int x = 0; x < 2 * L::UNITS; x++) {
+                if (x == 0 || x == L::UNITS) {
+                    dead = !wait_warp(x == 0 ? &k_empty[s] : &v_empty[s], par);
+                    if (dead) break;
+                }
+                cp_async_wait<L::NU - 1>();                         // the thread's own copies of this unit
+                store(x, smem + (x < L::UNITS ? L::OFF_K : L::OFF_V) + s * L::TILE, buf, ring);
+                if (x == L::UNITS - 1 || x == 2 * L::UNITS - 1) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(x < L::UNITS ? &k_full[s] : &v_full[s]);
+                }
+                // the unit NU on: of this tile or the next
+                if (x + L::NU < 2 * L::UNITS) load(x + L::NU, buf, h0, ring);
+                else if (more1) load(x + L::NU - 2 * L::UNITS, nb, h1, ring);
+                cp_async_commit();
+                ring = ring + 1 == L::NU ? 0 : ring + 1;
+            }
             if (dead) continue;                                     // all leave at the next barrier
-            store(smem + L::OFF_K + s * L::TILE, buf, 0, xk);
-            if (lane == 0) mbar_arrive(&k_full[s]);
-            if (more1) load(a.kv.Kq, nb, h1, xk);
-            dead = !wait_warp(&v_empty[s], par);
-            if (dead) continue;
-            store(smem + L::OFF_V + s * L::TILE, buf, 1, xv);
-            if (lane == 0) mbar_arrive(&v_full[s]);
-            if (more1) load(a.kv.Vq, nb, h1, xv);
             more0 = more1;
             more1 = more2;
             more2 = more3;
@@ -684,51 +746,37 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         }
     } else {
         // ================================ MMAs ==========================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
-        if (warp == 12 && lane == 0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == W_MMA) {
             constexpr uint32_t I1 = idesc(PK, false), I2 = idesc(HD, true);
-            const uint32_t base = smem_u32(smem);
-            int it = 0;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint64_t dq = desc_k(smem_u32(smem) + L::OFF_Q), dk = desc_k(smem_u32(smem) + L::OFF_K),
+                           dv = desc_mn(smem_u32(smem) + L::OFF_V);
             uint32_t ph = 0;                               // parities of q_full (bits 0, 1) and p_full (2, 3)
-            bool ok = true;
-            auto wait = [&](uint64_t* bar, uint32_t parity) {
-                if (ok && !mbar_wait(bar, parity, abort_flag)) {
-                    give_up();
-                    ok = false;
-                }
-                return ok;
-            };
-            auto scores = [&](int t, int s) {          // S_t = Q_t K^T
-                const uint32_t qa = base + L::OFF_Q + t * L::TILE, kb = base + L::OFF_K + s * L::TILE;
+            auto scores = [&](int t, int s) {              // S_t = Q_t K^T
 #pragma unroll
-                for (int c = 0; c < HD / 16; c++) {
-                    const uint32_t at = (uint32_t)((c >> 2) * L::HALF + (c & 3) * 32);
-                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}"
-                                 ::"r"(tmem + 128 * t), "l"(desc_k(qa + at)), "l"(desc_k(kb + at)), "r"(I1),
-                                   "r"(c > 0 ? 1u : 0u), "r"(0u) : "memory");
-                }
+                for (int c = 0; c < HD / 64; c++)
+                    mma_ss(tm + 128 * t, dq + (t * L::TILE + c * L::HALF) / 16, dk + (s * L::TILE + c * L::HALF) / 16, I1, c);
                 tc_commit(&s_full[t]);
             };
-            auto output = [&](int t, int s, bool add) {   // O_t (+)= P_t V
-                const uint32_t vb = base + L::OFF_V + s * L::TILE;
+            auto output = [&](int t, int s, bool add) {    // O_t (+)= P_t V
 #pragma unroll
-                for (int c = 0; c < PK / 16; c++)
-                    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}"
-                                 ::"r"(tmem + 256 + HD * t), "r"(tmem + 128 * t + 8 * c), "l"(desc_mn(vb + 2048 * c)),
-                                   "r"(I2), "r"(add || c > 0 ? 1u : 0u), "r"(0u) : "memory");
+                for (int c = 0; c < PK / 64; c++)
+                    mma_ts(tm + 256 + HD * t, tm + 128 * t + 32 * c, dv + (s * L::TILE + c * 64 * 128) / 16, I2,
+                           add || c > 0 ? 1u : 0u);
                 tc_commit(&o_done[t]);
             };
+            int it = 0;
+            bool ok = true;
             for (int k = 0; ok && k * grid < total; k++) {
                 const int i = nth(k, cta, grid);
                 if (i >= total) continue;
-                const Part p = a.parts[i / nKv];
-                const int nt = p.t1 - p.t0, tiles = p.nq * GRP > 128 ? 2 : 1;
+                const Part* p = a.parts + i / nKv;
+                const int nt = p->t1 - p->t0, tiles = p->nq * GRP > 128 ? 2 : 1;
                 if (nt <= 0) continue;
-                if (!wait(&k_full[it % KV_STAGES], (it / KV_STAGES) & 1)) break;
+                if (!(ok = wait_warp(&k_full[it % KV_STAGES], (it / KV_STAGES) & 1))) break;
                 for (int t = 0; t < tiles && ok; t++) {
-                    if (!wait(&q_full[t], (ph >> t) & 1)) break;
+                    if (!(ok = wait_warp(&q_full[t], (ph >> t) & 1))) break;
                     ph ^= 1u << t;
                     tc_after();
                     scores(t, it % KV_STAGES);
@@ -737,15 +785,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 tc_commit(&k_empty[it % KV_STAGES]);
                 for (int j = 0; j < nt && ok; j++, it++) {
                     const int s = it % KV_STAGES, sn = (it + 1) % KV_STAGES;
-                    if (!wait(&v_full[s], (it / KV_STAGES) & 1)) break;
+                    if (!(ok = wait_warp(&v_full[s], (it / KV_STAGES) & 1))) break;
                     for (int t = 0; t < tiles; t++) {
-                        if (!wait(&p_full[t], (ph >> (2 + t)) & 1)) break;
+                        if (!(ok = wait_warp(&p_full[t], (ph >> (2 + t)) & 1))) break;
                         ph ^= 4u << t;
                         tc_after();
                         output(t, s, j > 0);
                         if (j + 1 < nt) {
                             if (t == 0) {
-                                if (!wait(&k_full[sn], ((it + 1) / KV_STAGES) & 1)) break;
+                                if (!(ok = wait_warp(&k_full[sn], ((it + 1) / KV_STAGES) & 1))) break;
                                 tc_after();
                             }
                             scores(t, sn);
@@ -757,13 +805,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 }
             }
             tc_commit(done);
-            if (!mbar_wait(done, 0)) give_up();            // no MMA in flight past here
+            if (!mbar_wait(done, 0) && lane == 0) give_up();            // no MMA in flight past here
+            __syncwarp();
         }
-        __syncwarp();
     }
     tc_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == W_MMA) {
         tc_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
     }

@@ -8,7 +8,6 @@
 // cache does not depend on how a row's sum was split or in which call it was written
 // (f32 sums put a byte one step off wherever they differ next to a rounding border);
 // 64-bit FMAs run at half the f32 rate here and the kernel stays bound by its bytes.
-#include "tb_attn_dev.cuh"
 #include "tb_paged.cuh"
 
 namespace {
@@ -23,6 +22,11 @@ struct PrepArgs {
     double theta, eps;
 };
 
+// floor(0.5 + 127 x) of x clamped to [-1, 1] (pack4x8snorm)
+__device__ __forceinline__ int8_t snorm8(float x)
+{
+    return (int8_t)floorf(__fadd_rn(0.5f, __fmul_rn(127.0f, fminf(1.0f, fmaxf(-1.0f, x)))));
+}
 __device__ __forceinline__ double warp_sum_f64(double v)
 {
 #pragma unroll
