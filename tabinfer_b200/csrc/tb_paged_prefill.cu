@@ -62,15 +62,15 @@ struct PrefillArgs {
     int* head;              // parts, items
     Part* parts;
     Item* items;
-    float* PO;              // [slot][nKv][ROWS][HD]
+    float* PO;              // [slot][nKv][HD][ROWS]: a thread holds a row, so a warp writes 128 contiguous bytes
     float2* PML;            // [slot][nKv][ROWS]
     int T, nHq, grp, window, sinks, sms, max_items, max_parts, max_slots;
     float sl2;              // log2(e) / sqrt(HD)
 };
 
 // ---- the plan: one CTA ---------------------------------------------------------------
-// Items of a sequence and the sum over all threads of a value
-constexpr int PT = 1024;
+constexpr int PT = 256, CLASS_BITS = 8;      // threads, and as many classes of part lengths
+static_assert(PT == 1 << CLASS_BITS, "a thread a class");
 
 __device__ int block_scan(int x, int* buf, int* total)      // inclusive; buf: PT / 32 words
 {
@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(PT) k_prefill_plan(const PrefillArgs a)
     __shared__ int first[MAX_BATCH + 1];      // items below each sequence
     __shared__ int buf[PT / 32], hist[PT];
     __shared__ unsigned long long all_tiles;
+    __shared__ int split;
     tb_pdl_wait();
     tb_pdl_trigger();
     const int tid = threadIdx.x, B = a.kv.batch, qb = ROWS / a.grp;
@@ -125,40 +126,44 @@ __global__ void __launch_bounds__(PT) k_prefill_plan(const PrefillArgs a)
         return;
     }
     // the item's queries and tiles
-    auto item = [&](int i, int& b, int& row0, int& nq, int& p0, int& nt) {
+    struct Shape {
+        int b, row0, nq, p0, nt;
+    };
+    auto item = [&](int i) {
+        Shape v;
         int lo = 0, hi = B;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (first[mid] <= i) lo = mid;
             else hi = mid;
         }
-        b = lo;
-        const int c0 = a.cu[b], rows = a.cu[b + 1] - c0, at = (i - first[b]) * qb;
-        const int n = a.kv.checked_len(a.lens[b]);
-        row0 = c0 + at;
-        nq = min(qb, rows - at);
-        p0 = n - rows + at;
-        nt = SeenTiles(max(p0, 0), p0 + nq - 1, a.window, a.sinks, PK).count;
-        if (p0 < 0) atomicExch(a.kv.err, ERR_PAGED_LEN);
+        v.b = lo;
+        const int c0 = a.cu[lo], rows = a.cu[lo + 1] - c0, at = (i - first[lo]) * qb;
+        const int n = a.kv.checked_len(a.lens[lo]);
+        v.row0 = c0 + at;
+        v.nq = min(qb, rows - at);
+        v.p0 = n - rows + at;
+        v.nt = SeenTiles(max(v.p0, 0), v.p0 + v.nq - 1, a.window, a.sinks, PK).count;
+        if (v.p0 < 0) atomicExch(a.kv.err, ERR_PAGED_LEN);
+        return v;
     };
-    unsigned long long tiles = 0;
-    for (int i = tid; i < items; i += PT) {
-        int b, row0, nq, p0, nt;
-        item(i, b, row0, nq, p0, nt);
-        tiles += nt;
+    // the thread's first item stays in registers
+    const Shape own = tid < items ? item(tid) : Shape{0, 0, 0, 0, 0};
+    unsigned long long tiles = own.nt;
+    for (int i = tid + PT; i < items; i += PT) tiles += item(i).nt;
+    if (tid == 0) {
+        all_tiles = 0;
+        split = 0;
     }
-    if (tid == 0) all_tiles = 0;
     __syncthreads();
     for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
     if ((tid & 31) == 0) atomicAdd(&all_tiles, tiles);
     __syncthreads();
     // the longest part: a CTA's share of all heads' tiles
     const int share = (int)min(1ull << 24, max((unsigned long long)MIN_TILES, (all_tiles * a.kv.nKv + a.sms - 1) / a.sms));
-    const int shift = max(0, 32 - __clz(share) - 10);          // part lengths as at most PT classes
+    const int shift = max(0, 32 - __clz(share) - CLASS_BITS);  // part lengths as at most PT classes
     for (int i = tid; i < items; i += PT) {
-        int b, row0, nq, p0, nt;
-        item(i, b, row0, nq, p0, nt);
-        const int np = max(1, (nt + share - 1) / share);
+        const int nt = i == tid ? own.nt : item(i).nt, np = max(1, (nt + share - 1) / share);
         for (int k = 0; k < np; k++)
             atomicAdd(&hist[((k + 1) * nt / np - k * nt / np) >> shift], 1);
     }
@@ -173,26 +178,25 @@ __global__ void __launch_bounds__(PT) k_prefill_plan(const PrefillArgs a)
     int slots = 0;
     for (int i0 = 0; i0 < items; i0 += PT) {
         const int i = i0 + tid;
-        int b = 0, row0 = 0, nq = 0, p0 = 0, nt = 0, np = 0;
-        if (i < items) {
-            item(i, b, row0, nq, p0, nt);
-            np = max(1, (nt + share - 1) / share);
-        }
+        Shape v = own;
+        if (i0 > 0 && i < items) v = item(i);
+        const int nt = v.nt, np = i < items ? max(1, (nt + share - 1) / share) : 0;
         int all;
         const int mine_slots = np > 1 ? np : 0;
         const int s0 = slots + block_scan(mine_slots, buf, &all) - mine_slots;
         slots += all;
         if (i >= items) continue;
-        a.items[i] = Item{row0, nq, s0, np};
+        if (np > 1) a.items[atomicAdd(&split, 1)] = Item{v.row0, v.nq, s0, np};
         for (int k = 0; k < np; k++) {
             const int t0 = k * nt / np, t1 = (k + 1) * nt / np;
             const int at = atomicAdd(&hist[(t1 - t0) >> shift], 1);
-            if (at < a.max_parts) a.parts[at] = Part{b, row0, nq, p0, t0, t1, np > 1 ? s0 + k : -1, 0};
+            if (at < a.max_parts) a.parts[at] = Part{v.b, v.row0, v.nq, v.p0, t0, t1, np > 1 ? s0 + k : -1, 0};
         }
     }
+    __syncthreads();
     if (tid == 0) {
         a.head[0] = min(parts, a.max_parts);
-        a.head[1] = items;
+        a.head[1] = split;                    // the items that were cut
     }
 }
 
@@ -250,13 +254,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r)
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
                  "%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : TB_R32(r) : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r)
-{
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r)
 {
@@ -331,9 +328,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     uint64_t* v_full = k_empty + KV_STAGES;
     uint64_t* v_empty = v_full + KV_STAGES;
     uint64_t* s_full = v_empty + KV_STAGES;                                 // [2] S written
-    uint64_t* p_full = s_full + 2;                                          // [2] P written, O rescaled
-    uint64_t* o_done = p_full + 2;                                          // [2] O += P V completed
-    uint64_t* done = o_done + 2;                                            // every MMA completed
+    uint64_t* p_full = s_full + 2;                                          // [2][2] a half of P written, O rescaled
+    uint64_t* o_done = p_full + 4;                                          // [2][2] O += P V of a half completed
+    uint64_t* done = o_done + 4;                                            // every MMA completed
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(done + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(done + 2);
 
@@ -342,8 +339,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_full[i], 4);
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&o_done[i], 1);
+            mbar_init(&p_full[2 * i], 4);
+            mbar_init(&p_full[2 * i + 1], 4);
+            mbar_init(&o_done[2 * i], 1);
+            mbar_init(&o_done[2 * i + 1], 1);
         }
         for (int i = 0; i < KV_STAGES; i++) {
             mbar_init(&k_full[i], PROD / 32);
@@ -381,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
 
     if (warp < 8) {
         // =============================== softmax ======================================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");      // 256 x 152 + 128 x 128 + 128 x 80 = 65536
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");      // 256 x 152 + 128 x 120 + 128 x 88 = 65536
         const int t = warp >> 2, wq = warp & 3, row = 32 * wq + lane;      // row of the tile
         const uint32_t ts = tmem + ((uint32_t)(32 * wq) << 16) + 128 * t;
         const uint32_t to = tmem + ((uint32_t)(32 * wq) << 16) + 256 + HD * t;
@@ -389,7 +388,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         // Q rows of this warp: row r of the item = query r / GRP, head r % GRP
         auto load_q = [&](const Part& p, int h) {
             constexpr int C4 = HD / 4;                          // float4 columns a row
-#pragma unroll 4
+#pragma unroll 8
             for (int i = lane; i < 32 * C4; i += 32) {
                 const int r = 32 * wq + i / C4, c = i % C4, ir = 128 * t + r, qi = ir / GRP;
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -439,85 +438,92 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 const bool cut = k0 + PK - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window && k0 + PK > a.sinks) ||
                                  (bw.x | bw.y | bw.z | bw.w);
                 const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
-                auto mask = [&](int c0, float* s) {
-                    const uint32_t w = (c0 < 32 ? bw.x : c0 < 64 ? bw.y : c0 < 96 ? bw.z : bw.w) >> (c0 & 31);
+                // In two halves of 64 keys, so that the first half's product runs under the second's softmax.
+                // One pass over a half's scores against the reference maximum as it stands; a score that
+                // passes it by 2^RAISE raises it, rescales O (every column, once the last product is in) and
+                // repeats the pass.  The first half's maximum comes first.
+#pragma unroll 1
+                for (int hh = 0; hh < 2; hh++) {
+                    const bool fresh = j == p.t0 && hh == 0;
+                    const uint32_t th = ts + 64 * hh;
+                    auto mask = [&](int c0, float* s) {
+                        const uint32_t w = (hh == 0 ? (c0 < 32 ? bw.x : bw.y) : (c0 < 32 ? bw.z : bw.w)) >> (c0 & 31);
 #pragma unroll
-                    for (int c = 0; c < 16; c++)
-                        if (!(c0 + c <= hi && (c0 + c > lo || c0 + c < sk)) || ((w >> c) & 1)) s[c] = -INFINITY;
-                };
-                // One pass over the scores against the reference maximum as it stands; a score that passes it
-                // by 2^RAISE raises it, rescales O (every column, once the last product is in) and repeats
-                // the pass.  The first tile's maximum comes first.
-                if (j == p.t0) {
-                    float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        for (int c = 0; c < 16; c++) {
+                            const int k = 64 * hh + c0 + c;
+                            if (!(k <= hi && (k > lo || k < sk)) || ((w >> c) & 1)) s[c] = -INFINITY;
+                        }
+                    };
+                    if (fresh) {
+                        float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        float s[32];
-                        tmem_ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(s));
+                        for (int c = 0; c < 2; c++) {
+                            float s[32];
+                            tmem_ld32(th + 32 * c, reinterpret_cast<uint32_t*>(s));
+                            tmem_wait_ld();
+                            if (cut) {
+                                mask(32 * c, s);
+                                mask(32 * c + 16, s + 16);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 32; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
+                        }
+                        m = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.sl2;
+                    }
+                    uint32_t pk[32];
+                    float2 sum;
+                    for (;;) {
+                        const float off = m == -INFINITY ? 0.0f : -m;
+                        float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                        float t2[2] = {-INFINITY, -INFINITY};
+                        float x[64];                      // all of the half at once: one wait, and the exponentials
+                        tmem_ld32(th, reinterpret_cast<uint32_t*>(x));       // back to back (16 at a time took twice as long)
+                        tmem_ld32(th + 32, reinterpret_cast<uint32_t*>(x) + 32);
                         tmem_wait_ld();
                         if (cut) {
-                            mask(32 * c, s);
-                            mask(32 * c + 16, s + 16);
+#pragma unroll
+                            for (int c = 0; c < 4; c++) mask(16 * c, x + 16 * c);
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
-                    }
-                    m = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.sl2;
-                }
-                uint32_t pk[64];
-                float2 sum;
-                for (;;) {
-                    const float off = m == -INFINITY ? 0.0f : -m;
-                    float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                    float t2[2] = {-INFINITY, -INFINITY};
-                    float sc[2][16];
-                    tmem_ld16(ts, reinterpret_cast<uint32_t*>(sc[0]));
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int c = 0; c < 8; c++) {
-                        float* x = sc[c & 1];
-                        if (c < 7) tmem_ld16(ts + 16 * (c + 1), reinterpret_cast<uint32_t*>(sc[(c + 1) & 1]));
-                        if (cut) mask(16 * c, x);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
+                        for (int i = 0; i < 32; i++) {
                             const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2),
                                                    make_float2(off, off));
                             t2[i & 1] = fmaxf(t2[i & 1], fmaxf(y.x, y.y));
                             const float2 e = make_float2(ex2(y.x), ex2(y.y));
                             s2[i & 1] = fadd2(s2[i & 1], e);
-                            pk[8 * c + i] = pack_h2(e.x, e.y);
+                            pk[i] = pack_h2(e.x, e.y);
                         }
-                        if (c < 7) tmem_wait_ld();
-                    }
-                    sum = fadd2(s2[0], s2[1]);
-                    const float top = fmaxf(t2[0], t2[1]);           // the maximum, from the reference
-                    const bool up = top > (m == -INFINITY ? -INFINITY : RAISE);
-                    if (!__any_sync(0xffffffffu, up)) break;
-                    if (j > p.t0) {
-                        if (!(ok = wait_warp(&o_done[t], (seq - 1) & 1))) break;
-                        tc_after();
-                        const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(-top);
+                        sum = fadd2(s2[0], s2[1]);
+                        const float top = fmaxf(t2[0], t2[1]);           // the maximum, from the reference
+                        const bool up = top > (m == -INFINITY ? -INFINITY : RAISE);
+                        if (!__any_sync(0xffffffffu, up)) break;
+                        if (!fresh) {
+                            // the half before: the last tile's second, or this tile's first
+                            if (!(ok = wait_warp(&o_done[2 * t + (hh ^ 1)], (hh ? seq : seq - 1) & 1))) break;
+                            tc_after();
+                            const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(-top);
 #pragma unroll
-                        for (int c = 0; c < HD / 32; c++) {
-                            uint32_t o[32];
-                            tmem_ld32(to + 32 * c, o);
-                            tmem_wait_ld();
+                            for (int c = 0; c < HD / 32; c++) {
+                                uint32_t o[32];
+                                tmem_ld32(to + 32 * c, o);
+                                tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_st32(to + 32 * c, o);
+                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_st32(to + 32 * c, o);
+                            }
+                            l *= f;
                         }
-                        l *= f;
+                        if (up) m = m == -INFINITY ? top : m + top;
                     }
-                    if (up) m = m == -INFINITY ? top : m + top;
+                    if (!ok) break;
+                    tmem_st32(ts + 32 * hh, pk);          // over scores that are read
+                    l += sum.x + sum.y;
+                    tmem_wait_st();
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&p_full[2 * t + hh]);
                 }
                 if (!ok) break;
-                tmem_st32(ts, pk);
-                tmem_st32(ts + 32, pk + 32);
-                l += sum.x + sum.y;
-                tmem_wait_st();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[t]);
             }
             if (!ok) break;
             // the next part's Q goes in under this part's last product
@@ -525,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             int hn = 0;
             const int kn = find(k + 1, pn, hn);
             if (kn >= 0) load_q(pn, hn);
-            if (!wait_warp(&o_done[t], (seq - 1) & 1)) break;
+            if (!wait_warp(&o_done[2 * t + 1], (seq - 1) & 1)) break;
             tc_after();
             const bool live = qi < p.nq;
             const long long slot = p.slot < 0 ? 0 : (long long)p.slot * nKv + h;
@@ -537,11 +543,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 tmem_ld32(to + 32 * c, o);
                 tmem_wait_ld();
                 if (p.slot >= 0) {
-                    float4* dst = reinterpret_cast<float4*>(a.PO + (slot * ROWS + 128 * t + row) * HD + 32 * c);
+                    float* dst = a.PO + (slot * HD + 32 * c) * ROWS + 128 * t + row;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                             __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    for (int i = 0; i < 32; i++) dst[i * ROWS] = __uint_as_float(o[i]);
                 } else if (live) {
                     uint4* dst = reinterpret_cast<uint4*>(
                         a.out + ((long long)(p.row0 + qi) * a.nHq + h * GRP + (128 * t + row) % GRP) * HD + 32 * c);
@@ -565,6 +569,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         }
     } else if (warp < W_MMA) {
         // ============================ K / V tiles ======================================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
                 const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
         int* rows = reinterpret_cast<int*>(smem + L::OFF_ROW);
         uint2* scs = reinterpret_cast<uint2*>(smem + L::OFF_SC);    // [3][2][PK] four f16 scales
@@ -746,7 +751,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         }
     } else {
         // ================================ MMAs ==========================================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == W_MMA) {
             constexpr uint32_t I1 = idesc(PK, false), I2 = idesc(HD, true);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -759,12 +764,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     mma_ss(tm + 128 * t, dq + (t * L::TILE + c * L::HALF) / 16, dk + (s * L::TILE + c * L::HALF) / 16, I1, c);
                 tc_commit(&s_full[t]);
             };
-            auto output = [&](int t, int s, bool add) {    // O_t (+)= P_t V
-#pragma unroll
-                for (int c = 0; c < PK / 64; c++)
-                    mma_ts(tm + 256 + HD * t, tm + 128 * t + 32 * c, dv + (s * L::TILE + c * 64 * 128) / 16, I2,
-                           add || c > 0 ? 1u : 0u);
-                tc_commit(&o_done[t]);
+            auto output = [&](int t, int s, int c, bool add) {   // O_t (+)= P_t V over half c of the tile's keys
+                mma_ts(tm + 256 + HD * t, tm + 128 * t + 32 * c, dv + (s * L::TILE + c * 64 * 128) / 16, I2, add ? 1u : 0u);
+                tc_commit(&o_done[2 * t + c]);
             };
             int it = 0;
             bool ok = true;
@@ -787,10 +789,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     const int s = it % KV_STAGES, sn = (it + 1) % KV_STAGES;
                     if (!(ok = wait_warp(&v_full[s], (it / KV_STAGES) & 1))) break;
                     for (int t = 0; t < tiles; t++) {
-                        if (!(ok = wait_warp(&p_full[t], (ph >> (2 + t)) & 1))) break;
+                        for (int c = 0; c < 2; c++) {
+                            if (!(ok = wait_warp(&p_full[2 * t + c], (ph >> (2 + t)) & 1))) break;
+                            tc_after();
+                            output(t, s, c, j > 0 || c > 0);
+                        }
+                        if (!ok) break;
                         ph ^= 4u << t;
-                        tc_after();
-                        output(t, s, j > 0);
                         if (j + 1 < nt) {
                             if (t == 0) {
                                 if (!(ok = wait_warp(&k_full[sn], ((it + 1) / KV_STAGES) & 1))) break;
@@ -817,39 +822,47 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     }
 }
 
-// joins the parts of item x, kv head y, rows 32 z ..: a warp four rows at a time
+// joins the parts of item x, kv head y, rows 32 z ..: lane = row, a warp takes CW columns
+constexpr int JT = 512;
 template <int HD, int GRP>
-__global__ void __launch_bounds__(256) k_prefill_join(const __grid_constant__ PrefillArgs a)
+__global__ void __launch_bounds__(JT) k_prefill_join(const __grid_constant__ PrefillArgs a)
 {
+    constexpr int CW = HD / (JT / 32);
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int i = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nKv = a.kv.nKv;
-    if (i >= a.head[1]) return;
-    const Item it = a.items[i];
-    if (it.parts < 2) return;
-    for (int k = 0; k < 4; k++) {
-        const int row = 32 * blockIdx.z + 4 * wid + k, qi = row / GRP;
-        if (qi >= it.nq) return;
+    const int h = blockIdx.y, nKv = a.kv.nKv, c0 = (threadIdx.x >> 5) * CW;
+    const int row = 32 * blockIdx.z + (threadIdx.x & 31), qi = row / GRP;
+    for (int i = blockIdx.x; i < a.head[1]; i += gridDim.x) {
+        const Item it = a.items[i];
+        if (it.parts < 2 || 32 * (int)blockIdx.z >= it.nq * GRP) continue;
+        const float2* pml = a.PML + ((long long)it.slot0 * nKv + h) * ROWS + row;
+        const float* po = a.PO + (((long long)it.slot0 * nKv + h) * HD + c0) * ROWS + row;
         float M = -INFINITY;
-        for (int p = 0; p < it.parts; p++)
-            M = fmaxf(M, a.PML[((long long)(it.slot0 + p) * nKv + h) * ROWS + row].x);
+#pragma unroll 8
+        for (int p = 0; p < it.parts; p++) M = fmaxf(M, pml[(long long)p * nKv * ROWS].x);
         const float off = M == -INFINITY ? 0.0f : M;
-        float l = 0.0f, o[HD / 32];
+        float l = 0.0f, o[CW];
 #pragma unroll
-        for (int c = 0; c < HD / 32; c++) o[c] = 0.0f;
+        for (int c = 0; c < CW; c++) o[c] = 0.0f;
 #pragma unroll 4
         for (int p = 0; p < it.parts; p++) {
-            const long long s = ((long long)(it.slot0 + p) * nKv + h) * ROWS + row;
-            const float2 ml = a.PML[s];
+            const float2 ml = pml[(long long)p * nKv * ROWS];
             const float e = exp2f(ml.x - off);
             l = fmaf(ml.y, e, l);
 #pragma unroll
-            for (int c = 0; c < HD / 32; c++) o[c] = fmaf(a.PO[s * HD + 32 * c + lane], e, o[c]);
+            for (int c = 0; c < CW; c++) o[c] = fmaf(po[((long long)p * nKv * HD + c) * ROWS], e, o[c]);
         }
+        if (qi >= it.nq) continue;
         const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        __nv_bfloat16* dst = a.out + ((long long)(it.row0 + qi) * a.nHq + h * GRP + row % GRP) * HD;
+        uint32_t w[CW / 2];
 #pragma unroll
-        for (int c = 0; c < HD / 32; c++) dst[32 * c + lane] = __float2bfloat16_rn(o[c] * r);
+        for (int c = 0; c < CW / 2; c++) {
+            const __nv_bfloat162 v = __floats2bfloat162_rn(o[2 * c] * r, o[2 * c + 1] * r);
+            w[c] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        __nv_bfloat16* dst = a.out + ((long long)(it.row0 + qi) * a.nHq + h * GRP + row % GRP) * HD + c0;
+        if constexpr (CW == 8) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
     }
 }
 
@@ -890,7 +903,8 @@ int launch_prefill(tb_ctx* ctx, const PrefillArgs& a)
     if (e == cudaSuccess) e = tb_launch(ctx, k_prefill_plan, dim3(1), dim3(PT), 0, a);
     const int grid = (int)std::min<long long>(a.sms, (long long)a.max_parts * a.kv.nKv);
     if (e == cudaSuccess) e = tb_launch(ctx, kern, dim3(grid), dim3(THREADS), (size_t)smem, a);
-    if (e == cudaSuccess) e = tb_launch(ctx, k_prefill_join<HD, GRP>, dim3(a.max_items, a.kv.nKv, ROWS / 32), dim3(256), 0, a);
+    if (e == cudaSuccess) e = tb_launch(ctx, k_prefill_join<HD, GRP>, dim3(std::min(a.max_items, a.max_slots), a.kv.nKv, ROWS / 32),
+                                           dim3(JT), 0, a);
     if (e != cudaSuccess) return tb_fail(ctx, TB_ERR_CUDA, "attn_prefill_paged launch: %s", cudaGetErrorString(e));
     return TB_OK;
 }
