@@ -62,7 +62,9 @@ struct PrefillArgs {
     int* head;              // parts, items
     Part* parts;
     Item* items;
-    float* PO;              // [slot][nKv][HD][ROWS]: a thread holds a row, so a warp writes 128 contiguous bytes
+    // [slot][nKv][HD / 2][ROWS]: O / l as pairs of f16 (the operands' own rounding, half the bytes); a thread
+    // holds a row, so a warp writes 128 contiguous bytes
+    uint32_t* PO;
     float2* PML;            // [slot][nKv][ROWS]
     int T, nHq, grp, window, sinks, sms, max_items, max_parts, max_slots;
     float sl2;              // log2(e) / sqrt(HD)
@@ -313,6 +315,9 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// bits 0 .. n - 1 (n clamped to 0 .. 32)
+__device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
 // the k-th (part, head) of CTA c: rounds over the list, every other one backwards
 __device__ __forceinline__ int nth(int k, int c, int grid) { return k * grid + ((k & 1) ? grid - 1 - c : c); }
 
@@ -388,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         // Q rows of this warp: row r of the item = query r / GRP, head r % GRP
         auto load_q = [&](const Part& p, int h) {
             constexpr int C4 = HD / 4;                          // float4 columns a row
-#pragma unroll 8
+#pragma unroll 16
             for (int i = lane; i < 32 * C4; i += 32) {
                 const int r = 32 * wq + i / C4, c = i % C4, ir = 128 * t + r, qi = ir / GRP;
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -446,13 +451,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 for (int hh = 0; hh < 2; hh++) {
                     const bool fresh = j == p.t0 && hh == 0;
                     const uint32_t th = ts + 64 * hh;
-                    auto mask = [&](int c0, float* s) {
-                        const uint32_t w = (hh == 0 ? (c0 < 32 ? bw.x : bw.y) : (c0 < 32 ? bw.z : bw.w)) >> (c0 & 31);
+                    // the half's keys that this row sees, as bits
+                    uint32_t see0 = ~0u, see1 = ~0u;
+                    if (cut) {
+                        const int h0 = hi - 64 * hh, l0 = lo - 64 * hh, s0 = sk - 64 * hh;
+                        see0 = below(h0 + 1) & (~below(l0 + 1) | below(s0)) & ~(hh ? bw.z : bw.x);
+                        see1 = below(h0 - 31) & (~below(l0 - 31) | below(s0 - 32)) & ~(hh ? bw.w : bw.y);
+                    }
+                    auto mask = [&](float* s, uint32_t see) {
 #pragma unroll
-                        for (int c = 0; c < 16; c++) {
-                            const int k = 64 * hh + c0 + c;
-                            if (!(k <= hi && (k > lo || k < sk)) || ((w >> c) & 1)) s[c] = -INFINITY;
-                        }
+                        for (int c = 0; c < 32; c++)
+                            if (!((see >> c) & 1)) s[c] = -INFINITY;
                     };
                     if (fresh) {
                         float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -461,10 +470,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                             float s[32];
                             tmem_ld32(th + 32 * c, reinterpret_cast<uint32_t*>(s));
                             tmem_wait_ld();
-                            if (cut) {
-                                mask(32 * c, s);
-                                mask(32 * c + 16, s + 16);
-                            }
+                            if (cut) mask(s, c ? see1 : see0);
 #pragma unroll
                             for (int i = 0; i < 32; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
                         }
@@ -481,8 +487,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                         tmem_ld32(th + 32, reinterpret_cast<uint32_t*>(x) + 32);
                         tmem_wait_ld();
                         if (cut) {
-#pragma unroll
-                            for (int c = 0; c < 4; c++) mask(16 * c, x + 16 * c);
+                            mask(x, see0);
+                            mask(x + 32, see1);
                         }
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
@@ -536,16 +542,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             const bool live = qi < p.nq;
             const long long slot = p.slot < 0 ? 0 : (long long)p.slot * nKv + h;
             if (p.slot >= 0) a.PML[slot * ROWS + 128 * t + row] = make_float2(m, l);
-            const float r = p.slot >= 0 ? 1.0f : (l > 0.0f || l != l ? 1.0f / l : 0.0f);
+            const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
                 uint32_t o[32];
                 tmem_ld32(to + 32 * c, o);
                 tmem_wait_ld();
                 if (p.slot >= 0) {
-                    float* dst = a.PO + (slot * HD + 32 * c) * ROWS + 128 * t + row;
+                    uint32_t* dst = a.PO + (slot * HD / 2 + 16 * c) * ROWS + 128 * t + row;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) dst[i * ROWS] = __uint_as_float(o[i]);
+                    for (int i = 0; i < 16; i++)
+                        dst[i * ROWS] = pack_h2(__uint_as_float(o[2 * i]) * r, __uint_as_float(o[2 * i + 1]) * r);
                 } else if (live) {
                     uint4* dst = reinterpret_cast<uint4*>(
                         a.out + ((long long)(p.row0 + qi) * a.nHq + h * GRP + (128 * t + row) % GRP) * HD + 32 * c);
@@ -697,13 +704,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         if (more0) {
             row = finish(page, line);
             load_scales(row, h0, ks, vs);
-            publish(0, row, ks, vs);
+            rows[pt] = max(row, 0);
             sync(false);
 #pragma unroll
             for (int x = 0; x < L::NU; x++) {                       // the ring, from unit 0 on
                 load(x, 0, h0, x);
                 cp_async_commit();
             }
+            publish(0, row, ks, vs);                                // seen after the loop's first barrier
             if ((more1 = step(page, line, h1))) {
                 row = finish(page, line);
                 load_scales(row, h1, ks, vs);
@@ -836,7 +844,7 @@ __global__ void __launch_bounds__(JT) k_prefill_join(const __grid_constant__ Pre
         const Item it = a.items[i];
         if (it.parts < 2 || 32 * (int)blockIdx.z >= it.nq * GRP) continue;
         const float2* pml = a.PML + ((long long)it.slot0 * nKv + h) * ROWS + row;
-        const float* po = a.PO + (((long long)it.slot0 * nKv + h) * HD + c0) * ROWS + row;
+        const uint32_t* po = a.PO + (((long long)it.slot0 * nKv + h) * HD / 2 + c0 / 2) * ROWS + row;
         float M = -INFINITY;
 #pragma unroll 8
         for (int p = 0; p < it.parts; p++) M = fmaxf(M, pml[(long long)p * nKv * ROWS].x);
@@ -847,10 +855,15 @@ __global__ void __launch_bounds__(JT) k_prefill_join(const __grid_constant__ Pre
 #pragma unroll 4
         for (int p = 0; p < it.parts; p++) {
             const float2 ml = pml[(long long)p * nKv * ROWS];
-            const float e = exp2f(ml.x - off);
-            l = fmaf(ml.y, e, l);
+            const float e = ml.y * exp2f(ml.x - off);
+            l += e;
 #pragma unroll
-            for (int c = 0; c < CW; c++) o[c] = fmaf(po[((long long)p * nKv * HD + c) * ROWS], e, o[c]);
+            for (int c = 0; c < CW / 2; c++) {
+                const uint32_t v = po[((long long)p * nKv * HD / 2 + c) * ROWS];
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                o[2 * c] = fmaf(f.x, e, o[2 * c]);
+                o[2 * c + 1] = fmaf(f.y, e, o[2 * c + 1]);
+            }
         }
         if (qi >= it.nq) continue;
         const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
@@ -885,7 +898,7 @@ PrefillWs prefill_ws(const tb_ctx* ctx, const tb_paged_kv* kv, int64_t nHq, int6
     w.o_items = w.o_parts + up((size_t)w.parts * sizeof(Part));
     w.o_pml = w.o_items + up((size_t)w.items * sizeof(Item));
     w.o_po = w.o_pml + up((size_t)w.slots * kv->nKv * ROWS * sizeof(float2));
-    w.bytes = w.o_po + up((size_t)w.slots * kv->nKv * ROWS * kv->hd * sizeof(float));
+    w.bytes = w.o_po + up((size_t)w.slots * kv->nKv * ROWS * kv->hd * sizeof(uint16_t));
     return w;
 }
 
@@ -963,7 +976,7 @@ TB_API int tb_attn_prefill_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, uint16_t
     a.parts = reinterpret_cast<Part*>(p + w.o_parts);
     a.items = reinterpret_cast<Item*>(p + w.o_items);
     a.PML = reinterpret_cast<float2*>(p + w.o_pml);
-    a.PO = reinterpret_cast<float*>(p + w.o_po);
+    a.PO = reinterpret_cast<uint32_t*>(p + w.o_po);
     a.T = (int)T;
     a.nHq = (int)nHq;
     a.grp = (int)(nHq / kv->nKv);
