@@ -10,7 +10,11 @@
 
 namespace {
 
-constexpr int ST = 1024;   // threads of a selecting CTA
+constexpr int ST = 1024;          // threads of a selecting CTA
+constexpr int DIGIT = 11, BINS = 1 << DIGIT;
+constexpr int MAX_CLUSTER = 8;    // CTAs a sequence (portable)
+constexpr int SLOTS = 2048;       // rows a CTA at least, before a sequence gets another one
+constexpr int KEPT_KEYS = 16;     // keys a thread holds in registers; those beyond are read again each step
 
 struct EvictArgs {
     PagedArgs kv, dst;
@@ -31,130 +35,247 @@ __device__ __forceinline__ unsigned long long score_key(double s)
     return (u >> 63) ? ~u : u | (1ull << 63);
 }
 
-__global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
+__device__ __forceinline__ void cluster_sync()
 {
-    __shared__ unsigned hist[256];
-    __shared__ unsigned long long prefix;
-    __shared__ int remaining, base_kept, base_tie;
-    __shared__ int wkept[ST / 32], wtie[ST / 32];
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// a word of another CTA's shared memory, at the place of `p` in this one's
+__device__ __forceinline__ unsigned remote(const void* p, int rank)
+{
+    uint32_t at;
+    unsigned v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// scores of the rows that are to be chosen from, as ordered numbers: grid (rows / 256, sequences)
+__global__ void __launch_bounds__(256) k_evict_scores(const EvictArgs a)
+{
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-    const int cap = a.kv.cap(), nKv = a.kv.nKv;
+    const int b = blockIdx.y, cap = a.kv.cap(), nKv = a.kv.nKv;
     const int n = a.kv.checked_len(__ldg(a.lens + b));
-    const int left = min(n, a.budget);
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    if (n <= a.budget || j < a.sinks || j >= n - a.recent) return;
+    const float* w = a.weights + (long long)b * nKv * cap + j;
+    double s = 0.0;
+#pragma unroll 8
+    for (int h = 0; h < nKv; h++) s += (double)__ldg(w + (long long)h * cap);
+    a.keys[(long long)b * cap + j] = score_key(s);
+}
+
+// A cluster a sequence.  Its CTAs share the middle rows (between the first and the last
+// ones that stay): the need-th largest score by radix, 11 bits a step from the top -- each
+// CTA counts its rows' digits, all add up the counts of all over distributed shared memory --
+// until the digit's whole class is needed (two or three steps where scores differ, six at
+// most), then the rows above it and, in order, as many of its class as are still needed.
+// Bound by the steps' barriers.
+__global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
+{
+    __shared__ unsigned hist[2][BINS];       // two: a step's counts are read while the next one's are made
+    __shared__ int wsum[ST / 32];
+    __shared__ int found_bin, found_left, found_all;
+    __shared__ int wkeep[ST / 32], wtie[ST / 32], mine[2];
+    tb_pdl_wait();
+    tb_pdl_trigger();
+    const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+    int rank, ncta;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
+    const int b = blockIdx.x / ncta, cap = a.kv.cap();
+    const int n = a.kv.checked_len(__ldg(a.lens + b)), left = min(n, a.budget);
+    const int gt = rank * ST + tid, gs = ncta * ST;          // the thread's place in the cluster
     int* kept = a.kept + (long long)b * a.budget;
-    if (tid == 0) a.new_lens[b] = left;
-    for (int i = left + tid; i < a.budget; i += ST) kept[i] = -1;
+    if (gt == 0) a.new_lens[b] = left;
     if (n <= a.budget) {
-        for (int i = tid; i < n; i += ST) kept[i] = i;
+        for (int i = gt; i < a.budget; i += gs) kept[i] = i < n ? i : -1;
         return;
     }
     const int lo = a.sinks, hi = n - a.recent, need = a.budget - a.sinks - a.recent;
+    for (int i = gt; i < a.sinks; i += gs) kept[i] = i;
+    for (int i = gt; i < a.recent; i += gs) kept[a.budget - a.recent + i] = hi + i;
+    if (need == 0) return;
+    // this CTA's rows
+    const int span = ((hi - lo + ncta - 1) / ncta + 31) & ~31;
+    const int j0 = min(hi, lo + rank * span), j1 = min(hi, j0 + span);
     unsigned long long* keys = a.keys + (long long)b * cap;
-    const float* w = a.weights + (long long)b * nKv * cap;
-    for (int j = lo + tid; j < hi; j += ST) {
-        double s = 0.0;
-        for (int h = 0; h < nKv; h++) s += (double)w[(long long)h * cap + j];
-        keys[j] = score_key(s);
+    unsigned long long own[KEPT_KEYS];
+#pragma unroll
+    for (int i = 0; i < KEPT_KEYS; i++) {
+        const int j = j0 + tid + i * ST;
+        own[i] = j < j1 ? keys[j] : 0;
     }
-    if (tid == 0) {
-        prefix = 0;
-        remaining = need;
+    unsigned long long prefix = 0;           // of the class looked at: the key's bits from `shift` on
+    int shift = 64, remaining = need;
+    for (int step = 0; shift > 0; step++) {
+        const int bits = min(DIGIT, shift), next = shift - bits;
+        unsigned* cnt = hist[step & 1];
+        for (int i = tid; i < BINS; i += ST) cnt[i] = 0;
+        __syncthreads();
+        // equal digits of a warp are added at once: of a step's rows most have the same few (scores of
+        // one magnitude share their upper bits; one addition a row took 100 us for 131072)
+        auto count = [&](unsigned long long k, int j) {
+            const bool in = j < j1 && (shift == 64 || (k >> shift) == prefix);
+            if (!__any_sync(0xffffffffu, in)) return;
+            const unsigned d = in ? (unsigned)(k >> next) & ((1u << bits) - 1) : BINS;
+            const unsigned same = __match_any_sync(0xffffffffu, d);
+            if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(&cnt[d], (unsigned)__popc(same));
+        };
+#pragma unroll
+        for (int i = 0; i < KEPT_KEYS; i++) count(own[i], j0 + tid + i * ST);
+        for (int j = j0 + tid + KEPT_KEYS * ST; j - lane < j1; j += ST) count(j < j1 ? keys[j] : 0, j);
+        cluster_sync();
+        // classes from the top: thread t has 2047 - 2t and the one below
+        int c[2] = {0, 0};
+#pragma unroll
+        for (int r = 0; r < MAX_CLUSTER; r++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (r < ncta) c[i] += (int)remote(&cnt[BINS - 1 - 2 * tid - i], r);
+        int x = c[0] + c[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += v;
+        }
+        if (lane == 31) wsum[wid] = x;
+        __syncthreads();
+        int above = x - c[0] - c[1];
+        for (int i = 0; i < wid; i++) above += wsum[i];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            if (above < remaining && remaining <= above + c[i]) {
+                found_bin = BINS - 1 - 2 * tid - i;
+                found_left = remaining - above;
+                found_all = remaining == above + c[i];
+            }
+            above += c[i];
+        }
+        __syncthreads();
+        prefix = (prefix << bits) | (unsigned)found_bin;
+        remaining = found_left;
+        shift = next;
+        if (found_all) break;
+    }
+    // ---- rows above the class stay, and the first `remaining` of it: a warp a run of rows
+    const int run = (span / 32 + ST / 32 - 1) / (ST / 32) * 32, k0 = j0 + wid * run, k1 = min(j1, k0 + run);
+    auto look = [&](int j, unsigned& above, unsigned& tie) {
+        const unsigned long long k = j < k1 ? keys[j] >> shift : 0;
+        above = __ballot_sync(0xffffffffu, j < k1 && k > prefix);
+        tie = __ballot_sync(0xffffffffu, j < k1 && k == prefix);
+    };
+    int na = 0, nt = 0;
+#pragma unroll 4
+    for (int j = k0; j < k1; j += 32) {
+        unsigned above, tie;
+        look(j + lane, above, tie);
+        na += __popc(above);
+        nt += __popc(tie);
+    }
+    if (lane == 0) {
+        wkeep[wid] = na;
+        wtie[wid] = nt;
     }
     __syncthreads();
-    // the need-th largest key, eight bits at a time from the top
-    if (need > 0) {
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            if (tid < 256) hist[tid] = 0;
-            __syncthreads();
-            const unsigned long long pre = prefix;
-            for (int j = lo + tid; j < hi; j += ST) {
-                const unsigned long long k = keys[j];
-                if (shift == 56 || (k >> (shift + 8)) == (pre >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1u);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int r = remaining, bin = 255;
-                while (bin > 0 && (int)hist[bin] < r) r -= (int)hist[bin--];
-                remaining = r;
-                prefix = pre | ((unsigned long long)bin << shift);
-            }
-            __syncthreads();
-        }
+    if (tid < 2) {
+        int s = 0;
+        for (int i = 0; i < ST / 32; i++) s += tid ? wtie[i] : wkeep[i];
+        mine[tid] = s;
     }
-    const unsigned long long thr = need > 0 ? prefix : ~0ull;
-    const int ties = need > 0 ? remaining : 0;
-    if (tid == 0) {
-        base_kept = 0;
-        base_tie = 0;
+    cluster_sync();
+    int ka = 0, kt = 0;                       // above and ties before this warp's run
+    for (int r = 0; r < rank; r++) {
+        ka += (int)remote(&mine[0], r);
+        kt += (int)remote(&mine[1], r);
     }
-    __syncthreads();
-    for (int j0 = 0; j0 < n; j0 += ST) {
-        const int j = j0 + tid;
-        bool keep = j < n && (j < lo || j >= hi), tie = false;
-        if (j >= lo && j < hi) {
-            const unsigned long long k = keys[j];
-            tie = ties > 0 && k == thr;
-            keep = need > 0 && k > thr;
-        }
-        const unsigned mt = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) wtie[wid] = __popc(mt);
-        __syncthreads();
-        int t = base_tie + __popc(mt & ((1u << lane) - 1));
-        for (int i = 0; i < wid; i++) t += wtie[i];
-        keep = keep || (tie && t < ties);
-        const unsigned mk = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) wkept[wid] = __popc(mk);
-        __syncthreads();
-        int at = base_kept + __popc(mk & ((1u << lane) - 1));
-        for (int i = 0; i < wid; i++) at += wkept[i];
-        if (keep && at < a.budget) kept[at] = j;
-        __syncthreads();
-        if (tid == 0) {
-            for (int i = 0; i < ST / 32; i++) {
-                base_kept += wkept[i];
-                base_tie += wtie[i];
-            }
-        }
-        __syncthreads();
+    for (int i = 0; i < wid; i++) {
+        ka += wkeep[i];
+        kt += wtie[i];
     }
+#pragma unroll 4
+    for (int j = k0; j < k1; j += 32) {
+        unsigned above, tie;
+        look(j + lane, above, tie);
+        const unsigned low = (1u << lane) - 1;
+        const int t = kt + __popc(tie & low);
+        const bool keep = ((above >> lane) & 1) || (((tie >> lane) & 1) && t < remaining);
+        if (keep) kept[a.sinks + ka + __popc(above & low) + min(t, remaining)] = j + lane;
+        ka += __popc(above);
+        kt += __popc(tie);
+    }
+    cluster_sync();                           // no CTA leaves while its counts may be read
 }
 
-// a warp a kept row: K, V and their scales into the new page; then the weights
+// A warp CR kept rows at a time, K, V and their scales into the new pages: every load of a
+// round before its first store, so the rows' bytes are in flight together.  Then the weights.
+constexpr int CR = 4;
 __global__ void __launch_bounds__(256) k_evict_copy(const EvictArgs a)
 {
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warps = (int)(gridDim.x * blockDim.x) >> 5;
+    const int gw = (int)(blockIdx.x * blockDim.x + threadIdx.x) >> 5, chunks = a.row_bytes / 16;
     const long long rows = (long long)a.kv.batch * a.budget;
-    const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
-    for (long long i = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5; i < rows; i += warps) {
-        const int b = (int)(i / a.budget), at = (int)(i % a.budget);
-        const int j = a.kept[i];
-        if (j < 0) continue;
-        const int src = a.kv.row(b, j), dst = a.dst.row(b, at);
-        if (src < 0 || dst < 0) continue;
-        const uint4* k0 = reinterpret_cast<const uint4*>(a.kv.Kq + (long long)src * a.row_bytes);
-        const uint4* v0 = reinterpret_cast<const uint4*>(a.kv.Vq + (long long)src * a.row_bytes);
-        uint4* k1 = reinterpret_cast<uint4*>(a.dst.Kq + (long long)dst * a.row_bytes);
-        uint4* v1 = reinterpret_cast<uint4*>(a.dst.Vq + (long long)dst * a.row_bytes);
-        for (int c = lane; c < a.row_bytes / 16; c += 32) {
-            k1[c] = k0[c];
-            v1[c] = v0[c];
+    for (long long i0 = (long long)gw * CR; i0 < rows; i0 += (long long)warps * CR) {
+        // lanes 0 .. CR - 1 look the rows up
+        long long from = -1, to = -1;
+        const long long i = i0 + lane;
+        if (lane < CR && i < rows) {
+            const int b = (int)(i / a.budget), at = (int)(i - (long long)b * a.budget), j = __ldg(a.kept + i);
+            if (j >= 0) {
+                from = a.kv.row(b, j);
+                to = a.dst.row(b, at);
+            }
+        }
+        long long src[CR], dst[CR];
+#pragma unroll
+        for (int r = 0; r < CR; r++) {
+            src[r] = __shfl_sync(0xffffffffu, from, r);
+            dst[r] = __shfl_sync(0xffffffffu, to, r);
+            if (src[r] < 0) dst[r] = -1;
+        }
+        for (int c = lane; c < chunks; c += 32) {
+            uint4 k[CR], v[CR];
+#pragma unroll
+            for (int r = 0; r < CR; r++)
+                if (dst[r] >= 0) {
+                    k[r] = __ldcs(reinterpret_cast<const uint4*>(a.kv.Kq + src[r] * a.row_bytes) + c);
+                    v[r] = __ldcs(reinterpret_cast<const uint4*>(a.kv.Vq + src[r] * a.row_bytes) + c);
+                }
+#pragma unroll
+            for (int r = 0; r < CR; r++)
+                if (dst[r] >= 0) {
+                    reinterpret_cast<uint4*>(a.dst.Kq + dst[r] * a.row_bytes)[c] = k[r];
+                    reinterpret_cast<uint4*>(a.dst.Vq + dst[r] * a.row_bytes)[c] = v[r];
+                }
         }
         for (int c = lane; c < a.row_scales; c += 32) {
-            a.dst.Ks[(long long)dst * a.row_scales + c] = a.kv.Ks[(long long)src * a.row_scales + c];
-            a.dst.Vs[(long long)dst * a.row_scales + c] = a.kv.Vs[(long long)src * a.row_scales + c];
+            float k[CR], v[CR];
+#pragma unroll
+            for (int r = 0; r < CR; r++)
+                if (dst[r] >= 0) {
+                    k[r] = __ldcs(a.kv.Ks + src[r] * a.row_scales + c);
+                    v[r] = __ldcs(a.kv.Vs + src[r] * a.row_scales + c);
+                }
+#pragma unroll
+            for (int r = 0; r < CR; r++)
+                if (dst[r] >= 0) {
+                    a.dst.Ks[dst[r] * a.row_scales + c] = k[r];
+                    a.dst.Vs[dst[r] * a.row_scales + c] = v[r];
+                }
         }
     }
     const int cap = a.kv.cap(), new_cap = a.dst.cap(), nKv = a.kv.nKv;
-    const long long all = (long long)a.kv.batch * nKv * new_cap;
-    for (long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x; i < all; i += (long long)gridDim.x * blockDim.x) {
-        const int at = (int)(i % new_cap);
-        const long long bh = i / new_cap;
-        const int j = at < a.budget ? a.kept[bh / nKv * a.budget + at] : -1;
-        a.new_weights[i] = j >= 0 ? a.weights[bh * cap + j] : 0.0f;
+    // (sequence, head) pairs over the grid's y, rows over x
+    for (int bh = blockIdx.x % (a.kv.batch * nKv); bh < a.kv.batch * nKv; bh += gridDim.x) {
+        const int part = blockIdx.x / (a.kv.batch * nKv), parts = max(1, (int)gridDim.x / (a.kv.batch * nKv));
+        if (part >= parts) break;
+        const int* kept = a.kept + (long long)(bh / nKv) * a.budget;
+        for (int at = part * 256 + threadIdx.x; at < new_cap; at += parts * 256) {
+            const int j = at < a.budget ? __ldg(kept + at) : -1;
+            a.new_weights[(long long)bh * new_cap + at] = j >= 0 ? __ldg(a.weights + (long long)bh * cap + j) : 0.0f;
+        }
     }
 }
 
@@ -210,7 +331,26 @@ TB_API int tb_kv_evict_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, const tb_pag
     a.recent = (int)recent;
     a.row_bytes = (int)(kv->nKv * kv->hd);
     a.row_scales = a.row_bytes / 32;
-    cudaError_t e = tb_launch(ctx, k_evict_select, dim3((unsigned)kv->batch), dim3(ST), 0, a);
+    // budget == sinks + recent: nothing to choose
+    const int64_t cap = kv->max_pages * kv->page_rows;
+    cudaError_t e = cudaSuccess;
+    if (budget > sinks + recent)
+        e = tb_launch(ctx, k_evict_scores, dim3((unsigned)((cap + 255) / 256), (unsigned)kv->batch), dim3(256), 0, a);
+    int cluster = 1;
+    while (cluster < MAX_CLUSTER && cap > (int64_t)cluster * SLOTS) cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(kv->batch * cluster));
+    cfg.blockDim = dim3(ST);
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = ctx->pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, k_evict_select, a);
     if (e == cudaSuccess) e = tb_launch(ctx, k_evict_copy, dim3((unsigned)ctx->num_sms * 8), dim3(256), 0, a);
     if (e != cudaSuccess) return tb_fail(ctx, TB_ERR_CUDA, "kv_evict_paged launch: %s", cudaGetErrorString(e));
     return TB_OK;

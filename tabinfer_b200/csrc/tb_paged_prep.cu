@@ -6,8 +6,11 @@
 //
 // The q / k rows are formed in 64 bits and rounded to f32 once, so a byte of the
 // cache does not depend on how a row's sum was split or in which call it was written
-// (f32 sums put a byte one step off wherever they differ next to a rounding border);
-// 64-bit FMAs run at half the f32 rate here and the kernel stays bound by its bytes.
+// (f32 sums put a byte one step off wherever they differ next to a rounding border).
+// 64-bit arithmetic runs at half the f32 rate, so it is kept short: the norm weight goes
+// into the rotation's coefficients (A = w_lo cos, B = w_hi sin, ...), formed once a row and
+// warp, a head then costs 4 multiply-adds a pair and one multiplication by 1/rms an
+// element, and the sums of eight heads are reduced and inverted together.
 #include "tb_paged.cuh"
 
 namespace {
@@ -27,77 +30,138 @@ __device__ __forceinline__ int8_t snorm8(float x)
 {
     return (int8_t)floorf(__fadd_rn(0.5f, __fmul_rn(127.0f, fminf(1.0f, fmaxf(-1.0f, x)))));
 }
-__device__ __forceinline__ double warp_sum_f64(double v)
+__device__ __forceinline__ double shfl_xor_f64(double v, int m)
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    return __hiloint2double(__shfl_xor_sync(0xffffffffu, __double2hiint(v), m),
+                            __shfl_xor_sync(0xffffffffu, __double2loint(v), m));
 }
 
-// One CTA a row; a warp takes whole heads (q, k, then v), lane l holding elements
-// l + 32 i, so a rotary partner sits in the same lane hd/64 registers away.
-template <int HD>
-__global__ void __launch_bounds__(256) k_paged_prep(const PrepArgs a)
+// x of one head (element l + 32 i in lane l) as snorm bytes with a scale a 32-group
+template <int NW>
+__device__ __forceinline__ void store_q8(const float (&x)[NW], int8_t* dq, float* ds, int lane)
 {
-    __shared__ double cs[HD / 2], sn[HD / 2];
+    float m[NW];
+#pragma unroll
+    for (int i = 0; i < NW; i++) m[i] = fmaxf(1e-12f, warp_max(fabsf(x[i])));
+#pragma unroll
+    for (int i = 0; i < NW; i++) dq[32 * i + lane] = snorm8(__fdiv_rn(x[i], m[i]));
+    if (lane == 0) {
+        if constexpr (NW == 4) *reinterpret_cast<float4*>(ds) = make_float4(m[0], m[1], m[2], m[3]);
+        else *reinterpret_cast<float2*>(ds) = make_float2(m[0], m[1]);
+    }
+}
+
+// R rows a CTA (8 warps): the angles of all of them first (one a thread at R = 4, hd 128), then
+// 8 / R warps a row, each with every (8 / R)-th head, NB heads at a time: their loads are in
+// flight together.  Lane l holds elements l + 32 i, a rotary partner hd / 64 registers away.
+// One row a CTA where there are fewer rows than four a SM would take (latency).
+constexpr int NB = 8;
+template <int HD, int R>
+__global__ void __launch_bounds__(256) k_paged_prep(const PrepArgs a, int T)
+{
+    constexpr int HALF = HD / 2, NW = HD / 32, NP = NW / 2, WPR = 8 / R;
+    __shared__ double cs[R][HALF], sn[R][HALF];
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int t = blockIdx.x, lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    constexpr int half = HD / 2, nw = HD / 32;
-    const int b = a.seq[t], slot = a.slot[t];
-    if (b < 0) return;                       // a padding row
-    if (b >= a.kv.batch || slot < 0 || slot >= a.kv.cap()) {
-        if (threadIdx.x == 0) atomicExch(a.kv.err, ERR_PAGED_LEN);
-        return;
+    const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, t0 = blockIdx.x * R;
+    for (int i = threadIdx.x; i < R * HALF; i += 256) {
+        const int r = i / HALF, f = i % HALF;
+        if (t0 + r < T) {
+            const double ang = (double)a.pos[t0 + r] * pow(a.theta, -2.0 * (double)f / (double)HD);
+            sincos(ang, &sn[r][f], &cs[r][f]);
+        }
     }
-    const int row = a.kv.row(b, slot);
-    if (row < 0) return;
-    for (int f = threadIdx.x; f < half; f += blockDim.x) {
-        const double ang = (double)a.pos[t] * pow(a.theta, -2.0 * (double)f / (double)HD);
-        sincos(ang, &sn[f], &cs[f]);
+    const int rr = wid / WPR, t = t0 + rr, part = wid % WPR;
+    int row = -1;
+    if (t < T) {
+        const int b = a.seq[t], slot = a.slot[t];
+        if (b >= a.kv.batch || (b >= 0 && (slot < 0 || slot >= a.kv.cap()))) {
+            if (lane == 0) atomicExch(a.kv.err, ERR_PAGED_LEN);
+        } else if (b >= 0) {                 // else a padding row
+            row = a.kv.row(b, slot);
+        }
     }
     __syncthreads();
+    if (row < 0) return;
     const int nHq = a.nHq, nKv = a.kv.nKv;
-    for (int role = wid; role < nHq + 2 * nKv; role += 8) {
-        const bool isQ = role < nHq, isK = !isQ && role < nHq + nKv;
-        const int head = isQ ? role : (isK ? role - nHq : role - nHq - nKv);
-        const float* src = (isQ ? a.q + (long long)t * nHq * HD : (isK ? a.k : a.v) + (long long)t * nKv * HD) + head * HD;
-        float x[nw];
+#pragma unroll 1
+    for (int type = 0; type < 2; type++) {   // q, then k
+        const int heads = type ? nKv : nHq;
+        const float* src = (type ? a.k : a.q) + (long long)t * heads * HD;
+        const uint16_t* w16 = type ? a.kw : a.qw;
+        double A[NP], B[NP], C[NP], D[NP];
 #pragma unroll
-        for (int i = 0; i < nw; i++) x[i] = src[32 * i + lane];
-        if (isQ || isK) {
-            const uint16_t* w16 = isQ ? a.qw : a.kw;
-            double y[nw], ss = 0.0;
+        for (int i = 0; i < NP; i++) {
+            const double c = cs[rr][32 * i + lane], s = sn[rr][32 * i + lane];
+            const double wl = (double)tb_h2f(w16[32 * i + lane]), wh = (double)tb_h2f(w16[HALF + 32 * i + lane]);
+            A[i] = wl * c;
+            B[i] = wh * s;
+            C[i] = wh * c;
+            D[i] = wl * s;
+        }
+#pragma unroll 1
+        for (int h0 = part; h0 < heads; h0 += NB * WPR) {
+            float x[NB][NW];
 #pragma unroll
-            for (int i = 0; i < nw; i++) {
-                y[i] = (double)x[i];
-                ss = fma(y[i], y[i], ss);
+            for (int k = 0; k < NB; k++)
+#pragma unroll
+                for (int i = 0; i < NW; i++) {
+                    const int h = h0 + k * WPR;
+                    x[k][i] = h < heads ? __ldcs(src + h * HD + 32 * i + lane) : 0.0f;
+                }
+            double ss[NB];
+#pragma unroll
+            for (int k = 0; k < NB; k++) {
+                ss[k] = 0.0;
+#pragma unroll
+                for (int i = 0; i < NW; i++) {
+                    const double v = (double)x[k][i];
+                    ss[k] = fma(v, v, ss[k]);
+                }
             }
-            const double inv = 1.0 / sqrt(warp_sum_f64(ss) / (double)HD + a.eps);
+            // sums over the lanes: halves exchange halves of the heads, so a lane ends with the head of its
+            // bits 4, 3, 2
 #pragma unroll
-            for (int i = 0; i < nw; i++) y[i] = y[i] * inv * (double)tb_h2f(w16[32 * i + lane]);
+            for (int w = NB / 2, m = 16; w >= 1; w >>= 1, m >>= 1)
 #pragma unroll
-            for (int i = 0; i < nw / 2; i++) {
-                const double c = cs[32 * i + lane], s = sn[32 * i + lane], lo = y[i], hi = y[i + nw / 2];
-                x[i] = (float)(lo * c - hi * s);
-                x[i + nw / 2] = (float)(hi * c + lo * s);
-            }
-            if (isQ) {
-                float* dst = a.qr + (long long)t * nHq * HD + head * HD;
+                for (int k = 0; k < w; k++) {
+                    const bool up = lane & m;
+                    const double mine = up ? ss[k + w] : ss[k], other = up ? ss[k] : ss[k + w];
+                    ss[k] = mine + shfl_xor_f64(other, m);
+                }
+            ss[0] += shfl_xor_f64(ss[0], 2);
+            ss[0] += shfl_xor_f64(ss[0], 1);
+            const double inv = 1.0 / sqrt(ss[0] * (1.0 / HD) + a.eps);
 #pragma unroll
-                for (int i = 0; i < nw; i++) dst[32 * i + lane] = x[i];
-                continue;
+            for (int k = 0; k < NB; k++) {
+                const int from = (k & 4 ? 16 : 0) | (k & 2 ? 8 : 0) | (k & 1 ? 4 : 0), h = h0 + k * WPR;
+                const double n = __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(inv), from),
+                                                  __shfl_sync(0xffffffffu, __double2loint(inv), from));
+                if (h >= heads) break;
+#pragma unroll
+                for (int i = 0; i < NP; i++) {
+                    const double lo = (double)x[k][i], hi = (double)x[k][i + NP];
+                    x[k][i] = (float)(n * fma(lo, A[i], -(hi * B[i])));
+                    x[k][i + NP] = (float)(n * fma(hi, C[i], lo * D[i]));
+                }
+                if (type == 0) {
+                    float* dst = a.qr + ((long long)t * nHq + h) * HD;
+#pragma unroll
+                    for (int i = 0; i < NW; i++) dst[32 * i + lane] = x[k][i];
+                } else {
+                    const long long at = ((long long)row * nKv + h) * HD;
+                    store_q8<NW>(x[k], a.kv.Kq + at, a.kv.Ks + at / 32, lane);
+                }
             }
         }
-        const long long at = (long long)row * nKv * HD + head * HD;
-        int8_t* dq = (isK ? a.kv.Kq : a.kv.Vq) + at;
-        float* ds = (isK ? a.kv.Ks : a.kv.Vs) + at / 32;
+    }
+#pragma unroll 2
+    for (int h = part; h < nKv; h += WPR) {
+        float x[NW];
 #pragma unroll
-        for (int i = 0; i < nw; i++) {
-            const float m = fmaxf(1e-12f, warp_max(fabsf(x[i])));
-            dq[32 * i + lane] = snorm8(__fdiv_rn(x[i], m));
-            if (lane == 0) ds[i] = m;
-        }
+        for (int i = 0; i < NW; i++) x[i] = __ldcs(a.v + ((long long)t * nKv + h) * HD + 32 * i + lane);
+        const long long at = ((long long)row * nKv + h) * HD;
+        store_q8<NW>(x, a.kv.Vq + at, a.kv.Vs + at / 32, lane);
     }
 }
 
@@ -118,8 +182,10 @@ extern "C" TB_API int tb_attn_prep_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, 
     TB_REQUIRE(ctx, q && k && v && qw16 && kw16 && qr && seq && slot && pos, "null pointer");
     DeviceGuard dev(ctx->device);
     PrepArgs a{paged_args(ctx, kv), q, k, v, qw16, kw16, qr, seq, slot, pos, (int)nHq, (double)theta, (double)eps};
-    auto kern = kv->hd == 64 ? k_paged_prep<64> : k_paged_prep<128>;
-    cudaError_t e = tb_launch(ctx, kern, dim3((unsigned)T), dim3(256), 0, a);
+    const bool many = T >= 4LL * ctx->num_sms;
+    auto kern = kv->hd == 64 ? (many ? k_paged_prep<64, 4> : k_paged_prep<64, 1>)
+                             : (many ? k_paged_prep<128, 4> : k_paged_prep<128, 1>);
+    cudaError_t e = tb_launch(ctx, kern, dim3((unsigned)(many ? (T + 3) / 4 : T)), dim3(256), 0, a, (int)T);
     if (e != cudaSuccess) return tb_fail(ctx, TB_ERR_CUDA, "attn_prep_paged launch: %s", cudaGetErrorString(e));
     return TB_OK;
 }
