@@ -70,6 +70,14 @@ __device__ __forceinline__ bool key_seen(int key, int pos, int window, int sinks
     return key <= pos && (window <= 0 || pos - key < window || key < sinks);
 }
 
+// the warp's largest value (NaN left out, as fmaxf does)
+__device__ __forceinline__ float redux_max(float v)
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 // ---- mbarriers and asynchronous copies -------------------------------------------
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint64_t* b, unsigned count)

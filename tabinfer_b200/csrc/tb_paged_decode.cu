@@ -187,12 +187,6 @@ struct Walk {
     }
 };
 
-__device__ __forceinline__ float redux_max(float v)
-{
-    float r;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-    return r;
-}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, make_float2(0.0f, 0.0f)); }
 
 // What bounds it is HBM, so the arithmetic on each byte has to be short.  Both products run

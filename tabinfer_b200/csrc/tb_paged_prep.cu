@@ -10,7 +10,7 @@
 // 64-bit arithmetic runs at half the f32 rate, so it is kept short: the norm weight goes
 // into the rotation's coefficients (A = w_lo cos, B = w_hi sin, ...), formed once a row and
 // warp, a head then costs 4 multiply-adds a pair and one multiplication by 1/rms an
-// element, and the sums of eight heads are reduced and inverted together.
+// element, and the sums of four heads are reduced and inverted together.
 #include "tb_paged.cuh"
 
 namespace {
@@ -25,10 +25,15 @@ struct PrepArgs {
     double theta, eps;
 };
 
-// floor(0.5 + 127 x) of x clamped to [-1, 1] (pack4x8snorm)
-__device__ __forceinline__ int8_t snorm8(float x)
+// floor(0.5 + 127 x / m), |x| <= m (pack4x8snorm of the rounded quotient).  The quotient by
+// a reciprocal is off by less than 2^-21 of itself, so 127 times it by less than 7e-5: the
+// division itself is needed only next to a border.
+__device__ __forceinline__ int8_t snorm8(float x, float m, float inv)
 {
-    return (int8_t)floorf(__fadd_rn(0.5f, __fmul_rn(127.0f, fminf(1.0f, fmaxf(-1.0f, x)))));
+    float v = __fadd_rn(0.5f, __fmul_rn(127.0f, x * inv));
+    if (fabsf(v - rintf(v)) < 1e-4f || !(fabsf(v) < 200.0f) || m > 1e30f)
+        v = __fadd_rn(0.5f, __fmul_rn(127.0f, fminf(1.0f, fmaxf(-1.0f, __fdiv_rn(x, m)))));
+    return (int8_t)__float2int_rd(v);
 }
 __device__ __forceinline__ double shfl_xor_f64(double v, int m)
 {
@@ -42,9 +47,9 @@ __device__ __forceinline__ void store_q8(const float (&x)[NW], int8_t* dq, float
 {
     float m[NW];
 #pragma unroll
-    for (int i = 0; i < NW; i++) m[i] = fmaxf(1e-12f, warp_max(fabsf(x[i])));
+    for (int i = 0; i < NW; i++) m[i] = fmaxf(1e-12f, redux_max(fabsf(x[i])));
 #pragma unroll
-    for (int i = 0; i < NW; i++) dq[32 * i + lane] = snorm8(__fdiv_rn(x[i], m[i]));
+    for (int i = 0; i < NW; i++) dq[32 * i + lane] = snorm8(x[i], m[i], __fdividef(1.0f, m[i]));
     if (lane == 0) {
         if constexpr (NW == 4) *reinterpret_cast<float4*>(ds) = make_float4(m[0], m[1], m[2], m[3]);
         else *reinterpret_cast<float2*>(ds) = make_float2(m[0], m[1]);
@@ -55,21 +60,25 @@ __device__ __forceinline__ void store_q8(const float (&x)[NW], int8_t* dq, float
 // 8 / R warps a row, each with every (8 / R)-th head, NB heads at a time: their loads are in
 // flight together.  Lane l holds elements l + 32 i, a rotary partner hd / 64 registers away.
 // One row a CTA where there are fewer rows than four a SM would take (latency).
-constexpr int NB = 8;
+constexpr int NB = 4;
 template <int HD, int R>
-__global__ void __launch_bounds__(256) k_paged_prep(const PrepArgs a, int T)
+__global__ void __launch_bounds__(256, 4) k_paged_prep(const PrepArgs a, int T)
 {
     constexpr int HALF = HD / 2, NW = HD / 32, NP = NW / 2, WPR = 8 / R;
     __shared__ double cs[R][HALF], sn[R][HALF];
     tb_pdl_wait();
     tb_pdl_trigger();
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, t0 = blockIdx.x * R;
-    for (int i = threadIdx.x; i < R * HALF; i += 256) {
-        const int r = i / HALF, f = i % HALF;
-        if (t0 + r < T) {
-            const double ang = (double)a.pos[t0 + r] * pow(a.theta, -2.0 * (double)f / (double)HD);
-            sincos(ang, &sn[r][f], &cs[r][f]);
-        }
+    if (R > 1) {                             // the powers once a CTA
+        if (threadIdx.x < HALF) cs[0][threadIdx.x] = pow(a.theta, -2.0 * (double)threadIdx.x / (double)HD);
+        __syncthreads();
+    }
+    {
+        static_assert(R * HALF <= 256, "an angle a thread");
+        const int r = threadIdx.x / HALF, f = threadIdx.x % HALF;
+        const double p = R > 1 ? cs[0][f] : threadIdx.x < HALF ? pow(a.theta, -2.0 * (double)f / (double)HD) : 0.0;
+        if (R > 1) __syncthreads();
+        if (r < R && t0 + r < T) sincos((double)a.pos[t0 + r] * p, &sn[r][f], &cs[r][f]);
     }
     const int rr = wid / WPR, t = t0 + rr, part = wid % WPR;
     int row = -1;
@@ -120,7 +129,7 @@ __global__ void __launch_bounds__(256) k_paged_prep(const PrepArgs a, int T)
                 }
             }
             // sums over the lanes: halves exchange halves of the heads, so a lane ends with the head of its
-            // bits 4, 3, 2
+            // bits 4 and 3
 #pragma unroll
             for (int w = NB / 2, m = 16; w >= 1; w >>= 1, m >>= 1)
 #pragma unroll
@@ -129,12 +138,13 @@ __global__ void __launch_bounds__(256) k_paged_prep(const PrepArgs a, int T)
                     const double mine = up ? ss[k + w] : ss[k], other = up ? ss[k] : ss[k + w];
                     ss[k] = mine + shfl_xor_f64(other, m);
                 }
+            ss[0] += shfl_xor_f64(ss[0], 4);
             ss[0] += shfl_xor_f64(ss[0], 2);
             ss[0] += shfl_xor_f64(ss[0], 1);
             const double inv = 1.0 / sqrt(ss[0] * (1.0 / HD) + a.eps);
 #pragma unroll
             for (int k = 0; k < NB; k++) {
-                const int from = (k & 4 ? 16 : 0) | (k & 2 ? 8 : 0) | (k & 1 ? 4 : 0), h = h0 + k * WPR;
+                const int from = (k & 2 ? 16 : 0) | (k & 1 ? 8 : 0), h = h0 + k * WPR;
                 const double n = __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(inv), from),
                                                   __shfl_sync(0xffffffffu, __double2loint(inv), from));
                 if (h >= heads) break;

@@ -7,11 +7,12 @@ stream of the tensor's device.  Shape/alignment errors raise TabInferError
 with the library's message (the reference throws / panics).
 """
 import ctypes
+import struct
 import threading
 
 import torch
 
-from ._lib import LIB, P, PagedKV
+from ._lib import LIB, P
 
 TB_ACT_F32, TB_ACT_Q8 = 0, 1
 CUDA_STREAM_LEGACY = 0x1   # cudaStreamLegacy
@@ -634,56 +635,79 @@ def attention_decode_q8(qr, kv, S, nHq, nKv, hd, nsplit=0, out=None):
 # page table[b, r // page_rows].
 # --------------------------------------------------------------------------
 
-def _arg(t, what, dtype, shape, device):
-    """A dense device tensor of this type and shape (None: any extent) on `device` -> its address."""
-    if t.dtype != dtype or t.dim() != len(shape) or t.device != device or not t.is_contiguous():
-        raise TabInferError("%s must be a contiguous %s tensor of %d dimensions on %s" % (what, dtype, len(shape), device))
-    for have, want in zip(t.shape, shape):
-        if want is not None and have != want:
-            raise TabInferError("%s: shape %s does not fit %s" % (what, tuple(t.shape), tuple(shape)))
-    return t.data_ptr()
+def _arg(t, what, dtype, shape, index):
+    """A dense tensor of this type and shape on CUDA device `index` -> its address."""
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
+    raise TabInferError("%s must be a contiguous %s tensor of shape %s on cuda:%d (got %s %s on %s)"
+                        % (what, dtype, tuple(shape), index, t.dtype, tuple(t.shape), t.device))
 
 
-def _paged(kv, table, nKv, hd, device, what="kv"):
-    """The cache's tb_paged_kv, its tensors checked."""
-    if device.type != "cuda":
+_PAGED_KV = struct.Struct("@5P6q").pack     # tb_paged_kv (packed: half the time of a ctypes structure)
+
+
+def _paged(kv, table, nKv, hd, index, what="kv"):
+    """The cache's tb_paged_kv as bytes, its tensors checked, and (page_rows, batch, max_pages)."""
+    if index < 0:
         raise TabInferError("tensor must be on a CUDA device")
     Kq, Ks, Vq, Vs = kv
-    if Kq.dim() != 3:
-        raise TabInferError("%s: pools are [n_pages, page_rows, nKv*hd]" % what)
+    if Kq.dim() != 3 or table.dim() != 2:
+        raise TabInferError("%s: pools are [n_pages, page_rows, nKv*hd], the table [batch, max_pages]" % what)
     n, r, _ = Kq.shape
-    w = nKv * hd
-    kq = _arg(Kq, what + " Kq", torch.int8, (n, r, w), device)
-    ks = _arg(Ks, what + " Ks", torch.float32, (n, r, w // 32), device)
-    vq = _arg(Vq, what + " Vq", torch.int8, (n, r, w), device)
-    vs = _arg(Vs, what + " Vs", torch.float32, (n, r, w // 32), device)
-    tab = _arg(table, "table", torch.int32, (None, None), device)
-    return PagedKV(kq, ks, vq, vs, tab, n, r, table.shape[0], table.shape[1], nKv, hd)
+    B, most = table.shape
+    q, m = (n, r, nKv * hd), (n, r, nKv * hd // 32)
+    i8, f32 = torch.int8, torch.float32
+    return _PAGED_KV(_arg(Kq, what, i8, q, index), _arg(Ks, what, f32, m, index), _arg(Vq, what, i8, q, index),
+                     _arg(Vs, what, f32, m, index), _arg(table, "table", torch.int32, (B, most), index), n, r, B, most,
+                     nKv, hd), r, B, most
 
 
-def _workspace(c, what, query, device, *sizes):
+_ws_sizes = {}
+
+
+def _workspace(c, query, index, s, *sizes):
     """Workspace of a paged call: a tensor of the current stream's allocator, so calls on other
-    streams and captured graphs have their own."""
-    n = ctypes.c_size_t(0)
-    c.check(query(c.h, *sizes, ctypes.byref(n)), what)
-    return torch.empty(max(n.value, 256), dtype=torch.uint8, device=device), n.value
+    streams and captured graphs have their own.  sizes: what the query takes behind the cache."""
+    key = (query, index, s[40:], sizes)         # the cache's sizes without its addresses
+    n = _ws_sizes.get(key)
+    if n is None:
+        v = ctypes.c_size_t()
+        c.check(getattr(LIB, query)(c.h, s, *sizes, ctypes.byref(v)), query)
+        n = _ws_sizes[key] = max(v.value, 256)
+    return torch.empty(n, dtype=torch.uint8, device=_device(index)), n
+
+
+_devices = {}
+
+
+def _device(index):
+    d = _devices.get(index)
+    if d is None:
+        d = _devices[index] = torch.device("cuda", index)
+    return d
 
 
 def attn_prep_paged_q8(q, k, v, qw16, kw16, kv, table, seq, slot, pos, nHq, nKv, hd, theta, eps, qr=None):
     """attnPrepQ8 (qwen3.js:2297-2308) for T rows of any sequences: row t of q [T, nHq*hd] and
     k, v [T, nKv*hd] -> cache row slot[t] of sequence seq[t] at rotary position pos[t] (int32 [T];
     seq < 0: a padding row, nothing is written).  Returns qr f32 [T, nHq*hd]."""
-    d, T = q.device, q.shape[0]
-    s = _paged(kv, table, nKv, hd, d)
+    d, T, f32, i32 = q.get_device(), q.shape[0], torch.float32, torch.int32
+    s, _, _, _ = _paged(kv, table, nKv, hd, d)
+    wide, row, w16 = (T, nHq * hd), (T, nKv * hd), (hd,)
+    qp, kp, vp = _arg(q, "q", f32, wide, d), _arg(k, "k", f32, row, d), _arg(v, "v", f32, row, d)
     if qr is None:
-        qr = torch.empty((T, nHq * hd), dtype=torch.float32, device=d)
-    qp, op = _arg(q, "q", torch.float32, (T, nHq * hd), d), _arg(qr, "qr", torch.float32, (T, nHq * hd), d)
-    kp, vp = _arg(k, "k", torch.float32, (T, nKv * hd), d), _arg(v, "v", torch.float32, (T, nKv * hd), d)
-    i = [_arg(t, what, torch.int32, (T,), d) for t, what in ((seq, "seq"), (slot, "slot"), (pos, "pos"))]
-    w = [_arg(t.view(torch.int16), what, torch.int16, (hd,), d) for t, what in ((qw16, "qw16"), (kw16, "kw16"))]
-    c = _ctx(q)
-    c.check(LIB.tb_attn_prep_paged_q8(c.h, ctypes.byref(s), qp, kp, vp, w[0], w[1], op, nHq, T, *i, float(theta),
-                                      float(eps)), "attn_prep_paged_q8")
+        qr = torch.empty_like(q)
+        op = qr.data_ptr()
+    else:
+        op = _arg(qr, "qr", f32, wide, d)
+    if qw16.dtype.itemsize != 2 or kw16.dtype.itemsize != 2:
+        raise TabInferError("the norm weights are f16 (16-bit patterns)")
+    rc = LIB.tb_attn_prep_paged_q8(
+        default_context(d).h, s, qp, kp, vp, _arg(qw16, "qw16", qw16.dtype, w16, d),
+        _arg(kw16, "kw16", kw16.dtype, w16, d), op, nHq, T, _arg(seq, "seq", i32, (T,), d),
+        _arg(slot, "slot", i32, (T,), d), _arg(pos, "pos", i32, (T,), d), theta, eps)
+    if rc:
+        default_context(d).check(rc, "attn_prep_paged_q8")
     return qr
 
 
@@ -693,18 +717,22 @@ def attention_decode_paged_q8(qr, kv, table, lens, nHq, nKv, hd, window=0, sinks
     `window` rows and the first `sinks`.  weights f32 [batch, nKv, max_pages*page_rows]: each
     row's attention weight, summed over the kv head's q heads, is added to it.  Returns f32
     [batch, nHq*hd]."""
-    d, B = qr.device, table.shape[0]
-    s = _paged(kv, table, nKv, hd, d)
+    d, f32 = qr.get_device(), torch.float32
+    s, rows, B, most = _paged(kv, table, nKv, hd, d)
+    wide = (B, nHq * hd)
+    qp = _arg(qr, "qr", f32, wide, d)
     if out is None:
-        out = torch.empty((B, nHq * hd), dtype=torch.float32, device=d)
-    qp, op = _arg(qr, "qr", torch.float32, (B, nHq * hd), d), _arg(out, "out", torch.float32, (B, nHq * hd), d)
+        out = torch.empty_like(qr)
+        op = out.data_ptr()
+    else:
+        op = _arg(out, "out", f32, wide, d)
     lp = _arg(lens, "lens", torch.int32, (B,), d)
-    wp = None if weights is None else _arg(weights, "weights", torch.float32, (B, nKv, s.max_pages * s.page_rows), d)
-    c = _ctx(qr)
-    ws, n = _workspace(c, "attn_decode_paged_ws", LIB.tb_attn_decode_paged_ws, d, ctypes.byref(s), nHq,
-                       0 if weights is None else 1)
-    c.check(LIB.tb_attn_decode_paged_q8(c.h, ctypes.byref(s), op, qp, lp, nHq, int(window), int(sinks), wp,
-                                        ws.data_ptr(), n), "attn_decode_paged_q8")
+    wp = None if weights is None else _arg(weights, "weights", f32, (B, nKv, most * rows), d)
+    c = default_context(d)
+    ws, n = _workspace(c, "tb_attn_decode_paged_ws", d, s, nHq, 0 if wp is None else 1)
+    rc = LIB.tb_attn_decode_paged_q8(c.h, s, op, qp, lp, nHq, int(window), int(sinks), wp, ws.data_ptr(), n)
+    if rc:
+        c.check(rc, "attn_decode_paged_q8")
     return out
 
 
@@ -713,16 +741,21 @@ def attention_prefill_paged_q8(q, kv, table, cu, lens, nHq, nKv, hd, window=0, s
     q [T, nHq*hd] are the last rows of sequence b, which holds lens[b] rows; window and sinks as
     in attention_decode_paged_q8.  Returns bf16 [T, nHq*hd] (gemm_q's X); rows outside
     cu[0] .. cu[batch] are left as they were."""
-    d, B, T = q.device, table.shape[0], q.shape[0]
-    s = _paged(kv, table, nKv, hd, d)
+    d, T, i32 = q.get_device(), q.shape[0], torch.int32
+    s, _, B, _ = _paged(kv, table, nKv, hd, d)
+    wide = (T, nHq * hd)
+    qp = _arg(q, "q", torch.float32, wide, d)
     if out is None:
-        out = torch.empty((T, nHq * hd), dtype=torch.bfloat16, device=d)
-    qp, op = _arg(q, "q", torch.float32, (T, nHq * hd), d), _arg(out, "out", torch.bfloat16, (T, nHq * hd), d)
-    cp, lp = _arg(cu, "cu", torch.int32, (B + 1,), d), _arg(lens, "lens", torch.int32, (B,), d)
-    c = _ctx(q)
-    ws, n = _workspace(c, "attn_prefill_paged_ws", LIB.tb_attn_prefill_paged_ws, d, ctypes.byref(s), nHq, T)
-    c.check(LIB.tb_attn_prefill_paged_q8(c.h, ctypes.byref(s), op, qp, cp, lp, nHq, T, int(window), int(sinks),
-                                         ws.data_ptr(), n), "attn_prefill_paged_q8")
+        out = torch.empty_like(q, dtype=torch.bfloat16)
+        op = out.data_ptr()
+    else:
+        op = _arg(out, "out", torch.bfloat16, wide, d)
+    cp, lp = _arg(cu, "cu", i32, (B + 1,), d), _arg(lens, "lens", i32, (B,), d)
+    c = default_context(d)
+    ws, n = _workspace(c, "tb_attn_prefill_paged_ws", d, s, nHq, T)
+    rc = LIB.tb_attn_prefill_paged_q8(c.h, s, op, qp, cp, lp, nHq, T, int(window), int(sinks), ws.data_ptr(), n)
+    if rc:
+        c.check(rc, "attn_prefill_paged_q8")
     return out
 
 
@@ -733,21 +766,22 @@ def kv_evict_paged_q8(kv, table, lens, weights, new_table, budget, sinks, recent
     The rows are copied in order into new_table's pages (of kv, or of the pools kv_out; none of
     them a page that is read).  Returns (kept int32 [batch, budget], the old row of each new one, -1
     behind the last; lens int32 [batch]; weights f32 [batch, nKv, new rows], zero behind the last)."""
-    d, B = table.device, table.shape[0]
-    s = _paged(kv, table, nKv, hd, d)
-    t = _paged(kv if kv_out is None else kv_out, new_table, nKv, hd, d, "kv_out")
+    d = table.get_device()
+    s, rows, B, most = _paged(kv, table, nKv, hd, d)
+    t, new_rows, new_B, new_most = _paged(kv if kv_out is None else kv_out, new_table, nKv, hd, d, "kv_out")
+    dev = _device(d)
     lp = _arg(lens, "lens", torch.int32, (B,), d)
-    wp = _arg(weights, "weights", torch.float32, (B, nKv, s.max_pages * s.page_rows), d)
-    if t.batch != B:
+    wp = _arg(weights, "weights", torch.float32, (B, nKv, most * rows), d)
+    if new_B != B:
         raise TabInferError("new_table must have %d rows" % B)
     if budget < 0:
         raise TabInferError("budget must not be negative")
-    kept = torch.empty((B, int(budget)), dtype=torch.int32, device=d)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=d)
-    new_weights = torch.empty((B, nKv, t.max_pages * t.page_rows), dtype=torch.float32, device=d)
-    c = _ctx(table)
-    ws, n = _workspace(c, "kv_evict_paged_ws", LIB.tb_kv_evict_paged_ws, d, ctypes.byref(s))
-    c.check(LIB.tb_kv_evict_paged_q8(c.h, ctypes.byref(s), ctypes.byref(t), lp, wp, kept.data_ptr(),
+    kept = torch.empty((B, int(budget)), dtype=torch.int32, device=dev)
+    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    new_weights = torch.empty((B, nKv, new_most * new_rows), dtype=torch.float32, device=dev)
+    c = default_context(d)
+    ws, n = _workspace(c, "tb_kv_evict_paged_ws", d, s)
+    c.check(LIB.tb_kv_evict_paged_q8(c.h, s, t, lp, wp, kept.data_ptr(),
                                      new_lens.data_ptr(), new_weights.data_ptr(), int(budget), int(sinks),
                                      int(recent), ws.data_ptr(), n), "kv_evict_paged_q8")
     return kept, new_lens, new_weights
