@@ -92,6 +92,15 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* b)
 {
     asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}" ::"r"(smem_u32(b)) : "memory");
 }
+// whether the phase of this parity has completed (no suspension: half the time of a try_wait
+// whose phase has)
+__device__ __forceinline__ bool mbar_test(uint64_t* b, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(done) : "r"(smem_u32(b)), "r"(parity) : "memory");
+    return done != 0;
+}
 // Waits until the phase of this parity has completed; at most WAIT_TRIES tries of up to
 // 1 ms each, after which (or when *abort is up) it returns false.
 constexpr int WAIT_TRIES = 1000;

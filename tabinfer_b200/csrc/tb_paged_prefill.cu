@@ -15,7 +15,7 @@
 // Warp roles of k_paged_prefill:
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread a row: S from TMEM, P (f16) back
 //                    over it; the reference maximum is raised (and O rescaled in TMEM) only
-//                    when a score passes it by 2^8, so O is hardly ever touched; Q of the
+//                    when a score passes it by 2^9, so O is hardly ever touched; Q of the
 //                    next part into shared memory, then the part's outputs
 //   warps 8-11       K / V tiles: 16-byte copies ahead into thread-private shared memory, bytes
 //                    -> f16 (one exact step, one multiplication by the group's scale) into
@@ -41,7 +41,7 @@ constexpr int NC = 4;                      // 16-byte chunks a producer thread t
 constexpr int KV_STAGES = 2;
 constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps their sums in shared memory)
 constexpr int MIN_TILES = 2;             // an item is not cut below this many tiles a part
-constexpr float RAISE = 8.0f;            // log2 by which a score may pass the reference maximum
+constexpr float TOO_LARGE = 32768.0f;    // sum of a half's exponentials that raises the reference maximum
 
 struct Part {
     int b, row0, nq, p0;                 // sequence, first packed row, queries, row of the first in the sequence
@@ -332,8 +332,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     uint64_t* k_empty = k_full + KV_STAGES;
     uint64_t* v_full = k_empty + KV_STAGES;
     uint64_t* v_empty = v_full + KV_STAGES;
-    uint64_t* s_full = v_empty + KV_STAGES;                                 // [2] S written
-    uint64_t* p_full = s_full + 2;                                          // [2][2] a half of P written, O rescaled
+    uint64_t* s_full = v_empty + KV_STAGES;                                 // [2][2] a half of S written
+    uint64_t* p_full = s_full + 4;                                          // [2][2] a half of P written, O rescaled
     uint64_t* o_done = p_full + 4;                                          // [2][2] O += P V of a half completed
     uint64_t* done = o_done + 4;                                            // every MMA completed
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(done + 1);
@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&q_full[i], 4);
-            mbar_init(&s_full[i], 1);
+            mbar_init(&s_full[2 * i], 1);
+            mbar_init(&s_full[2 * i + 1], 1);
             mbar_init(&p_full[2 * i], 4);
             mbar_init(&p_full[2 * i + 1], 4);
             mbar_init(&o_done[2 * i], 1);
@@ -377,6 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     };
     // one outcome for the warp: its lanes then run the .aligned instructions together
     auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+        if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
         const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
         if (!ok && lane == 0) give_up();
         __syncwarp();
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             if (lane == 0) mbar_arrive(&q_full[t]);
         };
         // the CTA's next part that has rows in this tile
-        const uint4* bad = reinterpret_cast<const uint4*>(smem + L::OFF_BAD);
+        const uint2* bad = reinterpret_cast<const uint2*>(smem + L::OFF_BAD);
         int tile = 0;                                            // tiles of the CTA so far (the masks' ring)
         auto find = [&](int k, Part& p, int& h) {
             for (;; k++) {
@@ -435,35 +437,39 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int j = p.t0; j < p.t1; j++, seq++, tile++) {
-                if (!(ok = wait_warp(&s_full[t], seq & 1))) break;
-                tc_after();
                 const int k0 = seen.tile(j) * PK;
-                const uint4 bw = bad[tile & 7];
-                // a tile that some row sees only in part, or with keys on bad pages
-                const bool cut = k0 + PK - 1 > pmin || (a.window > 0 && k0 <= pmax - a.window && k0 + PK > a.sinks) ||
-                                 (bw.x | bw.y | bw.z | bw.w);
                 const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
-                // In two halves of 64 keys, so that the first half's product runs under the second's softmax.
-                // One pass over a half's scores against the reference maximum as it stands; a score that
-                // passes it by 2^RAISE raises it, rescales O (every column, once the last product is in) and
-                // repeats the pass.  The first half's maximum comes first.
+                // In two halves of 64 keys: a half's P V and the next tile's Q K^T over its place run under the
+                // other half's softmax, so scores are there when a thread comes for them.
+                // One pass over a half's scores against the reference maximum as it stands: no maximum is
+                // formed.  Where the sum tells that a score has passed it by 2^9 or more, the maximum is
+                // taken, O rescaled (every column, once the last product is in) and the pass repeated.  A
+                // row's first reference is the maximum of the first half in which it sees a key.
 #pragma unroll 1
                 for (int hh = 0; hh < 2; hh++) {
                     const bool fresh = j == p.t0 && hh == 0;
                     const uint32_t th = ts + 64 * hh;
+                    if (!(ok = wait_warp(&s_full[2 * t + hh], seq & 1))) break;
+                    tc_after();
+                    const uint2 bw = bad[2 * (tile & 7) + hh];
+                    const int kh = k0 + 64 * hh;
+                    // a half that some row sees only in part, or with keys on bad pages
+                    const bool cut = kh + 63 > pmin || (a.window > 0 && kh <= pmax - a.window && kh + 64 > a.sinks) ||
+                                     (bw.x | bw.y);
                     // the half's keys that this row sees, as bits
                     uint32_t see0 = ~0u, see1 = ~0u;
                     if (cut) {
                         const int h0 = hi - 64 * hh, l0 = lo - 64 * hh, s0 = sk - 64 * hh;
-                        see0 = below(h0 + 1) & (~below(l0 + 1) | below(s0)) & ~(hh ? bw.z : bw.x);
-                        see1 = below(h0 - 31) & (~below(l0 - 31) | below(s0 - 32)) & ~(hh ? bw.w : bw.y);
+                        see0 = below(h0 + 1) & (~below(l0 + 1) | below(s0)) & ~bw.x;
+                        see1 = below(h0 - 31) & (~below(l0 - 31) | below(s0 - 32)) & ~bw.y;
                     }
                     auto mask = [&](float* s, uint32_t see) {
 #pragma unroll
                         for (int c = 0; c < 32; c++)
                             if (!((see >> c) & 1)) s[c] = -INFINITY;
                     };
-                    if (fresh) {
+                    // the half's largest score, for the rows that need it
+                    auto largest = [&] {
                         float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int c = 0; c < 2; c++) {
@@ -474,14 +480,17 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
 #pragma unroll
                             for (int i = 0; i < 32; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
                         }
-                        m = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.sl2;
+                        return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.sl2;
+                    };
+                    if (__any_sync(0xffffffffu, m == -INFINITY)) {          // rows that have seen no key yet
+                        const float mx = largest();
+                        if (m == -INFINITY) m = mx;                         // O is zero, or not written
                     }
                     uint32_t pk[32];
-                    float2 sum;
+                    float sum;
                     for (;;) {
                         const float off = m == -INFINITY ? 0.0f : -m;
                         float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                        float t2[2] = {-INFINITY, -INFINITY};
                         float x[64];                      // all of the half at once: one wait, and the exponentials
                         tmem_ld32(th, reinterpret_cast<uint32_t*>(x));       // back to back (16 at a time took twice as long)
                         tmem_ld32(th + 32, reinterpret_cast<uint32_t*>(x) + 32);
@@ -494,20 +503,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                         for (int i = 0; i < 32; i++) {
                             const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2),
                                                    make_float2(off, off));
-                            t2[i & 1] = fmaxf(t2[i & 1], fmaxf(y.x, y.y));
                             const float2 e = make_float2(ex2(y.x), ex2(y.y));
                             s2[i & 1] = fadd2(s2[i & 1], e);
                             pk[i] = pack_h2(e.x, e.y);
                         }
-                        sum = fadd2(s2[0], s2[1]);
-                        const float top = fmaxf(t2[0], t2[1]);           // the maximum, from the reference
-                        const bool up = top > (m == -INFINITY ? -INFINITY : RAISE);
+                        s2[0] = fadd2(s2[0], s2[1]);
+                        sum = s2[0].x + s2[0].y;
+                        // below it every weight fits f16; past it some score is 2^9 above the reference
+                        const bool up = sum >= TOO_LARGE;
                         if (!__any_sync(0xffffffffu, up)) break;
+                        const float top = largest(), mx = up ? fmaxf(m, top) : m;
                         if (!fresh) {
                             // the half before: the last tile's second, or this tile's first
                             if (!(ok = wait_warp(&o_done[2 * t + (hh ^ 1)], (hh ? seq : seq - 1) & 1))) break;
                             tc_after();
-                            const float f = !up ? 1.0f : m == -INFINITY ? 0.0f : ex2(-top);
+                            const float f = up ? ex2(m - mx) : 1.0f;
 #pragma unroll
                             for (int c = 0; c < HD / 32; c++) {
                                 uint32_t o[32];
@@ -519,11 +529,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                             }
                             l *= f;
                         }
-                        if (up) m = m == -INFINITY ? top : m + top;
+                        m = mx;
                     }
                     if (!ok) break;
-                    tmem_st32(ts + 32 * hh, pk);          // over scores that are read
-                    l += sum.x + sum.y;
+                    tmem_st32(th, pk);                    // over scores that are read
+                    l += sum;
                     tmem_wait_st();
                     tc_before();
                     __syncwarp();
@@ -761,19 +771,20 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         // ================================ MMAs ==========================================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp == W_MMA) {
-            constexpr uint32_t I1 = idesc(PK, false), I2 = idesc(HD, true);
+            constexpr uint32_t I1 = idesc(PK / 2, false), I2 = idesc(HD, true);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const uint64_t dq = desc_k(smem_u32(smem) + L::OFF_Q), dk = desc_k(smem_u32(smem) + L::OFF_K),
                            dv = desc_mn(smem_u32(smem) + L::OFF_V);
             uint32_t ph = 0;                               // parities of q_full (bits 0, 1) and p_full (2, 3)
-            auto scores = [&](int t, int s) {              // S_t = Q_t K^T
+            auto scores = [&](int t, int s, int c) {       // S_t = Q_t K^T over half c of the tile's keys
 #pragma unroll
-                for (int c = 0; c < HD / 64; c++)
-                    mma_ss(tm + 128 * t, dq + (t * L::TILE + c * L::HALF) / 16, dk + (s * L::TILE + c * L::HALF) / 16, I1, c);
-                tc_commit(&s_full[t]);
+                for (int d = 0; d < HD / 64; d++)
+                    mma_ss(tm + 128 * t + 64 * c, dq + (t * L::TILE + d * L::HALF) / 16,
+                           dk + (s * L::TILE + d * L::HALF + c * 64 * 128) / 16, I1, d);
+                tc_commit(&s_full[2 * t + c]);
             };
             auto output = [&](int t, int s, int c, bool add) {   // O_t (+)= P_t V over half c of the tile's keys
-                mma_ts(tm + 256 + HD * t, tm + 128 * t + 32 * c, dv + (s * L::TILE + c * 64 * 128) / 16, I2, add ? 1u : 0u);
+                mma_ts(tm + 256 + HD * t, tm + 128 * t + 64 * c, dv + (s * L::TILE + c * 64 * 128) / 16, I2, add ? 1u : 0u);
                 tc_commit(&o_done[2 * t + c]);
             };
             int it = 0;
@@ -789,30 +800,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     if (!(ok = wait_warp(&q_full[t], (ph >> t) & 1))) break;
                     ph ^= 1u << t;
                     tc_after();
-                    scores(t, it % KV_STAGES);
+                    scores(t, it % KV_STAGES, 0);
+                    scores(t, it % KV_STAGES, 1);
                 }
                 if (!ok) break;
                 tc_commit(&k_empty[it % KV_STAGES]);
                 for (int j = 0; j < nt && ok; j++, it++) {
                     const int s = it % KV_STAGES, sn = (it + 1) % KV_STAGES;
                     if (!(ok = wait_warp(&v_full[s], (it / KV_STAGES) & 1))) break;
-                    for (int t = 0; t < tiles; t++) {
-                        for (int c = 0; c < 2; c++) {
+                    if (j + 1 < nt && !(ok = wait_warp(&k_full[sn], ((it + 1) / KV_STAGES) & 1))) break;
+                    for (int c = 0; c < 2 && ok; c++)
+                        for (int t = 0; t < tiles; t++) {
                             if (!(ok = wait_warp(&p_full[2 * t + c], (ph >> (2 + t)) & 1))) break;
                             tc_after();
                             output(t, s, c, j > 0 || c > 0);
+                            if (j + 1 < nt) scores(t, sn, c);
                         }
-                        if (!ok) break;
-                        ph ^= 4u << t;
-                        if (j + 1 < nt) {
-                            if (t == 0) {
-                                if (!(ok = wait_warp(&k_full[sn], ((it + 1) / KV_STAGES) & 1))) break;
-                                tc_after();
-                            }
-                            scores(t, sn);
-                        }
-                    }
                     if (!ok) break;
+                    ph ^= tiles == 2 ? 12u : 4u;
                     tc_commit(&v_empty[s]);
                     if (j + 1 < nt) tc_commit(&k_empty[sn]);
                 }
@@ -830,39 +835,53 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     }
 }
 
-// joins the parts of item x, kv head y, rows 32 z ..: lane = row, a warp takes CW columns
+// Joins the parts of item x, kv head y, rows 32 z ..: lane = row, a warp takes CW columns.
+// The parts' (m, l) come first (all at once, into shared memory), then eight parts' outputs
+// at a time.
 constexpr int JT = 512;
 template <int HD, int GRP>
 __global__ void __launch_bounds__(JT) k_prefill_join(const __grid_constant__ PrefillArgs a)
 {
     constexpr int CW = HD / (JT / 32);
+    extern __shared__ float2 ml[];            // [parts][32]: m and l
     tb_pdl_wait();
     tb_pdl_trigger();
-    const int h = blockIdx.y, nKv = a.kv.nKv, c0 = (threadIdx.x >> 5) * CW;
-    const int row = 32 * blockIdx.z + (threadIdx.x & 31), qi = row / GRP;
-    for (int i = blockIdx.x; i < a.head[1]; i += gridDim.x) {
+    const int h = blockIdx.y, nKv = a.kv.nKv, lane = threadIdx.x & 31, wid = threadIdx.x >> 5, c0 = wid * CW;
+    const int row = 32 * blockIdx.z + lane, qi = row / GRP;
+    const int split = a.head[1];
+    for (int i = blockIdx.x; i < split; i += gridDim.x) {
         const Item it = a.items[i];
-        if (it.parts < 2 || 32 * (int)blockIdx.z >= it.nq * GRP) continue;
+        if (32 * (int)blockIdx.z >= it.nq * GRP) continue;
         const float2* pml = a.PML + ((long long)it.slot0 * nKv + h) * ROWS + row;
         const uint32_t* po = a.PO + (((long long)it.slot0 * nKv + h) * HD / 2 + c0 / 2) * ROWS + row;
+        __syncthreads();                      // the last item's are read
+        for (int p = wid; p < it.parts; p += JT / 32) ml[p * 32 + lane] = pml[(long long)p * nKv * ROWS];
+        __syncthreads();
         float M = -INFINITY;
-#pragma unroll 8
-        for (int p = 0; p < it.parts; p++) M = fmaxf(M, pml[(long long)p * nKv * ROWS].x);
+        for (int p = 0; p < it.parts; p++) M = fmaxf(M, ml[p * 32 + lane].x);
         const float off = M == -INFINITY ? 0.0f : M;
         float l = 0.0f, o[CW];
 #pragma unroll
         for (int c = 0; c < CW; c++) o[c] = 0.0f;
-#pragma unroll 4
-        for (int p = 0; p < it.parts; p++) {
-            const float2 ml = pml[(long long)p * nKv * ROWS];
-            const float e = ml.y * exp2f(ml.x - off);
-            l += e;
+        for (int p0 = 0; p0 < it.parts; p0 += 8) {
+            uint32_t v[8][CW / 2];
 #pragma unroll
-            for (int c = 0; c < CW / 2; c++) {
-                const uint32_t v = po[((long long)p * nKv * HD / 2 + c) * ROWS];
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                o[2 * c] = fmaf(f.x, e, o[2 * c]);
-                o[2 * c + 1] = fmaf(f.y, e, o[2 * c + 1]);
+            for (int k = 0; k < 8; k++)
+#pragma unroll
+                for (int c = 0; c < CW / 2; c++)
+                    if (p0 + k < it.parts) v[k][c] = po[((long long)(p0 + k) * nKv * HD / 2 + c) * ROWS];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                if (p0 + k >= it.parts) break;
+                const float2 x = ml[(p0 + k) * 32 + lane];
+                const float e = x.y * exp2f(x.x - off);
+                l += e;
+#pragma unroll
+                for (int c = 0; c < CW / 2; c++) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[k][c]));
+                    o[2 * c] = fmaf(f.x, e, o[2 * c]);
+                    o[2 * c + 1] = fmaf(f.y, e, o[2 * c + 1]);
+                }
             }
         }
         if (qi >= it.nq) continue;
@@ -917,7 +936,7 @@ int launch_prefill(tb_ctx* ctx, const PrefillArgs& a)
     const int grid = (int)std::min<long long>(a.sms, (long long)a.max_parts * a.kv.nKv);
     if (e == cudaSuccess) e = tb_launch(ctx, kern, dim3(grid), dim3(THREADS), (size_t)smem, a);
     if (e == cudaSuccess) e = tb_launch(ctx, k_prefill_join<HD, GRP>, dim3(std::min(a.max_items, a.max_slots), a.kv.nKv, ROWS / 32),
-                                           dim3(JT), 0, a);
+                                           dim3(JT), (size_t)(a.max_slots / 2) * 32 * sizeof(float2), a);
     if (e != cudaSuccess) return tb_fail(ctx, TB_ERR_CUDA, "attn_prefill_paged launch: %s", cudaGetErrorString(e));
     return TB_OK;
 }
