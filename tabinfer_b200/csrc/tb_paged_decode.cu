@@ -119,7 +119,8 @@ struct RingLayout {
     static constexpr int ROWS = KT * HD, SCALES = KT * NG * 4;
     static constexpr int V = ROWS, KS = 2 * ROWS, VS = 2 * ROWS + SCALES;
     static constexpr int STAGE = 2 * ROWS + 2 * SCALES;          // 9216 or 4608: whole swizzle atoms
-    static constexpr int NST = GRP <= 2 || HD == 64 ? 3 : 2;     // tiles in flight a warp
+    // tiles in flight a warp (three: 131001 rows 67.3 us against 62.6)
+    static constexpr int NST = 2;
     static constexpr int WORDS = GRP * HD * 4;                   // [GRP][NG][KT] words = [GRP][HD] floats
     static constexpr int OFF_WORDS = W * NST * STAGE;
     static constexpr int OFF_M = OFF_WORDS + W * WORDS;          // float [2][W][GRP] m and l
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
 
         for (; c.tile() && alive; c.i += tw, used++) {
             const int s = used % NST;
-            if (!__all_sync(0xffffffffu, mbar_wait(&full[s], (used / NST) & 1))) {
+            if (!__all_sync(0xffffffffu, mbar_test(&full[s], (used / NST) & 1) || mbar_wait(&full[s], (used / NST) & 1))) {
                 if (lane == 0) atomicExch(a.kv.err, ERR_PAGED_WAIT);
                 alive = false;
                 break;
