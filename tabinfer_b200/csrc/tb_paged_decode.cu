@@ -232,15 +232,27 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     if (u0 >= u1) return;
 
     const int box = min(KT, 1 << a.kv.log_page);          // rows a copy
-    // the tile at the walk's place -> ring stage s
+    // The tile at the walk's place: look() requests the lane's page number (a lane a key; a page is looked up
+    // when one of its rows in this tile is seen), issue() sends the copies into ring stage s a tile's work
+    // later, when the number is there.
+    int pkey = 0, ppage = 0;
+    bool psee = false, plook = false;
+    auto look = [&](const Walk& p) {
+        pkey = p.seen.tile(p.i) * KT + lane;
+        psee = key_seen(pkey, p.n - 1, a.window, a.sinks);
+        const unsigned any = __ballot_sync(0xffffffffu, psee);
+        plook = box == KT || (any & (0xffffu << (lane & 16)));
+        if (plook) ppage = __ldg(a.kv.table + (long long)p.b * a.kv.max_pages + (pkey >> a.kv.log_page));
+    };
     auto issue = [&](const Walk& p, int s) {
-        const int key = p.seen.tile(p.i) * KT + lane, ph = p.head(a, wid);
-        const bool see = key_seen(key, p.n - 1, a.window, a.sinks);
-        const unsigned any = __ballot_sync(0xffffffffu, see);
-        // a page is looked up when one of its rows in this tile is seen
-        const unsigned mine = box == KT ? any : any & (0xffffu << (lane & 16));
-        const int row = mine ? a.kv.row(p.b, key) : -1;
+        const int ph = p.head(a, wid);
+        int row = -1;
+        if (plook) {
+            if ((unsigned)ppage < (unsigned)a.kv.n_pages) row = (ppage << a.kv.log_page) | (pkey & ((1 << a.kv.log_page) - 1));
+            else atomicExch(a.kv.err, ERR_PAGED_PAGE);
+        }
         const int row16 = __shfl_sync(0xffffffffu, row, 16);
+        const bool see = psee;
         const unsigned ok = __ballot_sync(0xffffffffu, see && row >= 0);
         uint8_t* st = ring + s * L::STAGE;
         if (lane == 0) {
@@ -273,6 +285,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     int issued = 0, used = 0;
     bool alive = true;
     for (; issued < NST && p.part(); issued++) {
+        look(p);
         issue(p, issued);
         p.advance(a, wid);
     }
@@ -344,6 +357,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
 
         for (; c.tile() && alive; c.i += tw, used++) {
             const int s = used % NST;
+            if (p.part()) look(p);
             if (!__all_sync(0xffffffffu, mbar_test(&full[s], (used / NST) & 1) || mbar_wait(&full[s], (used / NST) & 1))) {
                 if (lane == 0) atomicExch(a.kv.err, ERR_PAGED_WAIT);
                 alive = false;
@@ -538,14 +552,14 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
 }
 
 // Joins the parts of kv head x of sequence y; those that one CTA held are done.  The parts'
-// factors 2^(m - M) come first (in shared memory), then each thread sums a float4 column of
+// (m, l) come first, all at once into shared memory, then each thread sums a float4 column of
 // every CT-th part, eight loads in flight, and the CT sums are added in order.
 template <int HD, int GRP>
 __global__ void __launch_bounds__(CT) k_paged_combine(const __grid_constant__ DecArgs a)
 {
     constexpr int COLS = GRP * HD / 4, P = CT / COLS;
     static_assert(CT % COLS == 0 && CT / 32 >= GRP, "whole columns, a warp a q head");
-    extern __shared__ __align__(16) float fac[];     // [np][GRP]
+    extern __shared__ __align__(16) float2 ml[];     // [np][GRP]: m and l, then the factor 2^(m - M) for m
     __shared__ float4 part[P][COLS];
     __shared__ float sl[GRP];
     __shared__ int plan[CT / 32 + 3];
@@ -566,16 +580,21 @@ __global__ void __launch_bounds__(CT) k_paged_combine(const __grid_constant__ De
     // part k is CTA c0 + k's: its first part, but for a pair that starts inside CTA c0's range
     const int first = u0 == c0 * per ? 0 : 1, np = c1 - c0 + 1;
     auto slot = [&](int k) { return (size_t)((2 * (c0 + k) + (k == 0 ? first : 0)) * hg + (h & (hg - 1))) * GRP; };
+    // every part's (m, l) at once, then a warp a q head over them in shared memory
+    for (int i = tid; i < np * GRP; i += CT) {
+        const int k = i / GRP;
+        ml[i] = a.PML[slot(k) + i - k * GRP];
+    }
+    __syncthreads();
     if (wid < GRP) {
         float x = NEG_BIG;
-        for (int k = lane; k < np; k += 32) x = fmaxf(x, a.PML[slot(k) + wid].x);
+        for (int k = lane; k < np; k += 32) x = fmaxf(x, ml[k * GRP + wid].x);
         x = warp_max(x);
         float l = 0.0f;
         for (int k = lane; k < np; k += 32) {
-            const float2 ml = a.PML[slot(k) + wid];
-            const float e = exp2f(ml.x - x);
-            fac[k * GRP + wid] = e;
-            l = fmaf(ml.y, e, l);
+            const float e = exp2f(ml[k * GRP + wid].x - x);
+            l = fmaf(ml[k * GRP + wid].y, e, l);
+            ml[k * GRP + wid].x = e;
         }
         l = warp_sum(l);
         if (lane == 0) {
@@ -595,7 +614,7 @@ __global__ void __launch_bounds__(CT) k_paged_combine(const __grid_constant__ De
 #pragma unroll
         for (int i = 0; i < 8; i++)
             if (k + i * P < np) {
-                const float e = fac[(k + i * P) * GRP + g];
+                const float e = ml[(k + i * P) * GRP + g].x;
                 o.x = fmaf(v[i].x, e, o.x);
                 o.y = fmaf(v[i].y, e, o.y);
                 o.z = fmaf(v[i].z, e, o.z);
@@ -690,7 +709,7 @@ int launch_decode(tb_ctx* ctx, const DecArgs& a)
         if (e == cudaSuccess && ctx->device < 64) attr_set[ctx->device] = true;
     }
     if (e == cudaSuccess) e = tb_launch(ctx, kern, dim3(a.grid), dim3(NT), (size_t)smem, a);
-    if (e == cudaSuccess) e = tb_launch(ctx, k_paged_combine<HD, GRP>, dim3(a.kv.nKv, a.kv.batch), dim3(CT), (size_t)a.grid * GRP * 4, a);
+    if (e == cudaSuccess) e = tb_launch(ctx, k_paged_combine<HD, GRP>, dim3(a.kv.nKv, a.kv.batch), dim3(CT), (size_t)a.grid * GRP * sizeof(float2), a);
     if (e == cudaSuccess && a.weights)
         e = tb_launch(ctx, k_paged_weights<GRP>,
                       dim3(tb_cdiv((long long)a.kv.max_pages << a.kv.log_page, 1024), a.kv.nKv, a.kv.batch), dim3(256), 0, a);
