@@ -11,7 +11,7 @@
 namespace {
 
 constexpr int ST = 1024;          // threads of a selecting CTA
-constexpr int DIGIT = 11, BINS = 1 << DIGIT;
+constexpr int DIGIT = 8, BINS = 1 << DIGIT;   // larger digits cost more in reading the other CTAs' counts than they save
 constexpr int MAX_CLUSTER = 8;    // CTAs a sequence (portable)
 constexpr int SLOTS = 2048;       // rows a CTA at least, before a sequence gets another one
 constexpr int KEPT_KEYS = 16;     // keys a thread holds in registers; those beyond are read again each step
@@ -66,17 +66,19 @@ __global__ void __launch_bounds__(256) k_evict_scores(const EvictArgs a)
 }
 
 // A cluster a sequence.  Its CTAs share the middle rows (between the first and the last
-// ones that stay): the need-th largest score by radix, 11 bits a step from the top -- each
-// CTA counts its rows' digits, all add up the counts of all over distributed shared memory --
-// until the digit's whole class is needed (two or three steps where scores differ, six at
-// most), then the rows above it and, in order, as many of its class as are still needed.
-// Bound by the steps' barriers.
+// ones that stay): the need-th largest score by radix, 8 bits a step from the highest bit in
+// which two scores differ (above it a digit would be the same for all, and its additions in
+// shared memory would queue) -- each CTA counts its rows' digits, all add up the counts of all
+// over distributed shared memory -- until the digit's whole class is needed (three steps where
+// scores differ, eight at most), then the rows above it and, in order, as many of its class as
+// are still needed.  Bound by the steps' barriers.
 __global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
 {
     __shared__ unsigned hist[2][BINS];       // two: a step's counts are read while the next one's are made
     __shared__ int wsum[ST / 32];
     __shared__ int found_bin, found_left, found_all;
     __shared__ int wkeep[ST / 32], wtie[ST / 32], mine[2];
+    __shared__ unsigned differ[2];           // bits in which this CTA's scores differ from the first one
     tb_pdl_wait();
     tb_pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -106,34 +108,49 @@ __global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
         const int j = j0 + tid + i * ST;
         own[i] = j < j1 ? keys[j] : 0;
     }
-    unsigned long long prefix = 0;           // of the class looked at: the key's bits from `shift` on
-    int shift = 64, remaining = need;
+    // the bits that all scores share
+    const unsigned long long ref = __ldcg(keys + lo);
+    if (tid < 2) differ[tid] = 0;
+    __syncthreads();
+    {
+        unsigned long long d = 0;
+#pragma unroll
+        for (int i = 0; i < KEPT_KEYS; i++)
+            if (j0 + tid + i * ST < j1) d |= own[i] ^ ref;
+        for (int j = j0 + tid + KEPT_KEYS * ST; j < j1; j += ST) d |= keys[j] ^ ref;
+        const unsigned d0 = __reduce_or_sync(0xffffffffu, (unsigned)d), d1 = __reduce_or_sync(0xffffffffu, (unsigned)(d >> 32));
+        if (lane == 0) {
+            atomicOr(&differ[0], d0);
+            atomicOr(&differ[1], d1);
+        }
+    }
+    cluster_sync();
+    unsigned long long all = 0;
+#pragma unroll
+    for (int r = 0; r < MAX_CLUSTER; r++)
+        if (r < ncta) all |= (unsigned long long)remote(&differ[1], r) << 32 | remote(&differ[0], r);
+    int shift = 64 - __clzll((long long)all), remaining = need;
+    unsigned long long prefix = shift < 64 ? ref >> shift : 0;   // of the class looked at: the key's bits from `shift` on
     for (int step = 0; shift > 0; step++) {
         const int bits = min(DIGIT, shift), next = shift - bits;
         unsigned* cnt = hist[step & 1];
         for (int i = tid; i < BINS; i += ST) cnt[i] = 0;
         __syncthreads();
-        // equal digits of a warp are added at once: of a step's rows most have the same few (scores of
-        // one magnitude share their upper bits; one addition a row took 100 us for 131072)
         auto count = [&](unsigned long long k, int j) {
-            const bool in = j < j1 && (shift == 64 || (k >> shift) == prefix);
-            if (!__any_sync(0xffffffffu, in)) return;
-            const unsigned d = in ? (unsigned)(k >> next) & ((1u << bits) - 1) : BINS;
-            const unsigned same = __match_any_sync(0xffffffffu, d);
-            if (in && (same & ((1u << lane) - 1)) == 0) atomicAdd(&cnt[d], (unsigned)__popc(same));
+            if (j < j1 && (shift == 64 || (k >> shift) == prefix)) atomicAdd(&cnt[(k >> next) & ((1u << bits) - 1)], 1u);
         };
 #pragma unroll
         for (int i = 0; i < KEPT_KEYS; i++) count(own[i], j0 + tid + i * ST);
-        for (int j = j0 + tid + KEPT_KEYS * ST; j - lane < j1; j += ST) count(j < j1 ? keys[j] : 0, j);
+        for (int j = j0 + tid + KEPT_KEYS * ST; j < j1; j += ST) count(keys[j], j);
         cluster_sync();
-        // classes from the top: thread t has 2047 - 2t and the one below
-        int c[2] = {0, 0};
+        // classes from the top: thread t < 256 has 255 - t
+        int c = 0;
+        if (tid < BINS) {
 #pragma unroll
-        for (int r = 0; r < MAX_CLUSTER; r++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                if (r < ncta) c[i] += (int)remote(&cnt[BINS - 1 - 2 * tid - i], r);
-        int x = c[0] + c[1];
+            for (int r = 0; r < MAX_CLUSTER; r++)
+                if (r < ncta) c += (int)remote(&cnt[BINS - 1 - tid], r);
+        }
+        int x = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, x, o);
@@ -141,16 +158,14 @@ __global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
         }
         if (lane == 31) wsum[wid] = x;
         __syncthreads();
-        int above = x - c[0] - c[1];
-        for (int i = 0; i < wid; i++) above += wsum[i];
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            if (above < remaining && remaining <= above + c[i]) {
-                found_bin = BINS - 1 - 2 * tid - i;
+        if (tid < BINS) {
+            int above = x - c;
+            for (int i = 0; i < wid; i++) above += wsum[i];
+            if (above < remaining && remaining <= above + c) {
+                found_bin = BINS - 1 - tid;
                 found_left = remaining - above;
-                found_all = remaining == above + c[i];
+                found_all = remaining == above + c;
             }
-            above += c[i];
         }
         __syncthreads();
         prefix = (prefix << bits) | (unsigned)found_bin;
@@ -166,7 +181,7 @@ __global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
         tie = __ballot_sync(0xffffffffu, j < k1 && k == prefix);
     };
     int na = 0, nt = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int j = k0; j < k1; j += 32) {
         unsigned above, tie;
         look(j + lane, above, tie);
@@ -193,7 +208,7 @@ __global__ void __launch_bounds__(ST) k_evict_select(const EvictArgs a)
         ka += wkeep[i];
         kt += wtie[i];
     }
-#pragma unroll 4
+#pragma unroll 8
     for (int j = k0; j < k1; j += 32) {
         unsigned above, tie;
         look(j + lane, above, tie);
