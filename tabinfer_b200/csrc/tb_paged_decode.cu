@@ -742,7 +742,7 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, float* ou
     TB_REQUIRE(ctx, out && qr && lens, "null pointer");
     TB_REQUIRE(ctx, TB_ALIGNED(out, 16) && TB_ALIGNED(qr, 16), "q and out must be 16-byte aligned");
     TB_REQUIRE(ctx, window >= 0 && sinks >= 0, "window and sinks must not be negative");
-    TB_REQUIRE(ctx, kv->batch * kv->nKv * (kv->max_pages * kv->page_rows / KT + 1) < (1LL << 31),
+    TB_REQUIRE(ctx, kv->batch * kv->nKv * (kv->max_pages * kv->page_rows / KT + 1) < (1LL << 30),
                "batch x heads x rows too large");
     DeviceGuard dev(ctx->device);
     const DecWs w = dec_ws(ctx, kv, nHq, weights != nullptr);
@@ -767,8 +767,9 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, float* ou
         a.weights = weights;
     }
     a.nHq = (int)nHq;
-    a.window = (int)std::min<int64_t>(window, 1LL << 30);
-    a.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
+    const int64_t cap = kv->max_pages * kv->page_rows;
+    a.window = window < cap ? (int)window : 0;             // a window of every row is none
+    a.sinks = (int)std::min<int64_t>(sinks, cap);
     a.grid = w.grid;
     a.log_hg = log_group(kv->nKv);
     a.qscale = 1.4426950408889634f / (127.0f * sqrtf((float)kv->hd));

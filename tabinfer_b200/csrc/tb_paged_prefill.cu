@@ -999,8 +999,9 @@ TB_API int tb_attn_prefill_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, uint16_t
     a.T = (int)T;
     a.nHq = (int)nHq;
     a.grp = (int)(nHq / kv->nKv);
-    a.window = (int)std::min<int64_t>(window, 1LL << 30);
-    a.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
+    const int64_t cap = kv->max_pages * kv->page_rows;
+    a.window = window < cap ? (int)window : 0;             // a window of every row is none
+    a.sinks = (int)std::min<int64_t>(sinks, cap);
     a.sms = ctx->num_sms;
     a.max_items = w.items;
     a.max_parts = w.parts;

@@ -4,9 +4,12 @@ attention_prefill_paged_q8, kv_evict_paged_q8) against plain 64-bit forms (paged
 Tolerances.  u = 2^-24.  Decode: a score is a sum of hd exact or once-rounded products in
 f32, so it is off by at most (hd + 8) u sum|q_i k_i| / sqrt(hd) =: d; every weight is then
 off by at most a factor 1 + 2 d + (S + 16) u, and an output by that times the largest |v|
-seen.  Prefill: q and k rounded to f16 put a score off by at most 2^-10 of sum|q_i k_i| /
-sqrt(hd) =: d, p and v rounded to f16 add 2^-10, and the bf16 output 2^-8 of itself.  The
-sums are taken from the reference.  Prep: rows formed in 64 bits, so bytes and scales are
+seen.  Prefill: q, a key's scale and their product with its byte are rounded to f16 (2^-11
+each), which could put a score off by 1.5 * 2^-10 of sum|q_i k_i| / sqrt(hd) if every rounding
+of a sum had the same sign; d := 2^-10 of it is asked for.  A weight is then off by a factor
+1 + 2 d; p, v (scale and product) and a joined part's output add 2^-11 each, 2^-9 of the
+largest |v| together, and the bf16 output 2^-8 of itself.  The sums are taken from the
+reference.  Prep: rows formed in 64 bits, so bytes and scales are
 those of the reference and qr is within half a step of f32."""
 import pytest
 import torch
@@ -202,6 +205,58 @@ def test_prefill_unseen_rows_are_not_used(cuda):
     _prefill_check(c, lens, ts, 4, window, sinks)
 
 
+def test_freed_pages_are_not_looked_up(cuda):
+    """table entries of pages that no row under the window sees may be anything (their pages were freed)"""
+    c = ref.Cache(25, 2, 40, 16, 2, 64)
+    lens, window, sinks = [600, 333], 100, 5
+    whole = c.table.clone()
+    for b, n in enumerate(lens):
+        c.table[b, 1:(n - window) // 16] = -1
+        c.table[b, -(-n // 16):] = 2 ** 31 - 1
+    q = torch.randn(2, 4 * 64, generator=c.g).cuda()
+    a = tb.attention_decode_paged_q8(q, c.dev(), c.table.cuda(), _ints(lens), 4, 2, 64, window=window, sinks=sinks)
+    b = tb.attention_decode_paged_q8(q, c.dev(), whole.cuda(), _ints(lens), 4, 2, 64, window=window, sinks=sinks)
+    assert torch.equal(a, b)
+    args = (_ints([0, 1, 2]), _ints(lens), 4, 2, 64)
+    a = tb.attention_prefill_paged_q8(q, c.dev(), c.table.cuda(), *args, window=window, sinks=sinks)
+    b = tb.attention_prefill_paged_q8(q, c.dev(), whole.cuda(), *args, window=window, sinks=sinks)
+    assert torch.equal(a, b)
+    assert tb.default_context(0).device_error() == 0
+
+
+def test_prefill_many_sequences(cuda):
+    """more sequences than the plan has threads, most of them short, some without new rows"""
+    lens = [(37 * i) % 90 + 1 for i in range(600)]
+    ts = [min(n, (11 * i) % 7) for i, n in enumerate(lens)]
+    c = ref.Cache(26, 600, 6, 16, 1, 64)
+    _prefill_check(c, lens, ts, 8, window=50, sinks=2)
+
+
+@pytest.mark.parametrize("hd,slope", [(64, 1.0), (128, 1.0), (128, -1.0), (64, 0.3)])
+def test_prefill_rising_scores(cuda, hd, slope):
+    """scores that climb (or fall) by hundreds over the keys, so the running reference has to be raised again
+    and again.  K = byte / 64, V likewise and q in eighths are exact in f16, so scores are exact; what is left
+    is P's and a joined part's rounding (2^-11 each, relative), f32 and bf16's 2^-8 of the output."""
+    n, t, nKv, nHq = 900, 140, 2, 4
+    c = ref.Cache(27, 1, 60, 16, nKv, hd)
+    c.Ks[:] = 127.0 / 64
+    c.Vs[:] = 127.0 / 64
+    ramp = (slope * 127.0 * torch.arange(n) / n).round().to(torch.int8)
+    rows = c.rows(0, torch.arange(n))
+    c.Kq.view(-1, nKv, hd)[rows, :, 0] = ramp[:, None]
+    q = (torch.randint(-8, 9, (t, nHq * hd), generator=c.g).float() / 8)
+    q.view(t, nHq, hd)[:, :, 0] = 1600.0
+    got = tb.attention_prefill_paged_q8(q.cuda(), c.dev(), c.table.cuda(), _ints([0, t]), _ints([n]), nHq, nKv,
+                                        hd).cpu().double()
+    for i in list(range(0, t, 13)) + [t - 1]:
+        o, _, _, big = ref.attend(c, 0, q[i], n - t + i, nHq)
+        tol = 2.0 ** -8 * o.abs() + big * (2.0 ** -10 + 2.0 ** -14)
+        assert ((got[i].reshape(nHq, hd) - o).abs() <= tol).all(), i
+    dec = tb.attention_decode_paged_q8(q[-1:].cuda(), c.dev(), c.table.cuda(), _ints([n]), nHq, nKv, hd).cpu().double()
+    o, _, mag, big = ref.attend(c, 0, q[-1], n - 1, nHq)
+    assert float((dec[0].reshape(nHq, hd) - o).abs().max()) <= (2 * (hd + 8) * U * mag + (n + 16) * U) * big
+
+
 def test_prefill_last_row_is_decode(cuda):
     c = ref.Cache(24, 1, 20, 32, 4, 128)
     q = torch.randn(50, 8 * 128, generator=c.g).cuda()
@@ -298,6 +353,22 @@ def test_evict(cuda, lens, budget, sinks, recent, page, new_page, kind):
             assert (d[r1[len(want):]] == 9).all()              # the rest of the new pages stays as it was
     for have, need in zip(kv, (c.Kq, c.Ks, c.Vq, c.Vs)):
         assert torch.equal(have.cpu(), need)
+
+
+def test_evict_more_rows_than_registers(cuda):
+    """a cache beyond the rows that the selecting threads hold in registers, with ties"""
+    n, budget, page = 150001, 20000, 256
+    c = ref.Cache(42, 1, n // page + 1, page, 1, 64, fill=False)
+    g = torch.Generator().manual_seed(6)
+    for w in (torch.randn(1, 1, c.cap, generator=g).abs(), torch.randint(0, 5, (1, 1, c.cap), generator=g).float(),
+              torch.ones(1, 1, c.cap)):
+        fresh = torch.arange(-(-budget // page), dtype=torch.int32)[None]
+        dst = [torch.zeros(fresh.numel(), page, t.shape[-1], dtype=t.dtype, device="cuda") for t in c.dev()]
+        kept, nl, nw = tb.kv_evict_paged_q8(c.dev(), c.table.cuda(), _ints([n]), w.cuda(), fresh.cuda(), budget, 4, 100,
+                                            1, 64, kv_out=dst)
+        want = ref.evict(w[0], n, budget, 4, 100)
+        assert kept[0].tolist() == want and int(nl) == budget
+        assert torch.equal(nw[0, 0, :budget].cpu(), w[0, 0][want])
 
 
 def test_run_of_all(cuda):
