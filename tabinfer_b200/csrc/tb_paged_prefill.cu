@@ -24,7 +24,21 @@
 //                    TMEM, V MN-major as it lies in the cache), row tile 0 and 1 in turn so
 //                    that one's softmax runs under the other's MMAs
 // Roundings: Q, dequantized K and V (and their scales) and P to f16, relative 2^-11 each; S,
-// the statistics and O in f32.
+// the statistics and O in f32 (parts' outputs pass through memory as f16).
+//
+// What bounds it.  Its operations at the bf16 rate a library product reaches (1679 TFLOP/s)
+// would take 164 us at 8192 rows (16 / 8 heads of 128); it takes 314 (876 TFLOP/s), 2048 rows
+// 48 (356), three chunks of up to 2001 rows under a window of 1024 (32 / 8 heads of 64) 147
+// (286).  A half of 64 keys takes a softmax warp about 2200 cycles, two of them sharing a
+// scheduler: 1100 to 1500 for its 64 exponentials with their sums and conversions (1024 of the
+// special function unit for both warps), the rest waits, TMEM loads and stores and the
+// barriers; the tensor cores are busy half of the time, so 64-wide heads, with half the
+// product for the same exponentials, come out at a third of the rate.  Short chunks (77 rows
+// behind 8192: 31 us) are the plan, the first tiles' latency and the join.
+// Measured and not kept: 16 softmax warps of 16 columns (362 us at 8192 rows), whole tiles of
+// 128 keys a softmax step (340), a quarter of the exponentials by polynomial (315), taking
+// turns at the exponentials (352), the next half's scores fetched ahead of the weights' store
+// (320), an MMA warp a row tile (323), raw bytes in registers (348).
 // Every wait is bounded: one that gives up sets the error word and the CTA's abort flag, all
 // roles leave, the MMA thread waits for its last commit and TMEM is freed.
 #include <cuda_bf16.h>
@@ -41,6 +55,9 @@ constexpr int NC = 4;                      // 16-byte chunks a producer thread t
 constexpr int KV_STAGES = 2;
 constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps their sums in shared memory)
 constexpr int MIN_TILES = 2;             // an item is not cut below this many tiles a part
+// cycles by which row tile 1's softmax starts a part behind tile 0's (8192 rows 321 us with none, 318 with 300, 314
+// with 900 and 1200; three 2001-row chunks under a window 154, 149, 147, 149)
+constexpr int STAGGER = 900;
 constexpr float TOO_LARGE = 32768.0f;    // sum of a half's exponentials that raises the reference maximum
 
 struct Part {
@@ -66,7 +83,8 @@ struct PrefillArgs {
     // holds a row, so a warp writes 128 contiguous bytes
     uint32_t* PO;
     float2* PML;            // [slot][nKv][ROWS]
-    int T, nHq, grp, window, sinks, sms, max_items, max_parts, max_slots;
+    int T, nHq, grp, window, sinks, sms;
+    int max_items, max_parts, max_slots;   // what the workspace holds
     float sl2;              // log2(e) / sqrt(HD)
 };
 
@@ -435,8 +453,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             const int pos = p.p0 + min(qi, p.nq - 1), pmin = max(p.p0, 0), pmax = p.p0 + p.nq - 1;
             const SeenTiles seen(pmin, pmax, a.window, a.sinks, PK);
             float m = -INFINITY, l = 0.0f;
-            bool ok = true;
-            for (int j = p.t0; j < p.t1; j++, seq++, tile++) {
+            // tile 1 a little behind tile 0: its warps share their schedulers with tile 0's, and one's exponentials
+            // then run under the other's loads, stores and waits
+            bool ok = t == 0 || wait_warp(&s_full[2 * t], seq & 1);
+            if (t == 1)
+                for (const long long c0 = clock64(); clock64() - c0 < STAGGER;) {}
+            for (int j = p.t0; ok && j < p.t1; j++, seq++, tile++) {
                 const int k0 = seen.tile(j) * PK;
                 const int hi = pos - k0, lo = a.window > 0 ? hi - a.window : -1, sk = a.sinks - k0;
                 // In two halves of 64 keys: a half's P V and the next tile's Q K^T over its place run under the
@@ -587,7 +609,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
     } else if (warp < W_MMA) {
         // ============================ K / V tiles ======================================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-                const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
+        const int pt = tid - 256;                                  // 0 .. 127: its key of a tile
         int* rows = reinterpret_cast<int*>(smem + L::OFF_ROW);
         uint2* scs = reinterpret_cast<uint2*>(smem + L::OFF_SC);    // [3][2][PK] four f16 scales
         constexpr int NG = HD / 32, CPR = HD / 16, RPU = NC * PROD / CPR;   // 16-byte chunks a row, rows a unit
