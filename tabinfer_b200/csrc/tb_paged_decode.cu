@@ -127,7 +127,9 @@ struct RingLayout {
     static constexpr int OFF_BAR = OFF_M + 2 * W * GRP * 4;      // mbarriers, then the tiles' masks
     static constexpr int BYTES = OFF_BAR + W * NST * 12;
     // CTAs an SM: 232448 bytes of shared memory, 1 KB of them a CTA the system's
-    static constexpr int OCC = 232448 / (BYTES + 1024) < 4 ? 232448 / (BYTES + 1024) : 4;
+    // at most four, with 128 registers a thread; three for eight q heads a kv head, which take 168
+    static constexpr int MOST = GRP == 8 ? 3 : 4;
+    static constexpr int OCC = 232448 / (BYTES + 1024) < MOST ? 232448 / (BYTES + 1024) : MOST;
     static_assert(OCC >= 2, "two CTAs an SM");
     static_assert(GRP * 4 * HD <= WORDS, "q's digits fit in the words");
     static_assert(W * WORDS >= (W + 3) * 4, "the plan's sums fit in the words");
@@ -203,7 +205,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, 
 // issue slots that the tile's share of the HBM rate leaves an SM; the form that converts V
 // and K to f32 takes 1180.
 template <int HD, int GRP>
-__global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ DecArgs a)
+__global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(const __grid_constant__ DecArgs a)
 {
     using L = RingLayout<HD, GRP>;
     constexpr int NG = L::NG, NN = L::NN, NST = L::NST;
@@ -235,24 +237,29 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     // The tile at the walk's place: look() requests the lane's page number (a lane a key; a page is looked up
     // when one of its rows in this tile is seen), issue() sends the copies into ring stage s a tile's work
     // later, when the number is there.
-    int pkey = 0, ppage = 0;
-    bool psee = false, plook = false;
-    auto look = [&](const Walk& p) {
-        pkey = p.seen.tile(p.i) * KT + lane;
-        psee = key_seen(pkey, p.n - 1, a.window, a.sinks);
-        const unsigned any = __ballot_sync(0xffffffffu, psee);
-        plook = box == KT || (any & (0xffffu << (lane & 16)));
-        if (plook) ppage = __ldg(a.kv.table + (long long)p.b * a.kv.max_pages + (pkey >> a.kv.log_page));
+    struct Look {
+        int key, page, head;
+        bool see, wanted;
     };
-    auto issue = [&](const Walk& p, int s) {
-        const int ph = p.head(a, wid);
+    auto look = [&](const Walk& p) {
+        Look v;
+        v.key = p.seen.tile(p.i) * KT + lane;
+        v.head = p.head(a, wid);
+        v.see = key_seen(v.key, p.n - 1, a.window, a.sinks);
+        const unsigned any = __ballot_sync(0xffffffffu, v.see);
+        v.wanted = box == KT || (any & (0xffffu << (lane & 16)));
+        v.page = v.wanted ? __ldg(a.kv.table + (long long)p.b * a.kv.max_pages + (v.key >> a.kv.log_page)) : 0;
+        return v;
+    };
+    auto issue = [&](const Look& v, int s) {
+        const int ph = v.head;
         int row = -1;
-        if (plook) {
-            if ((unsigned)ppage < (unsigned)a.kv.n_pages) row = (ppage << a.kv.log_page) | (pkey & ((1 << a.kv.log_page) - 1));
+        if (v.wanted) {
+            if ((unsigned)v.page < (unsigned)a.kv.n_pages) row = (v.page << a.kv.log_page) | (v.key & ((1 << a.kv.log_page) - 1));
             else atomicExch(a.kv.err, ERR_PAGED_PAGE);
         }
         const int row16 = __shfl_sync(0xffffffffu, row, 16);
-        const bool see = psee;
+        const bool see = v.see;
         const unsigned ok = __ballot_sync(0xffffffffu, see && row >= 0);
         uint8_t* st = ring + s * L::STAGE;
         if (lane == 0) {
@@ -284,10 +291,26 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
     p.settle(a, wid);
     int issued = 0, used = 0;
     bool alive = true;
-    for (; issued < NST && p.part(); issued++) {
-        look(p);
-        issue(p, issued);
-        p.advance(a, wid);
+    // the first part's q and the first tiles' page numbers are requested together
+    float r[NG];
+    auto load_q = [&](int g) {
+        const float* src = a.q + (long long)c.b * nHq * HD + (c.head(a, wid) * GRP + g) * HD + lane;
+#pragma unroll
+        for (int i = 0; i < NG; i++) r[i] = __ldg(src + 32 * i);
+    };
+    load_q(0);
+    {
+        Look v[NST];
+#pragma unroll
+        for (int i = 0; i < NST; i++)
+            if (p.part()) {
+                v[i] = look(p);
+                issued++;
+                p.advance(a, wid);
+            }
+#pragma unroll
+        for (int i = 0; i < NST; i++)
+            if (i < issued) issue(v[i], i);
     }
     const float f1 = (t4 & 1) ? 0.0f : 256.0f, f2 = (t4 & 1) ? 65536.0f : 1.0f;
     const int lrow = (lane & 7) + (lane & 8), lchunk = lane >> 4;    // ldmatrix x4: 16 rows x two chunks
@@ -295,19 +318,18 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
         return HD == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
     };
 
-    for (; c.part(); c.next_part(a, wid)) {
+    for (bool first = true; c.part(); c.next_part(a, wid), first = false) {
         // ---- q of this warp's head: four signed digits, one step a q head
         const int h = c.head(a, wid);
         if (tw > 1) __syncthreads();       // the last part's merge has read the words
         float qf[GRP];
 #pragma unroll
         for (int g = 0; g < GRP; g++) {
-            const float* src = a.q + (long long)c.b * nHq * HD + (h * GRP + g) * HD;
-            float r[NG], mx = 0.0f;
+            if (g > 0 || !first) load_q(g);
+            float mx = 0.0f;
             bool fine = true;
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                r[i] = __ldg(src + 32 * i + lane);
                 mx = fmaxf(mx, fabsf(r[i]));
                 fine = fine && fabsf(r[i]) <= 3.0e38f;
             }
@@ -357,7 +379,8 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
 
         for (; c.tile() && alive; c.i += tw, used++) {
             const int s = used % NST;
-            if (p.part()) look(p);
+            Look v{};
+            if (p.part()) v = look(p);
             if (!__all_sync(0xffffffffu, mbar_test(&full[s], (used / NST) & 1) || mbar_wait(&full[s], (used / NST) & 1))) {
                 if (lane == 0) atomicExch(a.kv.err, ERR_PAGED_WAIT);
                 alive = false;
@@ -494,7 +517,7 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
             }
             __syncwarp();          // the stage and the words are read
             if (p.part()) {
-                issue(p, s);
+                issue(v, s);
                 issued++;
                 p.advance(a, wid);
             }
@@ -525,22 +548,34 @@ __global__ void __launch_bounds__(NT) k_paged_decode(const __grid_constant__ Dec
         else __syncwarp();
         const bool whole = c.c0 == 0 && c.c1 == c.nc;
         const long long slot = ((2LL * cta + (c.u == u0 ? 0 : 1)) << a.log_hg) + (wid & (hg - 1));
-        // the tw warps of a head share its outputs
-        for (int i = (wid >> a.log_hg) * 32 + lane; i < GRP * HD; i += 32 * tw) {
-            const int g = i / HD, d = i % HD;
-            float M = NEG_BIG, Ls = 0.0f, O = 0.0f;
-            for (int k = wid & (hg - 1); k < W; k += hg) M = fmaxf(M, wm[k * GRP + g]);
-            for (int k = wid & (hg - 1); k < W; k += hg) {
-                const float e = exp2f(wm[k * GRP + g] - M);
-                Ls = fmaf(wl[k * GRP + g], e, Ls);
-                O = fmaf(wo[(k * GRP + g) * HD + d], e, O);
-            }
-            O *= 1.0f / 127.0f;
+        // the tw warps of a head share its outputs: a float4 a lane
+        constexpr int QPH = HD / 4;
+        const int k0 = wid & (hg - 1);
+#pragma unroll
+        for (int i = 0; i < (GRP * QPH + 31) / 32; i++) {
+            if ((i & (tw - 1)) != wid >> a.log_hg) continue;
+            const int at = 32 * i + lane, g = at / QPH, d = at % QPH * 4;
+            if (GRP * QPH < 32 && at >= GRP * QPH) continue;
+            float M = NEG_BIG, Ls = 0.0f;
+            float4 O = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < W; k++)
+                if ((k & (hg - 1)) == k0) M = fmaxf(M, wm[k * GRP + g]);
+#pragma unroll
+            for (int k = 0; k < W; k++)
+                if ((k & (hg - 1)) == k0) {
+                    const float e = exp2f(wm[k * GRP + g] - M);
+                    const float4 x = *reinterpret_cast<const float4*>(wo + (k * GRP + g) * HD + d);
+                    Ls = fmaf(wl[k * GRP + g], e, Ls);
+                    O = make_float4(fmaf(x.x, e, O.x), fmaf(x.y, e, O.y), fmaf(x.z, e, O.z), fmaf(x.w, e, O.w));
+                }
+            const float f = whole ? (Ls > 0.0f || Ls != Ls ? 1.0f / (127.0f * Ls) : 0.0f) : 1.0f / 127.0f;
+            O = make_float4(O.x * f, O.y * f, O.z * f, O.w * f);
             if (whole) {
-                a.out[(long long)c.b * nHq * HD + (h * GRP + g) * HD + d] = Ls > 0.0f || Ls != Ls ? O / Ls : 0.0f;
+                *reinterpret_cast<float4*>(a.out + (long long)c.b * nHq * HD + (h * GRP + g) * HD + d) = O;
                 if (d == 0 && a.ML) a.ML[(long long)c.b * nHq + h * GRP + g] = make_float2(M, Ls);
             } else {
-                a.PO[(slot * GRP + g) * HD + d] = O;
+                *reinterpret_cast<float4*>(a.PO + (slot * GRP + g) * HD + d) = O;
                 if (d == 0) a.PML[slot * GRP + g] = make_float2(M, Ls);
             }
         }
