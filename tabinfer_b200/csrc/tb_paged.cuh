@@ -84,10 +84,6 @@ __device__ __forceinline__ void mbar_init(uint64_t* b, unsigned count)
 {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
 }
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* b, uint32_t bytes)
-{
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
-}
 __device__ __forceinline__ void mbar_arrive(uint64_t* b)
 {
     asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}" ::"r"(smem_u32(b)) : "memory");
@@ -129,12 +125,22 @@ __device__ __forceinline__ void cp_async8(void* sdst, const void* gsrc)
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// a box of a 2-D tensor map into shared memory (x: a multiple of 16 bytes)
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar)
+// The boxes at (x, y) of two 2-D tensor maps into shared memory (x: a multiple of 16 bytes), and the
+// bytes that a barrier is to expect: run by a whole warp with uniform operands, one thread issues.
+__device__ __forceinline__ void tma_2d_elect(void* dst0, const CUtensorMap* map0, void* dst1, const CUtensorMap* map1, int x,
+                                             int y, uint64_t* bar)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-                 ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%4, %5}], [%6];\n"
+                 " @e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%2], [%3, {%4, %5}], [%6];\n}"
+                 ::"r"(smem_u32(dst0)), "l"(reinterpret_cast<uint64_t>(map0)), "r"(smem_u32(dst1)),
+                   "l"(reinterpret_cast<uint64_t>(map1)), "r"(x), "r"(y), "r"(smem_u32(bar))
                  : "memory");
+}
+__device__ __forceinline__ void mbar_expect_elect(uint64_t* bar, uint32_t bytes)
+{
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // makes a context's device the current one for a call's launches

@@ -258,23 +258,15 @@ __global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(c
             if ((unsigned)v.page < (unsigned)a.kv.n_pages) row = (v.page << a.kv.log_page) | (v.key & ((1 << a.kv.log_page) - 1));
             else atomicExch(a.kv.err, ERR_PAGED_PAGE);
         }
-        const int row16 = __shfl_sync(0xffffffffu, row, 16);
+        const int row0 = __shfl_sync(0xffffffffu, row, 0), row16 = __shfl_sync(0xffffffffu, row, 16);
         const bool see = v.see;
         const unsigned ok = __ballot_sync(0xffffffffu, see && row >= 0);
         uint8_t* st = ring + s * L::STAGE;
-        if (lane == 0) {
-            okw[s] = ok;
-            const bool second = box < KT && row16 >= 0;
-            mbar_expect_tx(&full[s], (uint32_t)(2 * HD * box * ((row >= 0) + second)));
-            if (row >= 0) {
-                tma_2d(st, &a.mk, ph * HD, row, &full[s]);
-                tma_2d(st + L::V, &a.mv, ph * HD, row, &full[s]);
-            }
-            if (second) {
-                tma_2d(st + 16 * HD, &a.mk, ph * HD, row16, &full[s]);
-                tma_2d(st + L::V + 16 * HD, &a.mv, ph * HD, row16, &full[s]);
-            }
-        }
+        if (lane == 0) okw[s] = ok;
+        const bool second = box < KT && row16 >= 0;
+        mbar_expect_elect(&full[s], (uint32_t)(2 * HD * box * ((row0 >= 0) + second)));
+        if (row0 >= 0) tma_2d_elect(st, &a.mk, st + L::V, &a.mv, ph * HD, row0, &full[s]);
+        if (second) tma_2d_elect(st + 16 * HD, &a.mk, st + L::V + 16 * HD, &a.mv, ph * HD, row16, &full[s]);
         if (see && row >= 0) {
             const long long at = ((long long)row * nKv + ph) * NG;
             if constexpr (NG == 4) {
