@@ -424,14 +424,16 @@ TB_API int tb_attn_decode_q8_batch(tb_ctx *ctx, float *out, const float *qr,
  * pools Kq/Vq int8 [n_pages][page_rows][nKv*hd], Ks/Vs f32
  * [n_pages][page_rows][nKv*hd/32]; row r of sequence b is line r % page_rows of
  * pool page table[b][r / page_rows] (sequences may share pages; entries behind a
- * sequence's last row are not read).  An element stands for q / 127 * scale
- * (bytes -127 .. 127, as every writer here leaves them).
+ * sequence's last row are not read, nor those of pages on which no row under the
+ * window lies).  An element stands for q / 127 * scale (bytes -127 .. 127 and
+ * positive scales, as every writer here leaves them).
  * page_rows 16, 32, 64, 128 or 256; hd 64 or 128; nHq/nKv 1, 2, 4 or 8; n_pages *
  * page_rows < 2^31; pools 16-byte aligned.
  * What the host cannot see is checked on the device: a page number outside the
  * pool sets the context's error word (tb_ctx_device_error) to 0x6c01 and its rows
- * are neither read nor written; a length or row that the table cannot hold, or a
- * chunk longer than its sequence, sets 0x6c02 and counts as empty.
+ * are neither read nor written; a length or row that the table cannot hold sets
+ * 0x6c02 and counts as empty, as do those rows of a chunk longer than its sequence
+ * that would stand before the sequence's first; 0x6c03: a bounded wait gave up.
  * ws: device workspace of the size that the call's _ws query gives (it depends on
  * the sizes in kv, nHq and T only), 256-byte aligned and not shared by calls that
  * may overlap; NULL takes the context's scratch, which calls of one stream share
@@ -464,7 +466,8 @@ TB_API int tb_attn_prep_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, const float
  * [batch][nKv][max_pages*page_rows] or NULL: the softmax weight of every row seen,
  * summed over the kv head's q heads, is added to it (the input of
  * tb_kv_evict_paged_q8).  Same math as tb_attn_decode_q8; results do not depend on
- * timing. */
+ * timing.  batch * nKv * (max_pages*page_rows/32 + 1) < 2^30.  With weights the
+ * workspace holds a score a sequence, q head and table row. */
 TB_API int tb_attn_decode_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, int64_t nHq, int weights, size_t *bytes);
 TB_API int tb_attn_decode_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, float *out, const float *qr,
                                    const int32_t *lens, int64_t nHq, int64_t window, int64_t sinks,
@@ -474,8 +477,10 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, float *ou
  * tb_attn_prep_paged_q8), out bf16 [T][nHq*hd] (the X that tb_gemm_int4_g32
  * takes).  Rows cu[b] .. cu[b+1]-1 (device i32 [batch+1], ascending) are the last
  * rows of sequence b's lens[b]; each sees the rows up to its own, under window and
- * sinks as above.  Rows before cu[0] and from cu[batch] on are left as they were.
- * Operands may be rounded to f16 (as in tb_attn_prefill_q8); sums in f32. */
+ * sinks as above.  Rows before cu[0] and from cu[batch] on are left as they were,
+ * as are a sequence's where cu descends or passes T (0x6c02).  q, the cache's
+ * elements and the softmax weights are rounded to f16 (as in tb_attn_prefill_q8; what
+ * passes 65504 becomes infinite); sums in f32.  At most 4096 sequences; T < 2^24. */
 TB_API int tb_attn_prefill_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, int64_t nHq, int64_t T, size_t *bytes);
 TB_API int tb_attn_prefill_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, uint16_t *out_bf16, const float *q,
                                     const int32_t *cu, const int32_t *lens, int64_t nHq, int64_t T,
@@ -483,10 +488,11 @@ TB_API int tb_attn_prefill_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, uint16_t
 
 /* Shrinks every sequence to at most `budget` rows: its first `sinks` and last
  * `recent` rows stay, then those with the largest score = sum over kv heads of
- * weights[b][h][row] (formed in 64 bits; ties go to the lower row).  The rows that
- * stay are copied in order into the pages of dst (its table; the pools of kv or
- * others; none of its pages may be one that the call reads).  kept i32 [batch][budget]: the old row
- * of each new one, -1 behind the last; new_lens i32 [batch]; new_weights f32
+ * weights[b][h][row] (formed in 64 bits; ties go to the lower row; NaN counts as the
+ * largest).  The rows that stay are copied in order into the pages of dst (its table;
+ * the pools of kv or others; none of its pages may be one that the call reads).
+ * kept i32 [batch][budget]: the old row of each new one, -1 behind the last; new_lens
+ * i32 [batch]; new_weights f32
  * [batch][nKv][dst max_pages*page_rows]: the kept rows' weights, then zeros. */
 TB_API int tb_kv_evict_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, size_t *bytes);
 TB_API int tb_kv_evict_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, const tb_paged_kv *dst, const int32_t *lens,

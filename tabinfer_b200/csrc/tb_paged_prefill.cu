@@ -54,7 +54,6 @@ constexpr int PROD = 128, W_MMA = 12;
 constexpr int NC = 4;                      // 16-byte chunks a producer thread takes at a time
 constexpr int KV_STAGES = 2;
 constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps their sums in shared memory)
-constexpr int MIN_TILES = 2;             // an item is not cut below this many tiles a part
 // cycles by which row tile 1's softmax starts a part behind tile 0's (8192 rows 321 us with none, 318 with 300, 314
 // with 900 and 1200; three 2001-row chunks under a window 154, 149, 147, 149)
 constexpr int STAGGER = 900;
@@ -179,8 +178,9 @@ __global__ void __launch_bounds__(PT) k_prefill_plan(const PrefillArgs a)
     for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
     if ((tid & 31) == 0) atomicAdd(&all_tiles, tiles);
     __syncthreads();
-    // the longest part: a CTA's share of all heads' tiles
-    const int share = (int)min(1ull << 24, max((unsigned long long)MIN_TILES, (all_tiles * a.kv.nKv + a.sms - 1) / a.sms));
+    // the longest part: a CTA's share of all heads' tiles, down to one (77 rows behind 1000: 18.0 us, with two
+    // tiles at least 19.5, with four 23.5)
+    const int share = (int)min(1ull << 24, max(1ull, (all_tiles * a.kv.nKv + a.sms - 1) / a.sms));
     const int shift = max(0, 32 - __clz(share) - CLASS_BITS);  // part lengths as at most PT classes
     for (int i = tid; i < items; i += PT) {
         const int nt = i == tid ? own.nt : item(i).nt, np = max(1, (nt + share - 1) / share);

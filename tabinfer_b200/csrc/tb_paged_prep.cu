@@ -11,6 +11,10 @@
 // into the rotation's coefficients (A = w_lo cos, B = w_hi sin, ...), formed once a row and
 // warp, a head then costs 4 multiply-adds a pair and one multiplication by 1/rms an
 // element, and the sums of four heads are reduced and inverted together.
+//
+// Four prompts of up to 2048 rows (16 / 8 heads of 128; 154 MB) take 46.6 us, 3.3 TB/s: the
+// 64-bit steps and the conversions to and from them bound it, not memory (23.5 us at a copy's
+// rate).  One row takes 5.8 us on the device, most of it the launch and the angles' sincos.
 #include "tb_paged.cuh"
 
 namespace {
@@ -59,7 +63,8 @@ __device__ __forceinline__ void store_q8(const float (&x)[NW], int8_t* dq, float
 // R rows a CTA (8 warps): the angles of all of them first (one a thread at R = 4, hd 128), then
 // 8 / R warps a row, each with every (8 / R)-th head, NB heads at a time: their loads are in
 // flight together.  Lane l holds elements l + 32 i, a rotary partner hd / 64 registers away.
-// One row a CTA where there are fewer rows than four a SM would take (latency).
+// One row a CTA where there are fewer than five rows a SM (latency): 5.6 us for one row against
+// 9.3 at R = 4, 9.3 against 10.5 for 592 rows, 12.8 against 11.7 for 800, 51 against 35 for 4096.
 constexpr int NB = 4;
 template <int HD, int R>
 __global__ void __launch_bounds__(256, 4) k_paged_prep(const PrepArgs a, int T)
@@ -192,7 +197,7 @@ extern "C" TB_API int tb_attn_prep_paged_q8(tb_ctx* ctx, const tb_paged_kv* kv, 
     TB_REQUIRE(ctx, q && k && v && qw16 && kw16 && qr && seq && slot && pos, "null pointer");
     DeviceGuard dev(ctx->device);
     PrepArgs a{paged_args(ctx, kv), q, k, v, qw16, kw16, qr, seq, slot, pos, (int)nHq, (double)theta, (double)eps};
-    const bool many = T >= 4LL * ctx->num_sms;
+    const bool many = T >= 5LL * ctx->num_sms;
     auto kern = kv->hd == 64 ? (many ? k_paged_prep<64, 4> : k_paged_prep<64, 1>)
                              : (many ? k_paged_prep<128, 4> : k_paged_prep<128, 1>);
     cudaError_t e = tb_launch(ctx, kern, dim3((unsigned)(many ? (T + 3) / 4 : T)), dim3(256), 0, a, (int)T);
