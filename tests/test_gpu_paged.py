@@ -127,6 +127,22 @@ def test_decode_far_pages(cuda):
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_nan_in_a_query_stays_in_its_head(cuda, hd):
+    c = ref.Cache(51, 2, 20, 16, 2, hd)
+    lens = [300, 9]
+    q = torch.randn(2, 8 * hd, generator=c.g)
+    bad = q.clone()
+    bad.view(2, 8, hd)[1, 5, 3] = float("nan")
+    kv, table = c.dev(), c.table.cuda()
+    hit = torch.zeros(2, 8, dtype=torch.bool)
+    hit[1, 5] = True
+    for run in (lambda x: tb.attention_decode_paged_q8(x.cuda(), kv, table, _ints(lens), 8, 2, hd),
+                lambda x: tb.attention_prefill_paged_q8(x.cuda(), kv, table, _ints([0, 1, 2]), _ints(lens), 8, 2, hd)):
+        a, b = run(q).cpu().view(2, 8, hd), run(bad).cpu().view(2, 8, hd)
+        assert b[hit].isnan().all() and torch.equal(a[~hit], b[~hit])
+
+
 def test_decode_same_bits_every_time(cuda):
     c = ref.Cache(12, 3, 60, 32, 4, 128)
     a = _decode_check(c, [1900, 77, 1000], 16, weights=True)
@@ -304,6 +320,12 @@ def test_prep(cuda, nHq, nKv, hd, page, T):
         Vq.view(-1, w)[r], Vs.view(-1, w // 32)[r] = v8[t], vm[t]
     for have, need in zip(kv, (Kq, Ks, Vq, Vs)):              # rows that no call names stay as they were
         assert torch.equal(have.cpu(), need)
+
+
+@pytest.mark.parametrize("nHq,nKv,hd,page,T", [(6, 2, 128, 128, 803), (5, 3, 64, 64, 1001)])
+def test_prep_many_rows(cuda, nHq, nKv, hd, page, T):
+    """enough rows for four of them a CTA, the last CTA's not all there"""
+    test_prep(cuda, nHq, nKv, hd, page, T)
 
 
 @pytest.mark.parametrize("lens,budget,sinks,recent,page,new_page", [
