@@ -9,7 +9,9 @@
 //
 // 16 sequences of 8192 rows and below to 2048 (8 heads of 128; 146 MB) take 52 us: scores 5,
 // selection 19, copy 27 (5.4 TB/s); one of 131072 rows to 16384 (80 MB) 41: scores 5,
-// selection 25, copy 10.
+// selection 25, copy 10.  Slower: 16 CTAs a sequence (43 us for the long one), the scores
+// formed by the selecting clusters (one launch less, but 52, and 2 us more at 2048 rows),
+// 11-bit digits (61).
 #include "tb_paged.cuh"
 
 namespace {
