@@ -206,8 +206,8 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, 
 // and K to f32 takes 1180.
 // Measured with the join (bytes of the rows seen, their scales and the weights; 6.55 TB/s is
 // what a copy reaches): 131001 rows of 8 heads of 128, 302 MB, 60.8 us (5.0 TB/s: memory, and
-// a start of 6 us); 32 ragged sequences of 8192 rows and below with weights, 329 MB, 76.6 us
-// (4.3 TB/s: three kernels, and the scores pass through memory); 16 windows of 4096 rows of 8
+// a start of 6 us); 32 ragged sequences of 8192 rows and below with weights, 329 MB, 73.7 us
+// (4.5 TB/s: three kernels, and the scores pass through memory); 16 windows of 4096 rows of 8
 // heads of 64, 76 MB, 31 us (2.4 TB/s: a tile of half the bytes has as many steps behind one
 // another, 2100 cycles and 1000 for the next one's copies; 128 registers allow no more warps);
 // one sequence of 4096 rows 11.7 us, a chain of latencies: plan, page number, tile, products,
@@ -674,6 +674,7 @@ __global__ void __launch_bounds__(CT) k_paged_combine(const __grid_constant__ De
 }
 
 // weights[b][h][j] += sum over the group of 2^(s - m) / l, for the keys seen
+constexpr int KEYS = 4;    // a thread
 template <int GRP>
 __global__ void __launch_bounds__(256) k_paged_weights(const __grid_constant__ DecArgs a)
 {
@@ -681,8 +682,22 @@ __global__ void __launch_bounds__(256) k_paged_weights(const __grid_constant__ D
     tb_pdl_trigger();
     const int h = blockIdx.y, b = blockIdx.z, cap = a.kv.cap();
     const int n = a.kv.checked_len(__ldg(a.lens + b));
-    const int j0 = blockIdx.x * 1024;
+    const int j0 = blockIdx.x * 256 * KEYS;
     if (j0 >= n) return;
+    // every load before the first use
+    const long long at = ((long long)b * a.kv.nKv + h) * cap;
+    float sc[KEYS][GRP], old[KEYS];
+    bool see[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) {
+        const int j = j0 + 256 * i + threadIdx.x;
+        see[i] = j < n && key_seen(j, n - 1, a.window, a.sinks);
+        if (!see[i]) continue;
+        const float* src = a.SC + (at + j) * GRP;
+#pragma unroll
+        for (int g = 0; g < GRP; g++) sc[i][g] = __ldcg(src + g);
+        old[i] = a.weights[at + j];
+    }
     float m[GRP], r[GRP];
 #pragma unroll
     for (int g = 0; g < GRP; g++) {
@@ -690,13 +705,13 @@ __global__ void __launch_bounds__(256) k_paged_weights(const __grid_constant__ D
         m[g] = ml.x;
         r[g] = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
     }
-    const long long at = ((long long)b * a.kv.nKv + h) * cap;
-    for (int j = j0 + threadIdx.x; j < min(n, j0 + 1024); j += 256) {
-        if (!key_seen(j, n - 1, a.window, a.sinks)) continue;
+#pragma unroll
+    for (int i = 0; i < KEYS; i++) {
+        if (!see[i]) continue;
         float s = 0.0f;
 #pragma unroll
-        for (int g = 0; g < GRP; g++) s = fmaf(exp2f(a.SC[(at + j) * GRP + g] - m[g]), r[g], s);
-        a.weights[at + j] += s;
+        for (int g = 0; g < GRP; g++) s = fmaf(exp2f(sc[i][g] - m[g]), r[g], s);
+        a.weights[at + j0 + 256 * i + threadIdx.x] = old[i] + s;
     }
 }
 
@@ -747,7 +762,7 @@ int launch_decode(tb_ctx* ctx, const DecArgs& a)
     if (e == cudaSuccess) e = tb_launch(ctx, k_paged_combine<HD, GRP>, dim3(a.kv.nKv, a.kv.batch), dim3(CT), (size_t)a.grid * GRP * sizeof(float2), a);
     if (e == cudaSuccess && a.weights)
         e = tb_launch(ctx, k_paged_weights<GRP>,
-                      dim3(tb_cdiv((long long)a.kv.max_pages << a.kv.log_page, 1024), a.kv.nKv, a.kv.batch), dim3(256), 0, a);
+                      dim3(tb_cdiv((long long)a.kv.max_pages << a.kv.log_page, 256 * KEYS), a.kv.nKv, a.kv.batch), dim3(256), 0, a);
     if (e != cudaSuccess) return tb_fail(ctx, TB_ERR_CUDA, "attn_decode_paged launch: %s", cudaGetErrorString(e));
     return TB_OK;
 }
