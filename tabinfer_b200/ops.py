@@ -645,6 +645,7 @@ def _arg(t, what, dtype, shape, index):
 
 
 _PAGED_KV = struct.Struct("@5P6q").pack     # tb_paged_kv (packed: half the time of a ctypes structure)
+_PAGED_TABLE = struct.Struct("@P6q").pack   # its members behind the pools
 
 
 def _paged(kv, table, nKv, hd, index, what="kv"):
@@ -666,26 +667,17 @@ def _paged(kv, table, nKv, hd, index, what="kv"):
 _ws_sizes = {}
 
 
-def _workspace(c, query, index, s, *sizes):
-    """Workspace of a paged call: a tensor of the current stream's allocator, so calls on other
-    streams and captured graphs have their own.  sizes: what the query takes behind the cache."""
+def _workspace(c, query, index, s, lens, *sizes):
+    """Workspace of a paged call: a tensor of the current stream's allocator (int32, as lens: a
+    new_empty takes less than a torch.empty), so calls on other streams and captured graphs have
+    their own.  sizes: what the query takes behind the cache."""
     key = (query, index, s[40:], sizes)         # the cache's sizes without its addresses
     n = _ws_sizes.get(key)
     if n is None:
         v = ctypes.c_size_t()
         c.check(getattr(LIB, query)(c.h, s, *sizes, ctypes.byref(v)), query)
-        n = _ws_sizes[key] = max(v.value, 256)
-    return torch.empty(n, dtype=torch.uint8, device=_device(index)), n
-
-
-_devices = {}
-
-
-def _device(index):
-    d = _devices.get(index)
-    if d is None:
-        d = _devices[index] = torch.device("cuda", index)
-    return d
+        n = _ws_sizes[key] = max(v.value + 3 & ~3, 256)
+    return lens.new_empty(n >> 2), n
 
 
 def attn_prep_paged_q8(q, k, v, qw16, kw16, kv, table, seq, slot, pos, nHq, nKv, hd, theta, eps, qr=None):
@@ -730,7 +722,7 @@ def attention_decode_paged_q8(qr, kv, table, lens, nHq, nKv, hd, window=0, sinks
     lp = _arg(lens, "lens", torch.int32, (B,), d)
     wp = None if weights is None else _arg(weights, "weights", f32, (B, nKv, most * rows), d)
     c = default_context(d)
-    ws, n = _workspace(c, "tb_attn_decode_paged_ws", d, s, nHq, 0 if wp is None else 1)
+    ws, n = _workspace(c, "tb_attn_decode_paged_ws", d, s, lens, nHq, 0 if wp is None else 1)
     rc = LIB.tb_attn_decode_paged_q8(c.h, s, op, qp, lp, nHq, int(window), int(sinks), wp, ws.data_ptr(), n)
     if rc:
         c.check(rc, "attn_decode_paged_q8")
@@ -753,7 +745,7 @@ def attention_prefill_paged_q8(q, kv, table, cu, lens, nHq, nKv, hd, window=0, s
         op = _arg(out, "out", torch.bfloat16, wide, d)
     cp, lp = _arg(cu, "cu", i32, (B + 1,), d), _arg(lens, "lens", i32, (B,), d)
     c = default_context(d)
-    ws, n = _workspace(c, "tb_attn_prefill_paged_ws", d, s, nHq, T)
+    ws, n = _workspace(c, "tb_attn_prefill_paged_ws", d, s, lens, nHq, T)
     rc = LIB.tb_attn_prefill_paged_q8(c.h, s, op, qp, cp, lp, nHq, T, int(window), int(sinks), ws.data_ptr(), n)
     if rc:
         c.check(rc, "attn_prefill_paged_q8")
@@ -769,19 +761,24 @@ def kv_evict_paged_q8(kv, table, lens, weights, new_table, budget, sinks, recent
     behind the last; lens int32 [batch]; weights f32 [batch, nKv, new rows], zero behind the last)."""
     d = table.get_device()
     s, rows, B, most = _paged(kv, table, nKv, hd, d)
-    t, new_rows, new_B, new_most = _paged(kv if kv_out is None else kv_out, new_table, nKv, hd, d, "kv_out")
-    dev = _device(d)
+    if kv_out is None:                          # the same pools, checked above, under another table
+        if new_table.dim() != 2:
+            raise TabInferError("the table is [batch, max_pages]")
+        n, new_rows, (new_B, new_most) = kv[0].shape[0], rows, new_table.shape
+        t = s[:32] + _PAGED_TABLE(_arg(new_table, "new_table", torch.int32, (new_B, new_most), d), n, rows, new_B,
+                                  new_most, nKv, hd)
+    else:
+        t, new_rows, new_B, new_most = _paged(kv_out, new_table, nKv, hd, d, "kv_out")
     lp = _arg(lens, "lens", torch.int32, (B,), d)
     wp = _arg(weights, "weights", torch.float32, (B, nKv, most * rows), d)
     if new_B != B:
         raise TabInferError("new_table must have %d rows" % B)
     if budget < 0:
         raise TabInferError("budget must not be negative")
-    kept = torch.empty((B, int(budget)), dtype=torch.int32, device=dev)
-    new_lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    new_weights = torch.empty((B, nKv, new_most * new_rows), dtype=torch.float32, device=dev)
+    kept, new_lens = lens.new_empty((B, int(budget))), torch.empty_like(lens)
+    new_weights = weights.new_empty((B, nKv, new_most * new_rows))
     c = default_context(d)
-    ws, n = _workspace(c, "tb_kv_evict_paged_ws", d, s)
+    ws, n = _workspace(c, "tb_kv_evict_paged_ws", d, s, lens)
     c.check(LIB.tb_kv_evict_paged_q8(c.h, s, t, lp, wp, kept.data_ptr(),
                                      new_lens.data_ptr(), new_weights.data_ptr(), int(budget), int(sinks),
                                      int(recent), ws.data_ptr(), n), "kv_evict_paged_q8")
