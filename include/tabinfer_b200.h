@@ -427,8 +427,9 @@ TB_API int tb_attn_decode_q8_batch(tb_ctx *ctx, float *out, const float *qr,
  * sequence's last row are not read, nor those of pages on which no row under the
  * window lies).  An element stands for q / 127 * scale (bytes -127 .. 127 and
  * positive scales, as every writer here leaves them).
- * page_rows 16, 32, 64, 128 or 256; hd 64 or 128; nHq/nKv 1, 2, 4 or 8; n_pages *
- * page_rows < 2^31; pools 16-byte aligned.
+ * page_rows 16, 32, 64, 128 or 256; hd 64 or 128; nHq/nKv 1, 2, 4 or 8 (prep: any
+ * nHq up to 8192); nKv <= 1024; batch <= 65535; n_pages * page_rows < 2^31;
+ * max_pages * page_rows <= 2^30; pools 16-byte aligned.
  * What the host cannot see is checked on the device: a page number outside the
  * pool sets the context's error word (tb_ctx_device_error) to 0x6c01 and its rows
  * are neither read nor written; a length or row that the table cannot hold sets
