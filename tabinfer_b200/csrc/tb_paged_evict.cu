@@ -43,9 +43,10 @@ __device__ __forceinline__ unsigned long long score_key(double s)
     return (u >> 63) ? ~u : u | (1ull << 63);
 }
 
+// not the .aligned form: it follows loops and branches in which a warp's lanes part
 __device__ __forceinline__ void cluster_sync()
 {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;\n barrier.cluster.wait.acquire;" ::: "memory");
 }
 // a word of another CTA's shared memory, at the place of `p` in this one's
 __device__ __forceinline__ unsigned remote(const void* p, int rank)
