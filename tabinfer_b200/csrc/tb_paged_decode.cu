@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(c
         const unsigned ok = __ballot_sync(0xffffffffu, see && row >= 0);
         uint8_t* st = ring + s * L::STAGE;
         if (lane == 0) okw[s] = ok;
+        __syncwarp();          // before the arrival that releases it, which another lane may make
         const bool second = box < KT && row16 >= 0;
         mbar_expect_elect(&full[s], (uint32_t)(2 * HD * box * ((row0 >= 0) + second)));
         if (row0 >= 0) tma_2d_elect(st, &a.mk, st + L::V, &a.mv, ph * HD, row0, &full[s]);

@@ -48,3 +48,33 @@ def test_evict_lanes_with_other_counts(cuda, n):
     w = torch.randn(1, 1, c.cap, generator=c.g).abs()
     _evict(c, [n], w, 900, 3, 7)
     _evict(c, [n], w.round(), 900, 0, 0)
+
+
+@pytest.mark.parametrize("nHq,nKv,hd,page", [(16, 8, 128, 16), (8, 1, 64, 32), (4, 2, 64, 16), (2, 2, 128, 64)])
+def test_decode_masks_of_many_tiles(cuda, nHq, nKv, hd, page):
+    """another set of left-out keys in every tile (pages outside the pool here and there): a tile is
+    read with its own mask"""
+    n = 1500
+    c = ref.Cache(44, 1, -(-n // page), page, nKv, hd)
+    gone = torch.rand(c.table.shape[1], generator=c.g) < 0.4
+    table = c.table.clone()
+    table[0, gone] = -1
+    q = torch.randn(1, nHq * hd, generator=c.g) * 1.5
+    w = torch.zeros(1, nKv, c.cap, device="cuda")
+    got = tb.attention_decode_paged_q8(q.cuda(), c.dev(), table.cuda(), _ints([n]), nHq, nKv, hd, weights=w).cpu()
+    assert tb.default_context(0).device_error() == 0x6c01
+    ok = ~gone.repeat_interleave(page)[:n]
+    grp = nHq // nKv
+    for h in range(nKv):
+        k, v = c.head(0, n, h)
+        total = torch.zeros(n, dtype=torch.float64)
+        for g in range(grp):
+            x = q.double().reshape(nHq, hd)[h * grp + g]
+            p = torch.softmax(k[ok] @ x * hd ** -0.5, 0)
+            total[ok] += p
+            mag = float((k[ok].abs() @ x.abs()).max()) * hd ** -0.5
+            rel = 2 * (hd + 8) * U * mag + (n + 16) * U
+            err = (got.double().reshape(nHq, hd)[h * grp + g] - p @ v[ok]).abs().max()
+            assert float(err) <= rel * float(v[ok].abs().max())
+        assert (w[0, h, :n].cpu()[~ok] == 0).all()
+        assert float((w[0, h, :n].cpu().double() - total).abs().max()) <= grp * rel + 4 * U * float(total.max())
