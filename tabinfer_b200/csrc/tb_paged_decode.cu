@@ -437,8 +437,8 @@ __global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(c
                         scs[hd_ * KT + 16 * mt + g8 + 8] = y;
                     }
                 }
+                __syncwarp();      // the lanes that wrote meet the others before the next ldmatrix
             }
-            __syncwarp();
             float pr[GRP], corr[GRP];
 #pragma unroll
             for (int g = 0; g < GRP; g++) pr[g] = ok ? scs[g * KT + lane] : NEG_BIG;
@@ -489,13 +489,11 @@ __global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(c
                 const float2 cr2 = make_float2(cr, cr);
 #pragma unroll
                 for (int G = 0; G < NG; G++) {
-                    uint32_t b0 = 0, b1 = 0;
-                    if (hb < GRP) {
-                        const uint4 x = *reinterpret_cast<const uint4*>(words + (hb * NG + G) * KT + 4 * t4);
-                        const uint4 y = *reinterpret_cast<const uint4*>(words + (hb * NG + G) * KT + 16 + 4 * t4);
-                        b0 = __byte_perm(__byte_perm(x.x, x.y, sel), __byte_perm(x.z, x.w, sel), 0x5410);
-                        b1 = __byte_perm(__byte_perm(y.x, y.y, sel), __byte_perm(y.z, y.w, sel), 0x5410);
-                    }
+                    // columns of no head (GRP = 1) take a head's digits and are not written: no branch before ldmatrix
+                    const uint32_t* src = words + ((GRP == 1 ? 0 : hb) * NG + G) * KT + 4 * t4;
+                    const uint4 x = *reinterpret_cast<const uint4*>(src), y = *reinterpret_cast<const uint4*>(src + 16);
+                    const uint32_t b0 = __byte_perm(__byte_perm(x.x, x.y, sel), __byte_perm(x.z, x.w, sel), 0x5410);
+                    const uint32_t b1 = __byte_perm(__byte_perm(y.x, y.y, sel), __byte_perm(y.z, y.w, sel), 0x5410);
                     const float so = (2 * nt + 1 < GRP && (t4 >> 1) ? sc[(2 * nt + 1) % GRP][G] : sc[2 * nt][G]) * f2;
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
