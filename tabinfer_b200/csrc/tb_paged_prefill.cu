@@ -578,6 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
                 uint32_t o[32];
+                __syncwarp();                     // rows that are there meet those behind the last one
                 tmem_ld32(to + 32 * c, o);
                 tmem_wait_ld();
                 if (p.slot >= 0) {
@@ -601,6 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     }
                 }
             }
+            __syncwarp();
             tc_before();       // O is read before the p_full that lets the next part's product write it
             p = pn;
             h = hn;

@@ -78,3 +78,33 @@ def test_decode_masks_of_many_tiles(cuda, nHq, nKv, hd, page):
             assert float(err) <= rel * float(v[ok].abs().max())
         assert (w[0, h, :n].cpu()[~ok] == 0).all()
         assert float((w[0, h, :n].cpu().double() - total).abs().max()) <= grp * rel + 4 * U * float(total.max())
+
+
+def _prefill(c, q, ts, lens, nHq, window=0, sinks=0, tail=0):
+    """(outputs f64 [T, nHq, hd], cu) of packed chunks; rows behind the last stay as they were"""
+    cu = [sum(ts[:b]) for b in range(c.B + 1)]
+    out = torch.full((cu[-1] + tail, nHq * c.hd), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = tb.attention_prefill_paged_q8(q.cuda(), c.dev(), c.table.cuda(), _ints(cu), _ints(lens), nHq, c.nKv, c.hd,
+                                        window=window, sinks=sinks, out=out).cpu().double()
+    assert (got[cu[-1]:] == 7).all()
+    return got.reshape(-1, nHq, c.hd), cu
+
+
+def _prefill_rows(c, q, ts, lens, nHq, window=0, sinks=0, tail=0):
+    got, cu = _prefill(c, q, ts, lens, nHq, window, sinks, tail)
+    for b, (n, t) in enumerate(zip(lens, ts)):
+        for i in range(t):
+            o, _, mag, big = ref.attend(c, b, q[cu[b] + i], n - t + i, nHq, window, sinks)
+            tol = big * (2.0 ** -9 * mag + 2.0 ** -9) + 2.0 ** -8 * o.abs()
+            assert ((got[cu[b] + i] - o).abs() <= tol).all(), (b, i)
+
+
+@pytest.mark.parametrize("nHq,nKv,hd", [(2, 2, 128), (6, 3, 64), (4, 1, 128), (8, 1, 64)])
+def test_prefill_rows_that_end_inside_a_warp(cuda, nHq, nKv, hd):
+    """chunks of 1 to 9 and some 33 rows: a warp of rows with and without a query"""
+    ts = [1, 2, 3, 5, 7, 9, 33, 17]
+    lens = [t + 40 * (i % 3) for i, t in enumerate(ts)]
+    c = ref.Cache(45, len(ts), 8, 16, nKv, hd)
+    q = torch.randn(sum(ts) + 3, nHq * hd, generator=c.g) * 1.5
+    _prefill_rows(c, q, ts, lens, nHq, tail=3)
+    _prefill_rows(c, q, ts, lens, nHq, window=20, sinks=2, tail=3)
