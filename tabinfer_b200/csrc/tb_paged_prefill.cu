@@ -44,6 +44,7 @@
 #include <cuda_bf16.h>
 
 #include "tb_paged.cuh"
+#include "tb_rounds.h"
 
 namespace {
 
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 *reinterpret_cast<uint4*>(half + sw128(ri, c0 + 1 - swap)) = swap ? lo4 : hi4;
             }
         };
-        // a barrier of the producers; true when one of them has given up
+        // a barrier of the producers (the walks' tb_rounds.h); true when one of them has given up
         auto sync = [](bool dead) {
             uint32_t any;
             asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n"
@@ -734,7 +735,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         // tile it is stored, it + 1's bytes are loaded, it + 2's scales and it + 3's page numbers requested
         int ring = 0, row = -1, page = 0, line = -1, h0 = 0, h1 = 0, h2 = 0, h3 = 0;
         float ks[4], vs[4];
-        bool more0 = step(page, line, h0), more1 = false, more2 = false, more3 = false, dead = false;
+        bool more0 = step(page, line, h0), more1 = false, more2 = false;
         if (more0) {
             row = finish(page, line);
             load_scales(row, h0, ks, vs);
@@ -752,45 +753,41 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 more2 = step(page, line, h2);
             }
         }
-        for (int it = 0; more0; it++) {
-            const int s = it % KV_STAGES, buf = it % 3, nb = (it + 1) % 3;
-            const uint32_t par = ((it / KV_STAGES) & 1) ^ 1;
+        producer_rounds(
+            more0, more1, more2,
             // rows and scales of the next tile (their buffer was last read two tiles ago)
-            if (more1) publish(nb, row, ks, vs);
-            if (sync(dead)) break;
-            if (more2) {
+            [&](int it) { publish(it % 3, row, ks, vs); }, sync,
+            [&] {
                 row = finish(page, line);
                 load_scales(row, h2, ks, vs);
-                more3 = step(page, line, h3);
-            }
+                return step(page, line, h3);
+            },
+            [&](int it, bool next) {
+                const int s = it % KV_STAGES, buf = it % 3, nb = (it + 1) % 3;
+                const uint32_t par = ((it / KV_STAGES) & 1) ^ 1;
 #pragma unroll
-            for (int x = 0; x < 2 * L::UNITS; x++) {
-                if (x == 0 || x == L::UNITS) {
-                    dead = !wait_warp(x == 0 ? &k_empty[s] : &v_empty[s], par);
-                    if (dead) break;
+                for (int x = 0; x < 2 * L::UNITS; x++) {
+                    if (x == 0 || x == L::UNITS)
+                        if (!wait_warp(x == 0 ? &k_empty[s] : &v_empty[s], par)) return false;
+                    cp_async_wait<L::NU - 1>();                     // the thread's own copies of this unit
+                    store(x, smem + (x < L::UNITS ? L::OFF_K : L::OFF_V) + s * L::TILE, buf, ring);
+                    if (x == L::UNITS - 1 || x == 2 * L::UNITS - 1) {
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(x < L::UNITS ? &k_full[s] : &v_full[s]);
+                    }
+                    // the unit NU on: of this tile or the next
+                    if (x + L::NU < 2 * L::UNITS) load(x + L::NU, buf, h0, ring);
+                    else if (next) load(x + L::NU - 2 * L::UNITS, nb, h1, ring);
+                    cp_async_commit();
+                    ring = ring + 1 == L::NU ? 0 : ring + 1;
                 }
-                cp_async_wait<L::NU - 1>();                         // the thread's own copies of this unit
-                store(x, smem + (x < L::UNITS ? L::OFF_K : L::OFF_V) + s * L::TILE, buf, ring);
-                if (x == L::UNITS - 1 || x == 2 * L::UNITS - 1) {
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(x < L::UNITS ? &k_full[s] : &v_full[s]);
-                }
-                // the unit NU on: of this tile or the next
-                if (x + L::NU < 2 * L::UNITS) load(x + L::NU, buf, h0, ring);
-                else if (more1) load(x + L::NU - 2 * L::UNITS, nb, h1, ring);
-                cp_async_commit();
-                ring = ring + 1 == L::NU ? 0 : ring + 1;
-            }
-            if (dead) continue;                                     // all leave at the next barrier
-            more0 = more1;
-            more1 = more2;
-            more2 = more3;
-            more3 = false;
-            h0 = h1;
-            h1 = h2;
-            h2 = h3;
-        }
+                h0 = h1;
+                h1 = h2;
+                h2 = h3;
+                return true;
+            });
+        cp_async_wait<0>();                                         // no copy in flight past here
     } else {
         // ================================ MMAs ==========================================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
