@@ -231,10 +231,12 @@ struct PrefillLayout {
     static constexpr int OFF_V = OFF_K + KV_STAGES * TILE;
     static constexpr int OFF_ROW = OFF_V + KV_STAGES * TILE;   // int [3][PK] pool rows
     static constexpr int OFF_SC = OFF_ROW + 3 * PK * 4;        // f16 [3][2][PK][4] scales of K and V
-    static constexpr int OFF_BAD = OFF_SC + 3 * 2 * PK * 8;   // uint [8][PK / 32]: keys of pages outside the pool
+    // uint4 [8][2]: of a half's two 32-key groups the keys of pages outside the pool, and marks: bit 16 + G where
+    // some V has no number in its group G; then, where there is a mark, which keys: uint4 [8][PK / 32]
+    static constexpr int OFF_MARK = OFF_SC + 3 * 2 * PK * 8, OFF_NAN = OFF_MARK + 8 * 2 * 16;
     // the producers' raw bytes: units of NC x 16 bytes a thread, thread-private (cp.async), NU in flight
     static constexpr int UNITS = HD / 64, NU = HD == 128 ? 3 : 2;
-    static constexpr int OFF_RAW = OFF_BAD + 8 * PK / 8;
+    static constexpr int OFF_RAW = OFF_NAN + 8 * PK / 32 * 16;
     static constexpr int OFF_BAR = OFF_RAW + NU * NC * 16 * PROD;
     static constexpr int BYTES = 1024 + OFF_BAR + 256;
     static_assert(BYTES <= 227 * 1024, "shared memory");
@@ -428,7 +430,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             if (lane == 0) mbar_arrive(&q_full[t]);
         };
         // the CTA's next part that has rows in this tile
-        const uint2* bad = reinterpret_cast<const uint2*>(smem + L::OFF_BAD);
+        const uint4* mark = reinterpret_cast<const uint4*>(smem + L::OFF_MARK);
+        const uint4* nans = reinterpret_cast<const uint4*>(smem + L::OFF_NAN);
         int tile = 0;                                            // tiles of the CTA so far (the masks' ring)
         auto find = [&](int k, Part& p, int& h) {
             for (;; k++) {
@@ -454,6 +457,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             const int pos = p.p0 + min(qi, p.nq - 1), pmin = max(p.p0, 0), pmax = p.p0 + p.nq - 1;
             const SeenTiles seen(pmin, pmax, a.window, a.sinks, PK);
             float m = -INFINITY, l = 0.0f;
+            uint32_t none = 0;                       // 32-groups of the row's output that have no number
             // tile 1 a little behind tile 0: its warps share their schedulers with tile 0's, and one's exponentials
             // then run under the other's loads, stores and waits
             bool ok = t == 0 || wait_warp(&s_full[2 * t], seq & 1);
@@ -474,17 +478,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     const uint32_t th = ts + 64 * hh;
                     if (!(ok = wait_warp(&s_full[2 * t + hh], seq & 1))) break;
                     tc_after();
-                    const uint2 bw = bad[2 * (tile & 7) + hh];
+                    const uint4 mk = mark[2 * (tile & 7) + hh];
                     const int kh = k0 + 64 * hh;
-                    // a half that some row sees only in part, or with keys on bad pages
+                    // a half that some row sees only in part, or with keys on bad pages or of no number
                     const bool cut = kh + 63 > pmin || (a.window > 0 && kh <= pmax - a.window && kh + 64 > a.sinks) ||
-                                     (bw.x | bw.y);
+                                     (mk.x | mk.y | ((mk.z | mk.w) >> 16));
                     // the half's keys that this row sees, as bits
                     uint32_t see0 = ~0u, see1 = ~0u;
+                    auto told = [&](uint32_t w, uint32_t see, int g) {
+                        if (!(w >> 16)) return;
+                        const uint4 n = nans[4 * (tile & 7) + g];
+                        none |= (n.x & see ? 1u : 0u) | (n.y & see ? 2u : 0u) | (n.z & see ? 4u : 0u) | (n.w & see ? 8u : 0u);
+                    };
                     if (cut) {
                         const int h0 = hi - 64 * hh, l0 = lo - 64 * hh, s0 = sk - 64 * hh;
-                        see0 = below(h0 + 1) & (~below(l0 + 1) | below(s0)) & ~bw.x;
-                        see1 = below(h0 - 31) & (~below(l0 - 31) | below(s0 - 32)) & ~bw.y;
+                        see0 = below(h0 + 1) & (~below(l0 + 1) | below(s0)) & ~mk.x;
+                        see1 = below(h0 - 31) & (~below(l0 - 31) | below(s0 - 32)) & ~mk.y;
+                        told(mk.z, see0, 2 * hh);
+                        told(mk.w, see1, 2 * hh + 1);
                     }
                     auto mask = [&](float* s, uint32_t see) {
 #pragma unroll
@@ -575,9 +586,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             const bool live = qi < p.nq;
             const long long slot = p.slot < 0 ? 0 : (long long)p.slot * nKv + h;
             if (p.slot >= 0) a.PML[slot * ROWS + 128 * t + row] = make_float2(m, l);
-            const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const float rl = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
+                const float r = (none >> c) & 1 ? __int_as_float(0x7fc00000) : rl;
                 uint32_t o[32];
                 __syncwarp();                     // rows that are there meet those behind the last one
                 tmem_ld32(to + 32 * c, o);
@@ -618,7 +630,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         constexpr int NG = HD / 32, CPR = HD / 16, RPU = NC * PROD / CPR;   // 16-byte chunks a row, rows a unit
         // the walk over the tiles of the CTA's parts
         int wk = -1, wj = 0, wt1 = 0, wb = 0, wh = 0, pmin = 0, pmax = 0, published = 0;
-        uint32_t* bads = reinterpret_cast<uint32_t*>(smem + L::OFF_BAD);
+        uint32_t* marks = reinterpret_cast<uint32_t*>(smem + L::OFF_MARK);
+        uint32_t* nans = reinterpret_cast<uint32_t*>(smem + L::OFF_NAN);
         SeenTiles seen(-1, -1, 0, 0, PK);
         // The thread's key of the next tile: its page number (requested here, looked at a tile later) and line;
         // a row that no query of the part sees is line -1 and stays zero.
@@ -676,10 +689,35 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             // its key, on a page outside the pool, is left out by the softmax; of the eight masks the one
             // written here was last read seven tiles ago, four more than the stages hold
             const unsigned miss = __ballot_sync(0xffffffffu, row == -2);
-            if (lane == 0) bads[(published & 7) * 4 + (pt >> 5)] = miss;
+            const int at = (published & 7) * 4 + (pt >> 5), mat = (published & 7) * 8 + (pt >> 6) * 4 + ((pt >> 5) & 1);
             published++;
+            // V without a number (an infinite scale, or NaN) goes in as zero: as it is, it would reach the rows that
+            // do not see the key too, whose weight for it is zero (0 * inf).  The rows that see it are told.
+            // (K's reaches its own column of scores only, and a score that is not seen is masked.)
+            uint32_t mk = 0;
+            float w[4];
+            bool fine = true;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                w[i] = vs[i] * S;                                   // below 65520 it is a number in f16
+                const bool number = fabsf(w[i]) < 65520.0f;
+                if (!number) w[i] = 0.0f;
+                fine = fine && number;
+            }
+            if (!__all_sync(0xffffffffu, fine)) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, !(fabsf(vs[i] * S) < 65520.0f));
+                    if (lane == 0) nans[4 * at + i] = who;
+                    if (who) mk |= 0x10000u << i;
+                }
+            }
+            if (lane == 0) {
+                marks[mat] = miss;
+                marks[mat + 2] = mk;
+            }
             scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * S, ks[1] * S), pack_h2(ks[2] * S, ks[3] * S));
-            scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(vs[0] * S, vs[1] * S), pack_h2(vs[2] * S, vs[3] * S));
+            scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(w[0], w[1]), pack_h2(w[2], w[3]));
         };
         const int ch = pt % CPR, r0 = pt / CPR;                     // chunk of a row; rows r0 + i * PROD / CPR
         uint4* raw = reinterpret_cast<uint4*>(smem + L::OFF_RAW) + pt;

@@ -108,3 +108,35 @@ def test_prefill_rows_that_end_inside_a_warp(cuda, nHq, nKv, hd):
     q = torch.randn(sum(ts) + 3, nHq * hd, generator=c.g) * 1.5
     _prefill_rows(c, q, ts, lens, nHq, tail=3)
     _prefill_rows(c, q, ts, lens, nHq, window=20, sinks=2, tail=3)
+
+
+@pytest.mark.parametrize("hd,nKv,nHq", [(128, 2, 4), (64, 1, 4)])
+@pytest.mark.parametrize("n,ts", [([300], [140]), ([6001, 90], [7, 60])])
+@pytest.mark.parametrize("what", [float("inf"), float("nan")])
+def test_prefill_rows_of_no_number_stay_with_those_who_see_them(cuda, hd, nKv, nHq, n, ts, what):
+    """A scale of infinity or NaN in one 32-group of one key: queries before the key, or whose window has left
+    it, are what they are without it; those that see V's have no number in the group's 32 dimensions alone;
+    those that see K's have none in the heads that read it.  (Whole items, and items in parts.)"""
+    window, sinks, grp, G = 90, 3, nHq // nKv, hd // 32 - 1
+    c = ref.Cache(46, len(n), -(-max(n) // 16) + 1, 16, nKv, hd)
+    q = torch.randn(sum(ts), nHq * hd, generator=c.g) * 1.5
+    for b, w in ((0, 0), (0, window), (len(n) - 1, 0)):
+        j = n[b] - ts[b] // 2 - 1 if w == 0 else n[b] - ts[b] - window // 2
+        r = int(c.rows(b, j))
+        for key in (False, True):
+            pool = (c.Ks if key else c.Vs).view(-1, nKv, hd // 32)
+            was = pool[r, 0, G].clone()
+            pool[r, 0, G] = what
+            got, cu = _prefill(c, q, ts, n, nHq, w, sinks)
+            pool[r, 0, G] = was
+            for s in range(len(n)):
+                for i in range(ts[s]):
+                    pos = n[s] - ts[s] + i
+                    o, _, mag, big = ref.attend(c, s, q[cu[s] + i], pos, nHq, w, sinks)
+                    tol = big * (2.0 ** -9 * mag + 2.0 ** -9) + 2.0 ** -8 * o.abs()
+                    hit = torch.zeros(nHq, hd, dtype=torch.bool)
+                    if s == b and bool(ref.seen(n[s], pos, w, sinks)[j]):
+                        hit[:grp, slice(None) if key else slice(32 * G, 32 * G + 32)] = True
+                    x = got[cu[s] + i]
+                    assert not x[hit].isfinite().any(), (s, i)
+                    assert ((x - o).abs() <= tol)[~hit].all(), (s, i)
