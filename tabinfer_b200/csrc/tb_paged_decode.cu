@@ -442,6 +442,18 @@ __global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(c
             float pr[GRP], corr[GRP];
 #pragma unroll
             for (int g = 0; g < GRP; g++) pr[g] = ok ? scs[g * KT + lane] : NEG_BIG;
+            {   // a K scale without a number: inf times a group's exact sum has a sign that inf times its elements,
+                // one by one, has not (a score of -inf would leave the key out)
+                float z = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NG; i += 2) {
+                    const float2 x = *reinterpret_cast<const float2*>(ks + lane * NG + i);
+                    z = fmaf(x.x, 0.0f, fmaf(x.y, 0.0f, z));
+                }
+                if (ok && z != 0.0f)
+#pragma unroll
+                    for (int g = 0; g < GRP; g++) pr[g] = z;
+            }
             __syncwarp();
             if (a.SC) {
                 const int key = c.seen.tile(c.i) * KT + lane;

@@ -140,3 +140,26 @@ def test_prefill_rows_of_no_number_stay_with_those_who_see_them(cuda, hd, nKv, n
                     x = got[cu[s] + i]
                     assert not x[hit].isfinite().any(), (s, i)
                     assert ((x - o).abs() <= tol)[~hit].all(), (s, i)
+
+
+def test_decode_rows_of_no_number(cuda):
+    """the same of a new token: V's group alone, K's heads alone, and no trace of a row that is not seen"""
+    nKv, hd, nHq, n = 2, 128, 4, 400
+    c = ref.Cache(47, 1, 26, 16, nKv, hd)
+    q = torch.randn(1, nHq * hd, generator=c.g) * 1.5
+    o, _, mag, big = ref.attend(c, 0, q[0], n - 1, nHq, 200, 2)
+    rel = 2 * (hd + 8) * U * mag + (n + 16) * U
+    for j in (100, 300):
+        r = int(c.rows(0, j))
+        for key in (False, True):
+            pool = (c.Ks if key else c.Vs).view(-1, nKv, hd // 32)
+            was = pool[r, 0, 2].clone()
+            pool[r, 0, 2] = float("inf")
+            x = tb.attention_decode_paged_q8(q.cuda(), c.dev(), c.table.cuda(), _ints([n]), nHq, nKv, hd, window=200,
+                                             sinks=2).cpu().double().reshape(nHq, hd)
+            pool[r, 0, 2] = was
+            hit = torch.zeros(nHq, hd, dtype=torch.bool)
+            if j >= n - 200:
+                hit[:2, slice(None) if key else slice(64, 96)] = True
+            assert not x[hit].isfinite().any()
+            assert float((x - o).abs()[~hit].max()) <= rel * big
