@@ -42,6 +42,7 @@
 // Every wait is bounded: one that gives up sets the error word and the CTA's abort flag, all
 // roles leave, the MMA thread waits for its last commit and TMEM is freed.
 #include <cuda_bf16.h>
+#include <type_traits>
 
 #include "tb_paged.cuh"
 #include "tb_rounds.h"
@@ -59,6 +60,7 @@ constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps the
 // with 900 and 1200; three 2001-row chunks under a window 154, 149, 147, 149)
 constexpr int STAGGER = 900;
 constexpr float TOO_LARGE = 32768.0f;    // sum of a half's exponentials that raises the reference maximum
+constexpr float FAR = 1048576.0f;        // scores (log2) whose last bit, 2^-4, is felt in a weight
 
 struct Part {
     int b, row0, nq, p0;                 // sequence, first packed row, queries, row of the first in the sequence
@@ -470,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 // other half's softmax, so scores are there when a thread comes for them.
                 // One pass over a half's scores against the reference maximum as it stands: no maximum is
                 // formed.  Where the sum tells that a score has passed it by 2^9 or more, the maximum is
-                // taken, O rescaled (every column, once the last product is in) and the pass repeated.  A
+                // taken, O rescaled (every column, once the last product is in) and the pass repeated, once.  A
                 // row's first reference is the maximum of the first half in which it sees a key.
 #pragma unroll 1
                 for (int hh = 0; hh < 2; hh++) {
@@ -522,7 +524,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     }
                     uint32_t pk[32];
                     float sum;
-                    for (;;) {
+                    // The argument is x scale - m, of the product as it is (exact) or rounded as m was.  For the largest x the
+                    // first is up to half an ulp of m from 0, which is nothing below FAR and past 2^24 any size, up or down;
+                    // the second is 0 at most, and 0 for the largest x.
+                    auto pass = [&](auto exact) {
                         const float off = m == -INFINITY ? 0.0f : -m;
                         float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                         float x[64];                      // all of the half at once: one wait, and the exponentials
@@ -535,23 +540,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                         }
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
-                            const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2),
-                                                   make_float2(off, off));
+                            float2 y;
+                            if (exact) y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2), make_float2(off, off));
+                            else y = make_float2(__fadd_rn(__fmul_rn(x[2 * i], a.sl2), off), __fadd_rn(__fmul_rn(x[2 * i + 1], a.sl2), off));
                             const float2 e = make_float2(ex2(y.x), ex2(y.y));
                             s2[i & 1] = fadd2(s2[i & 1], e);
                             pk[i] = pack_h2(e.x, e.y);
                         }
                         s2[0] = fadd2(s2[0], s2[1]);
                         sum = s2[0].x + s2[0].y;
-                        // below it every weight fits f16; past it some score is 2^9 above the reference
-                        const bool up = sum >= TOO_LARGE;
-                        if (!__any_sync(0xffffffffu, up)) break;
-                        const float top = largest(), mx = up ? fmaxf(m, top) : m;
+                    };
+                    pass(std::true_type());
+                    // below it every weight fits f16; past it some score is 2^9 above the reference
+                    if (__any_sync(0xffffffffu, sum >= TOO_LARGE || (fabsf(m) > FAR && m != -INFINITY))) {
+                        const float mx = fmaxf(m, largest());
                         if (!fresh) {
                             // the half before: the last tile's second, or this tile's first
                             if (!(ok = wait_warp(&o_done[2 * t + (hh ^ 1)], (hh ? seq : seq - 1) & 1))) break;
                             tc_after();
-                            const float f = up ? ex2(m - mx) : 1.0f;
+                            const float f = mx > m ? ex2(m - mx) : 1.0f;
 #pragma unroll
                             for (int c = 0; c < HD / 32; c++) {
                                 uint32_t o[32];
@@ -564,8 +571,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                             l *= f;
                         }
                         m = mx;
+                        pass(std::false_type());          // once: every weight of every row is 1 at most now
                     }
-                    if (!ok) break;
                     tmem_st32(th, pk);                    // over scores that are read
                     l += sum;
                     tmem_wait_st();

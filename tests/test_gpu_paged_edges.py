@@ -163,3 +163,28 @@ def test_decode_rows_of_no_number(cuda):
                 hit[:2, slice(None) if key else slice(64, 96)] = True
             assert not x[hit].isfinite().any()
             assert float((x - o).abs()[~hit].max()) <= rel * big
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bits", [0, 6, 10, 14, 15])
+def test_prefill_scores_of_any_size(cuda, hd, bits):
+    """Scores up to some 2^28, where the last bit of a score is larger than 1: the keys with the largest score
+    share the weight.  Products and sums are exact: q = +-2^bits in one element of a head, K = byte / 128 *
+    2^bits in it, with bytes 10 apart; V's bytes are exact in f16.  (Tolerance as in the test of rising scores:
+    P's and a part's 2^-11 each, f32, the output's bf16.)"""
+    n, t, nKv, nHq = 700, 130, 1, 2
+    c = ref.Cache(56, 1, 45, 16, nKv, hd)
+    c.Kq[:] = 0
+    c.Ks[:] = 127.0 / 128 * 2.0 ** bits
+    c.Vs[:] = 127.0 / 64
+    rows = c.rows(0, torch.arange(n))
+    place = torch.randperm(n, generator=c.g)
+    q = torch.zeros(t, nHq, hd)
+    q[:, 0, 0], q[:, 1, 0] = 2.0 ** bits, -2.0 ** bits
+    order = torch.randint(-11, 11, (n,), generator=c.g)
+    order[place[:2]] = torch.tensor([12, -12])                      # the largest for either head
+    c.Kq.view(-1, hd)[rows, 0] = (order * 10).to(torch.int8)
+    got, _ = _prefill(c, q.reshape(t, -1), [t], [n], nHq)
+    for i in list(range(0, t, 9)) + [t - 1]:
+        o, _, _, big = ref.attend(c, 0, q[i].reshape(-1), n - t + i, nHq)
+        assert ((got[i] - o).abs() <= 2.0 ** -8 * o.abs() + big * (2.0 ** -10 + 2.0 ** -14)).all(), (bits, i)
