@@ -23,8 +23,12 @@
 //   warp 12          TMEM and the MMAs: S_t = Q_t K^T (both K-major), O_t += P_t V (P from
 //                    TMEM, V MN-major as it lies in the cache), row tile 0 and 1 in turn so
 //                    that one's softmax runs under the other's MMAs
-// Roundings: Q, dequantized K and V (and their scales) and P to f16, relative 2^-11 each; S,
-// the statistics and O in f32 (parts' outputs pass through memory as f16).
+// Roundings: Q, dequantized K and V (and their scales) and P to f16, relative 2^-11 each, and
+// parts' outputs on their way through memory; S, the statistics and O in f32.  Q's rows, K and V
+// of 32 keys, O and a part's outputs carry powers of two of their own (below), so this holds for
+// numbers of any size: an element of K or V loses digits below 2^-25 of the largest one of its
+// head in the same 32 rows (2^-36 of that one at most), one of Q below 2^-12 of its row's
+// largest (2^-23).
 //
 // What bounds it.  Its operations at the bf16 rate a library product reaches (1679 TFLOP/s)
 // would take 164 us at 8192 rows (16 / 8 heads of 128); it takes 314 (876 TFLOP/s), 2048 rows
@@ -59,6 +63,13 @@ constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps the
 // cycles by which row tile 1's softmax starts a part behind tile 0's (8192 rows 321 us with none, 318 with 300, 314
 // with 900 and 1200; three 2001-row chunks under a window 154, 149, 147, 149)
 constexpr int STAGGER = 900;
+// Powers of two.  f16 holds 30 binades, so Q's rows and the K and V of 32 keys are brought to its upper end first:
+// x = x' 2^(e - TOP), the largest |x'| of K and of V in [2^11, 2^15), e a multiple of 4, so that a group's powers are
+// mostly the last one's.  K's and Q's powers go into the factor of the scores; a weight is multiplied by V's power over
+// O's unit, the largest V's of the row so far, by an addition to the exponential's argument.
+// The smallest e, a zero's too, leaves the factor of the scores a normal number: a score masked with -inf stays it.
+constexpr int BIAS = 128, TOP = 15, E_MIN = -40;
+constexpr int Q_E = 11, Q_MIN = -6;       // q whose rows' largest lie between 2^Q_MIN and 2^Q_E share e = Q_E
 constexpr float TOO_LARGE = 32768.0f;    // sum of a half's exponentials that raises the reference maximum
 constexpr float FAR = 1048576.0f;        // scores (log2) whose last bit, 2^-4, is felt in a weight
 
@@ -81,10 +92,12 @@ struct PrefillArgs {
     int* head;              // parts, items
     Part* parts;
     Item* items;
-    // [slot][nKv][HD / 2][ROWS]: O / l as pairs of f16 (the operands' own rounding, half the bytes); a thread
-    // holds a row, so a warp writes 128 contiguous bytes
+    // [slot][nKv][HD / 2][ROWS]: O / l as pairs of f16 (the operands' own rounding, half the bytes: as f32, 2048 rows
+    // took 59 us instead of 53); a thread holds a row, so a warp writes 128 contiguous bytes
     uint32_t* PO;
-    float2* PML;            // [slot][nKv][ROWS]
+    // [slot][nKv][ROWS] m and l, whose last 8 bits hold the unit of the part's outputs (a part's weight is then off by
+    // 2^-16, far below the operands' 2^-11)
+    float2* PML;
     int T, nHq, grp, window, sinks, sms;
     int max_items, max_parts, max_slots;   // what the workspace holds
     float sl2;              // log2(e) / sqrt(HD)
@@ -233,8 +246,9 @@ struct PrefillLayout {
     static constexpr int OFF_V = OFF_K + KV_STAGES * TILE;
     static constexpr int OFF_ROW = OFF_V + KV_STAGES * TILE;   // int [3][PK] pool rows
     static constexpr int OFF_SC = OFF_ROW + 3 * PK * 4;        // f16 [3][2][PK][4] scales of K and V
-    // uint4 [8][2]: of a half's two 32-key groups the keys of pages outside the pool, and marks: bit 16 + G where
-    // some V has no number in its group G; then, where there is a mark, which keys: uint4 [8][PK / 32]
+    // uint4 [8][2]: of a half's two 32-key groups the keys of pages outside the pool, and marks: K's power of two in
+    // byte 0, V's in byte 1 (both + BIAS; 0: no V but zero), bit 16 + G where some V has no number in its 32 dims G;
+    // then, where there is such a bit, which keys: uint4 [8][PK / 32]
     static constexpr int OFF_MARK = OFF_SC + 3 * 2 * PK * 8, OFF_NAN = OFF_MARK + 8 * 2 * 16;
     // the producers' raw bytes: units of NC x 16 bytes a thread, thread-private (cp.async), NU in flight
     static constexpr int UNITS = HD / 64, NU = HD == 128 ? 3 : 2;
@@ -338,6 +352,10 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
+// 2^e, -126 <= e <= 127
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// e with 2^(e-1) <= |x| < 2^e for the bits of |x|, at least E_MIN
+__device__ __forceinline__ int size_of(uint32_t bits) { return max(E_MIN, (int)(bits >> 23) - 126); }
 // bits 0 .. n - 1 (n clamped to 0 .. 32)
 __device__ __forceinline__ uint32_t below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
 
@@ -415,21 +433,62 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         const uint32_t ts = tmem + ((uint32_t)(32 * wq) << 16) + 128 * t;
         const uint32_t to = tmem + ((uint32_t)(32 * wq) << 16) + 256 + HD * t;
         uint8_t* qs = smem + L::OFF_Q + t * L::TILE;
-        // Q rows of this warp: row r of the item = query r / GRP, head r % GRP
+        // Q rows of this warp: row r of the item = query r / GRP, head r % GRP.  Returns the factor of the scores that
+        // belongs to the row of this lane.  As a rule a row goes in as 2^(TOP - Q_E) times itself; where that is too large
+        // for f16 in one, or one has no element of 2^Q_MIN, the warp's rows go in again, each by its own power of two.
         auto load_q = [&](const Part& p, int h) {
             constexpr int C4 = HD / 4;                          // float4 columns a row
-#pragma unroll 16
-            for (int i = lane; i < 32 * C4; i += 32) {
-                const int r = 32 * wq + i / C4, c = i % C4, ir = 128 * t + r, qi = ir / GRP;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (qi < p.nq)
-                    v = __ldg(reinterpret_cast<const float4*>(a.q + ((long long)(p.row0 + qi) * a.nHq + h * GRP + ir % GRP) * HD) + c);
+            auto load = [&](int i) {
+                const int ir = 128 * t + 32 * wq + i / C4, qi = ir / GRP;
+                return qi < p.nq ? __ldg(reinterpret_cast<const float4*>(a.q + ((long long)(p.row0 + qi) * a.nHq + h * GRP + ir % GRP) * HD) + i % C4)
+                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            };
+            auto store = [&](int i, float4 v, float f) {
+                const int r = 32 * wq + i / C4, c = i % C4;
                 *reinterpret_cast<uint2*>(qs + (c >> 4) * L::HALF + sw128(r, (c & 15) >> 1) + (c & 1) * 8) =
-                    make_uint2(pack_h2(v.x, v.y), pack_h2(v.z, v.w));
+                    make_uint2(pack_h2(v.x * f, v.y * f), pack_h2(v.z * f, v.w * f));
+            };
+            auto large = [](float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); };
+            int e = Q_E;
+            constexpr int NL = 16;                              // loads in flight
+            const int rows = p.nq * GRP - 128 * t - 32 * wq;    // the warp's rows that are there, and those behind them
+            float most = 0.0f;
+            bool fine = true;
+#pragma unroll 1
+            for (int i0 = lane; i0 < 32 * C4; i0 += 32 * NL) {
+                float4 v[NL];
+#pragma unroll
+                for (int i = 0; i < NL; i++) v[i] = load(i0 + 32 * i);
+                uint32_t has = 0;                               // bit i: load i has an element of 2^Q_MIN or more
+#pragma unroll
+                for (int i = 0; i < NL; i++) {
+                    const float x = large(v[i]);
+                    most = fmaxf(most, x);
+                    if (x >= pow2(Q_MIN)) has |= 1u << i;
+                    store(i0 + 32 * i, v[i], pow2(TOP - Q_E));
+                }
+                // of the row of load i; of the rows 2 i (bit i) and 2 i + 1 (bit 16 + i)
+                has = __reduce_or_sync(0xffffffffu, C4 < 32 && lane >= 16 ? has << 16 : has);
+                const uint32_t all = C4 == 32 ? below(min(16, rows - i0 / C4)) : below(min(16, (rows + 1) / 2)) | below(min(16, rows / 2)) << 16;
+                fine = fine && (has & all) == all;
+            }
+            if (!__all_sync(0xffffffffu, fine && most < pow2(Q_E))) {
+#pragma unroll 1
+                for (int i = lane; i < 32 * C4; i += 32) {
+                    const float4 v = load(i);
+                    float x = large(v);
+#pragma unroll
+                    for (int o = C4 / 2; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    const int er = min(127, size_of(__float_as_uint(x)));        // of the row that this lane loads
+                    const int mine = __shfl_sync(0xffffffffu, er, C4 == 32 ? 0 : (lane & 1) * 16);
+                    if ((C4 == 32 ? lane : lane >> 1) == i / 32) e = mine;
+                    store(i, v, pow2(TOP - er));
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[t]);
+            return a.sl2 * pow2(e - TOP);
         };
         // the CTA's next part that has rows in this tile
         const uint4* mark = reinterpret_cast<const uint4*>(smem + L::OFF_MARK);
@@ -453,12 +512,18 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
         };
         Part p;
         int h = 0, k = find(0, p, h), seq = 0;                   // seq: tiles of this row tile so far
-        if (k >= 0) load_q(p, h);
+        float sl = 0.0f;                                         // log2 of a weight a unit of S, before K's power
+        if (k >= 0) sl = load_q(p, h);
         while (k >= 0) {
             const int qi = (128 * t + row) / GRP;
             const int pos = p.p0 + min(qi, p.nq - 1), pmin = max(p.p0, 0), pmax = p.p0 + p.nq - 1;
             const SeenTiles seen(pmin, pmax, a.window, a.sinks, PK);
             float m = -INFINITY, l = 0.0f;
+            int unit = 0;                            // O's power of two + BIAS; 0: O is zero
+            // the last half's marks (none is 0), its groups' factors of the scores, and how many binades d their V lies
+            // below the unit, and b = 2^d
+            uint32_t last0 = 0, last1 = 0;
+            float sc0 = 0.0f, sc1 = 0.0f, d0 = 0.0f, d1 = 0.0f, b0 = 1.0f, b1 = 1.0f;
             uint32_t none = 0;                       // 32-groups of the row's output that have no number
             // tile 1 a little behind tile 0: its warps share their schedulers with tile 0's, and one's exponentials
             // then run under the other's loads, stores and waits
@@ -482,22 +547,42 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     tc_after();
                     const uint4 mk = mark[2 * (tile & 7) + hh];
                     const int kh = k0 + 64 * hh;
-                    // a half that some row sees only in part, or with keys on bad pages or of no number
-                    const bool cut = kh + 63 > pmin || (a.window > 0 && kh <= pmax - a.window && kh + 64 > a.sinks) ||
-                                     (mk.x | mk.y | ((mk.z | mk.w) >> 16));
+                    // a half that some row sees only in part, or with keys on bad pages
+                    const bool part = kh + 63 > pmin || (a.window > 0 && kh <= pmax - a.window && kh + 64 > a.sinks) ||
+                                      (mk.x | mk.y);
+                    // or with other marks than the last half's
+                    const bool cut = part || mk.z != last0 || mk.w != last1;
                     // the half's keys that this row sees, as bits
                     uint32_t see0 = ~0u, see1 = ~0u;
-                    auto told = [&](uint32_t w, uint32_t see, int g) {
-                        if (!(w >> 16)) return;
-                        const uint4 n = nans[4 * (tile & 7) + g];
-                        none |= (n.x & see ? 1u : 0u) | (n.y & see ? 2u : 0u) | (n.z & see ? 4u : 0u) | (n.w & see ? 8u : 0u);
-                    };
+                    float lower = 1.0f;                   // what a larger unit makes of O
                     if (cut) {
                         const int h0 = hi - 64 * hh, l0 = lo - 64 * hh, s0 = sk - 64 * hh;
                         see0 = below(h0 + 1) & (~below(l0 + 1) | below(s0)) & ~mk.x;
                         see1 = below(h0 - 31) & (~below(l0 - 31) | below(s0 - 32)) & ~mk.y;
+                        auto told = [&](uint32_t w, uint32_t see, int g) {
+                            if (!(w >> 16)) return;
+                            const uint4 n = nans[4 * (tile & 7) + g];
+                            none |= (n.x & see ? 1u : 0u) | (n.y & see ? 2u : 0u) | (n.z & see ? 4u : 0u) | (n.w & see ? 8u : 0u);
+                        };
                         told(mk.z, see0, 2 * hh);
                         told(mk.w, see1, 2 * hh + 1);
+                        // (marks with a key of no number are looked at in every half; a half seen in part may leave the
+                        // row's unit below its V's, so the next one looks again)
+                        last0 = part || (mk.z >> 16) ? 0u : mk.z;
+                        last1 = part || (mk.w >> 16) ? 0u : mk.w;
+                        sc0 = fminf(3.0e38f, sl * pow2((int)(mk.z & 255) - BIAS));
+                        sc1 = fminf(3.0e38f, sl * pow2((int)(mk.w & 255) - BIAS));
+                        // O's unit: the largest power of a V that the row sees
+                        const int v0 = mk.z >> 8 & 255, v1 = mk.w >> 8 & 255, top = max(unit, max(see0 ? v0 : 0, see1 ? v1 : 0));
+                        if (top > unit && unit > 0) lower = pow2(max(-126, unit - top));
+                        unit = top;
+                        // binades of a group's V below it; from 64 on its weights are zero in f16 whatever they are (the
+                        // sums keep them in f32)
+                        const int e0 = v0 ? max(0, min(64, unit - v0)) : 0, e1 = v1 ? max(0, min(64, unit - v1)) : 0;
+                        d0 = (float)e0;
+                        d1 = (float)e1;
+                        b0 = pow2(e0);
+                        b1 = pow2(e1);
                     }
                     auto mask = [&](float* s, uint32_t see) {
 #pragma unroll
@@ -514,21 +599,21 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                             tmem_wait_ld();
                             if (cut) mask(s, c ? see1 : see0);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) t4[i & 3] = fmaxf(t4[i & 3], s[i]);
+                            for (int i = 0; i < 32; i++) t4[2 * c + (i & 1)] = fmaxf(t4[2 * c + (i & 1)], s[i]);
                         }
-                        return fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * a.sl2;
+                        return fmaxf(fmaxf(t4[0], t4[1]) * sc0, fmaxf(t4[2], t4[3]) * sc1);
                     };
                     if (__any_sync(0xffffffffu, m == -INFINITY)) {          // rows that have seen no key yet
                         const float mx = largest();
                         if (m == -INFINITY) m = mx;                         // O is zero, or not written
                     }
                     uint32_t pk[32];
-                    float sum;
+                    float2 sum;                           // of either group
                     // The argument is x scale - m, of the product as it is (exact) or rounded as m was.  For the largest x the
                     // first is up to half an ulp of m from 0, which is nothing below FAR and past 2^24 any size, up or down;
                     // the second is 0 at most, and 0 for the largest x.
                     auto pass = [&](auto exact) {
-                        const float off = m == -INFINITY ? 0.0f : -m;
+                        const float off = m == -INFINITY ? 0.0f : -m, off0 = off - d0, off1 = off - d1;
                         float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                         float x[64];                      // all of the half at once: one wait, and the exponentials
                         tmem_ld32(th, reinterpret_cast<uint32_t*>(x));       // back to back (16 at a time took twice as long)
@@ -540,19 +625,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                         }
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
+                            const float sc = i < 16 ? sc0 : sc1, of = i < 16 ? off0 : off1, d = i < 16 ? d0 : d1;
                             float2 y;
-                            if (exact) y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(a.sl2, a.sl2), make_float2(off, off));
-                            else y = make_float2(__fadd_rn(__fmul_rn(x[2 * i], a.sl2), off), __fadd_rn(__fmul_rn(x[2 * i + 1], a.sl2), off));
+                            if (exact) y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sc, sc), make_float2(of, of));
+                            else {                        // (the rounded product less m first: 0 for the largest)
+                                y.x = __fadd_rn(__fadd_rn(__fmul_rn(x[2 * i], sc), off), -d);
+                                y.y = __fadd_rn(__fadd_rn(__fmul_rn(x[2 * i + 1], sc), off), -d);
+                            }
                             const float2 e = make_float2(ex2(y.x), ex2(y.y));
-                            s2[i & 1] = fadd2(s2[i & 1], e);
+                            s2[i >> 4] = fadd2(s2[i >> 4], e);
                             pk[i] = pack_h2(e.x, e.y);
                         }
-                        s2[0] = fadd2(s2[0], s2[1]);
-                        sum = s2[0].x + s2[0].y;
+                        sum = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
                     };
                     pass(std::true_type());
                     // below it every weight fits f16; past it some score is 2^9 above the reference
-                    if (__any_sync(0xffffffffu, sum >= TOO_LARGE || (fabsf(m) > FAR && m != -INFINITY))) {
+                    if (__any_sync(0xffffffffu, sum.x + sum.y >= TOO_LARGE || lower < 1.0f || (fabsf(m) > FAR && m != -INFINITY))) {
                         const float mx = fmaxf(m, largest());
                         if (!fresh) {
                             // the half before: the last tile's second, or this tile's first
@@ -565,7 +653,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                                 tmem_ld32(to + 32 * c, o);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * (f * lower));
                                 tmem_st32(to + 32 * c, o);
                             }
                             l *= f;
@@ -574,7 +662,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                         pass(std::false_type());          // once: every weight of every row is 1 at most now
                     }
                     tmem_st32(th, pk);                    // over scores that are read
-                    l += sum;
+                    l = fmaf(sum.x, b0, fmaf(sum.y, b1, l));
                     tmem_wait_st();
                     tc_before();
                     __syncwarp();
@@ -587,13 +675,16 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             Part pn;
             int hn = 0;
             const int kn = find(k + 1, pn, hn);
-            if (kn >= 0) load_q(pn, hn);
+            float sn = 0.0f;
+            if (kn >= 0) sn = load_q(pn, hn);
             if (!wait_warp(&o_done[2 * t + 1], (seq - 1) & 1)) break;
             tc_after();
             const bool live = qi < p.nq;
             const long long slot = p.slot < 0 ? 0 : (long long)p.slot * nKv + h;
-            if (p.slot >= 0) a.PML[slot * ROWS + 128 * t + row] = make_float2(m, l);
-            const float rl = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            if (p.slot >= 0)
+                a.PML[slot * ROWS + 128 * t + row] = make_float2(m, __int_as_float((__float_as_int(l) & ~255) | unit));
+            // (a part's outputs stay in the row's unit, so that they fit f16)
+            const float rl = (l > 0.0f || l != l ? 1.0f / l : 0.0f) * (p.slot < 0 && unit ? pow2(unit - BIAS) : 1.0f);
 #pragma unroll
             for (int c = 0; c < HD / 32; c++) {
                 const float r = (none >> c) & 1 ? __int_as_float(0x7fc00000) : rl;
@@ -627,6 +718,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             p = pn;
             h = hn;
             k = kn;
+            sl = sn;
         }
     } else if (warp < W_MMA) {
         // ============================ K / V tiles ======================================
@@ -689,42 +781,57 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 }
             }
         };
-        auto publish = [&](int buf, int row, const float (&ks)[4], const float (&vs)[4]) {
+        // of the next tile to be published: the mark and the factors of the scales
+        uint32_t mk = 0;
+        float fk = 0.0f, fv = 0.0f;
+        auto measure = [&](const float (&ks)[4], float (&vs)[4]) {
             constexpr float S = 128.0f / 127.0f;                    // bytes become q / 128
+            // the warp's 32 keys: K's and V's powers of two from their largest scales (the bits of a scale that is not a
+            // number are above those of every number)
+            constexpr uint32_t INF = 0x7f800000u;
+            auto bits = [](float x) { return __float_as_uint(fabsf(x)); };
+            auto large = [&](const float (&x)[4]) {
+                return max(max(bits(x[0]), bits(x[1])), max(bits(x[2]), bits(x[3])));
+            };
+            mk = 0;
+            uint32_t kb = __reduce_max_sync(0xffffffffu, large(ks)), vb = __reduce_max_sync(0xffffffffu, large(vs));
+            if (kb >= INF || vb >= INF) {
+                // V without a number (an infinite scale, or NaN) goes in as zero: as it is, it would reach the rows that
+                // do not see the key too, whose weight for it is zero (0 * inf).  The rows that see it are told.
+                // (K's reaches its own column of scores only, and a score that is not seen is masked.)
+                kb = vb = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, bits(vs[i]) >= INF);
+                    if (lane == 0) nans[4 * (4 * (published & 7) + (pt >> 5)) + i] = who;
+                    if (who) mk |= 0x10000u << i;
+                    if (bits(vs[i]) >= INF) vs[i] = 0.0f;
+                    kb = max(kb, bits(ks[i]) < INF ? bits(ks[i]) : 0u);
+                    vb = max(vb, bits(vs[i]));
+                }
+                kb = __reduce_max_sync(0xffffffffu, kb);
+                vb = __reduce_max_sync(0xffffffffu, vb);
+            }
+            const int ke = (size_of(kb) + 3) & ~3, ve = (size_of(vb) + 3) & ~3;
+            mk |= (uint32_t)(ke - TOP + BIAS) | (vb ? (uint32_t)(ve - TOP + BIAS) << 8 : 0u);
+            fk = S * pow2(TOP - ke);
+            fv = S * pow2(TOP - ve);
+        };
+        auto publish = [&](int buf, int row, const float (&ks)[4], float (&vs)[4]) {
+            measure(ks, vs);
             // a row that is not there: any bytes, of scale zero
             rows[buf * PK + pt] = max(row, 0);
             // its key, on a page outside the pool, is left out by the softmax; of the eight masks the one
             // written here was last read seven tiles ago, four more than the stages hold
             const unsigned miss = __ballot_sync(0xffffffffu, row == -2);
-            const int at = (published & 7) * 4 + (pt >> 5), mat = (published & 7) * 8 + (pt >> 6) * 4 + ((pt >> 5) & 1);
+            const int mat = (published & 7) * 8 + (pt >> 6) * 4 + ((pt >> 5) & 1);
             published++;
-            // V without a number (an infinite scale, or NaN) goes in as zero: as it is, it would reach the rows that
-            // do not see the key too, whose weight for it is zero (0 * inf).  The rows that see it are told.
-            // (K's reaches its own column of scores only, and a score that is not seen is masked.)
-            uint32_t mk = 0;
-            float w[4];
-            bool fine = true;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                w[i] = vs[i] * S;                                   // below 65520 it is a number in f16
-                const bool number = fabsf(w[i]) < 65520.0f;
-                if (!number) w[i] = 0.0f;
-                fine = fine && number;
-            }
-            if (!__all_sync(0xffffffffu, fine)) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t who = __ballot_sync(0xffffffffu, !(fabsf(vs[i] * S) < 65520.0f));
-                    if (lane == 0) nans[4 * at + i] = who;
-                    if (who) mk |= 0x10000u << i;
-                }
-            }
             if (lane == 0) {
                 marks[mat] = miss;
                 marks[mat + 2] = mk;
             }
-            scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * S, ks[1] * S), pack_h2(ks[2] * S, ks[3] * S));
-            scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(w[0], w[1]), pack_h2(w[2], w[3]));
+            scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * fk, ks[1] * fk), pack_h2(ks[2] * fk, ks[3] * fk));
+            scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(vs[0] * fv, vs[1] * fv), pack_h2(vs[2] * fv, vs[3] * fv));
         };
         const int ch = pt % CPR, r0 = pt / CPR;                     // chunk of a row; rows r0 + i * PROD / CPR
         uint4* raw = reinterpret_cast<uint4*>(smem + L::OFF_RAW) + pt;
@@ -940,13 +1047,14 @@ __global__ void __launch_bounds__(JT) k_prefill_join(const __grid_constant__ Pre
             for (int k = 0; k < 8; k++) {
                 if (p0 + k >= it.parts) break;
                 const float2 x = ml[(p0 + k) * 32 + lane];
-                const float e = x.y * exp2f(x.x - off);
+                const int lu = __float_as_int(x.y), u = lu & 255;
+                const float e = __int_as_float(lu & ~255) * exp2f(x.x - off), eu = u ? e * pow2(u - BIAS) : e;
                 l += e;
 #pragma unroll
                 for (int c = 0; c < CW / 2; c++) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[k][c]));
-                    o[2 * c] = fmaf(f.x, e, o[2 * c]);
-                    o[2 * c + 1] = fmaf(f.y, e, o[2 * c + 1]);
+                    o[2 * c] = fmaf(f.x, eu, o[2 * c]);
+                    o[2 * c + 1] = fmaf(f.y, eu, o[2 * c + 1]);
                 }
             }
         }

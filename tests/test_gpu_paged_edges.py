@@ -188,3 +188,81 @@ def test_prefill_scores_of_any_size(cuda, hd, bits):
     for i in list(range(0, t, 9)) + [t - 1]:
         o, _, _, big = ref.attend(c, 0, q[i].reshape(-1), n - t + i, nHq)
         assert ((got[i] - o).abs() <= 2.0 ** -8 * o.abs() + big * (2.0 ** -10 + 2.0 ** -14)).all(), (bits, i)
+
+
+@pytest.mark.parametrize("hd,nKv,nHq", [(64, 2, 4), (128, 1, 2)])
+@pytest.mark.parametrize("kscale", [1.0, 1e-7, 1e8])
+@pytest.mark.parametrize("vscale", [1e-11, 1e-7, 1e-4, 1.0, 1e4, 1e9, 1e30])
+def test_prefill_of_small_and_large_numbers(cuda, hd, nKv, nHq, kscale, vscale):
+    """K and V of any size (and q of the size that keeps the scores): errors relative to what is seen"""
+    ts, lens = [20, 150], [700, 150]
+    c = ref.Cache(52, 2, 45, 16, nKv, hd)
+    c.Ks *= kscale
+    c.Vs *= vscale
+    q = torch.randn(sum(ts), nHq * hd, generator=c.g) * (1.5 / kscale)
+    got, cu = _prefill(c, q, ts, lens, nHq)
+    for b, (n, t) in enumerate(zip(lens, ts)):
+        for i in range(0, t, 7):
+            o, _, mag, big = ref.attend(c, b, q[cu[b] + i], n - t + i, nHq)
+            tol = big * (2.0 ** -9 * mag + 2.0 ** -9) + 2.0 ** -8 * o.abs()
+            assert ((got[cu[b] + i] - o).abs() <= tol).all(), (b, i)
+            assert float((got[cu[b] + i] - o).norm() / o.norm()) < 2.0 ** -7
+
+
+@pytest.mark.parametrize("hd,nKv,nHq", [(64, 1, 4), (128, 2, 4)])
+@pytest.mark.parametrize("slope", [-0.2, 0.2])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (60, 3)])
+def test_prefill_of_numbers_that_grow_along_the_cache(cuda, hd, nKv, nHq, slope, window, sinks):
+    """V's size changes by 2^slope from row to row, in all by 2^120: a query's output is right relative to
+    the rows that it sees, whatever the others hold"""
+    ts, lens = [4, 300], [601, 300]
+    c = ref.Cache(53, 2, 40, 16, nKv, hd)
+    for b, n in enumerate(lens):
+        size = 2.0 ** torch.clamp(slope * (torch.arange(n) - n // 2), -38, 60).float()
+        c.Vs.view(-1, nKv * hd // 32)[c.rows(b, torch.arange(n))] *= size[:, None]
+    q = torch.randn(sum(ts), nHq * hd, generator=c.g) * 1.5
+    got, cu = _prefill(c, q, ts, lens, nHq, window, sinks)
+    for b, (n, t) in enumerate(zip(lens, ts)):
+        for i in range(0, t, 5 if t > 9 else 1):
+            o, _, mag, big = ref.attend(c, b, q[cu[b] + i], n - t + i, nHq, window, sinks)
+            tol = big * (2.0 ** -9 * mag + 2.0 ** -9) + 2.0 ** -8 * o.abs()
+            assert ((got[cu[b] + i] - o).abs() <= tol).all(), (b, i)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_rows_of_q_of_any_size(cuda, hd):
+    """a query's size is its own: tiny, huge and ordinary ones side by side"""
+    nKv, nHq, t = 2, 8, 40
+    c = ref.Cache(54, 1, 10, 16, nKv, hd)
+    size = 10.0 ** torch.randint(-12, 13, (t, nHq, 1), generator=c.g).float()
+    q = (torch.randn(t, nHq, hd, generator=c.g) * size).reshape(t, nHq * hd)
+    got, _ = _prefill(c, q, [t], [150], nHq)
+    for i in range(t):
+        for h in range(nHq):
+            one = q[i].clone().view(nHq, hd)
+            one[torch.arange(nHq) != h] = 0
+            o, _, mag, big = ref.attend(c, 0, one.view(-1), 150 - t + i, nHq)
+            # where the scores are large the best key's lead decides, and a rounding of them may be more than it
+            if mag < 100:
+                tol = big * (2.0 ** -9 * mag + 2.0 ** -9) + 2.0 ** -8 * o[h].abs()
+                assert ((got[i, h] - o[h]).abs() <= tol).all(), (i, h)
+            assert got[i, h].isfinite().all() and float(got[i, h].abs().max()) <= big * (1 + 2.0 ** -7)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prefill_small_outputs_of_parts(cuda, hd):
+    """V = +-1 that all but cancels (one key more of one sign): an item in parts keeps the small output's digits.
+    All scores are zero, so weights and products are exact and sums of them too; what is left is 1/l and the
+    join (f32, 2^-20 of the parts' outputs, which are at most 2^-8 here) and bf16's 2^-8 (twice the half step)."""
+    n, t, nHq = 4097, 2, 2
+    c = ref.Cache(50, 1, n // 32 + 1, 32, 1, hd)
+    c.Kq[:] = 0
+    c.Vs[:] = 127.0
+    sign = torch.ones(c.cap, dtype=torch.int8)
+    sign[1::2] = -1
+    c.Vq.view(-1, hd)[c.rows(0, torch.arange(c.cap))] = sign[:, None]
+    q = torch.randn(t, nHq * hd, generator=c.g)
+    got, _ = _prefill(c, q, [t], [n], nHq)
+    o = ref.attend(c, 0, q[1], n - 1, nHq)[0]
+    assert torch.allclose(o, torch.full_like(o, 1.0 / n), rtol=1e-9)
+    assert float((got[1] / o - 1).abs().max()) <= 2.0 ** -7
