@@ -483,7 +483,8 @@ TB_API int tb_attn_decode_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, float *ou
  * elements and the softmax weights are rounded to f16 (as in tb_attn_prefill_q8), behind
  * powers of two of their own: q's a row and head, K's and V's for 32 rows and a head, so
  * numbers may be of any size, and an element loses digits only far below the largest beside
- * it (K, V: 2^-25 of it; q: 2^-12); sums in f32.  At most 4096 sequences; T < 2^24. */
+ * it (K, V: 2^-25 of it; q: 2^-12), a
+ * weight below 2^-22 of the largest score's; sums in f32.  At most 4096 sequences; T < 2^24. */
 TB_API int tb_attn_prefill_paged_ws(tb_ctx *ctx, const tb_paged_kv *kv, int64_t nHq, int64_t T, size_t *bytes);
 TB_API int tb_attn_prefill_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, uint16_t *out_bf16, const float *q,
                                     const int32_t *cu, const int32_t *lens, int64_t nHq, int64_t T,

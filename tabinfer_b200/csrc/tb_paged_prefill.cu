@@ -15,7 +15,7 @@
 // Warp roles of k_paged_prefill:
 //   warps 0-3, 4-7   softmax of row tile 0 / 1, a thread a row: S from TMEM, P (f16) back
 //                    over it; the reference maximum is raised (and O rescaled in TMEM) only
-//                    when a score passes it by 2^9, so O is hardly ever touched; Q of the
+//                    when scores pass it by 2^2 to 2^8, so O is hardly ever touched; Q of the
 //                    next part into shared memory, then the part's outputs
 //   warps 8-11       K / V tiles: 16-byte copies ahead into thread-private shared memory, bytes
 //                    -> f16 (one exact step, one multiplication by the group's scale) into
@@ -26,7 +26,8 @@
 // Roundings: Q, dequantized K and V (and their scales) and P to f16, relative 2^-11 each, and
 // parts' outputs on their way through memory; S, the statistics and O in f32.  Q's rows, K and V
 // of 32 keys, O and a part's outputs carry powers of two of their own (below), so this holds for
-// numbers of any size: an element of K or V loses digits below 2^-25 of the largest one of its
+// numbers of any size and for weights down to 2^-22 of the reference (2^-33 of it is the error of
+// those below): an element of K or V loses digits below 2^-25 of the largest one of its
 // head in the same 32 rows (2^-36 of that one at most), one of Q below 2^-12 of its row's
 // largest (2^-23).
 //
@@ -70,7 +71,13 @@ constexpr int STAGGER = 900;
 // The smallest e, a zero's too, leaves the factor of the scores a normal number: a score masked with -inf stays it.
 constexpr int BIAS = 128, TOP = 15, E_MIN = -40;
 constexpr int Q_E = 11, Q_MIN = -6;       // q whose rows' largest lie between 2^Q_MIN and 2^Q_E share e = Q_E
-constexpr float TOO_LARGE = 32768.0f;    // sum of a half's exponentials that raises the reference maximum
+// A weight goes to f16 as 2^(score - reference + LIFT): one of the reference's size uses the upper part of f16's
+// range, so weights down to 2^-22 of it keep 2^-11 of themselves, and those below lose 2^-33 of it at most (without
+// the lift 2^-14 and 2^-25: many light keys beside a heavy one then came out wrong).
+constexpr float LIFT = 8.0f;
+// Sum of a half's weights that raises the reference: below it each of them fits f16, and with every score at or below
+// the reference the 64 come to 2^14 at most.  (At 2^15 more halves are repeated: 77 rows 33.8 us instead of 33.1.)
+constexpr float TOO_LARGE = 65504.0f;
 constexpr float FAR = 1048576.0f;        // scores (log2) whose last bit, 2^-4, is felt in a weight
 
 struct Part {
@@ -536,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 // In two halves of 64 keys: a half's P V and the next tile's Q K^T over its place run under the
                 // other half's softmax, so scores are there when a thread comes for them.
                 // One pass over a half's scores against the reference maximum as it stands: no maximum is
-                // formed.  Where the sum tells that a score has passed it by 2^9 or more, the maximum is
+                // formed.  Where the sum tells that scores have passed it (one by 2^8, or all by 2^2), the maximum is
                 // taken, O rescaled (every column, once the last product is in) and the pass repeated, once.  A
                 // row's first reference is the maximum of the first half in which it sees a key.
 #pragma unroll 1
@@ -613,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     // first is up to half an ulp of m from 0, which is nothing below FAR and past 2^24 any size, up or down;
                     // the second is 0 at most, and 0 for the largest x.
                     auto pass = [&](auto exact) {
-                        const float off = m == -INFINITY ? 0.0f : -m, off0 = off - d0, off1 = off - d1;
+                        const float off = m == -INFINITY ? 0.0f : -m, off0 = off + (LIFT - d0), off1 = off + (LIFT - d1);
                         float2 s2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
                         float x[64];                      // all of the half at once: one wait, and the exponentials
                         tmem_ld32(th, reinterpret_cast<uint32_t*>(x));       // back to back (16 at a time took twice as long)
@@ -629,8 +636,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                             float2 y;
                             if (exact) y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), make_float2(sc, sc), make_float2(of, of));
                             else {                        // (the rounded product less m first: 0 for the largest)
-                                y.x = __fadd_rn(__fadd_rn(__fmul_rn(x[2 * i], sc), off), -d);
-                                y.y = __fadd_rn(__fadd_rn(__fmul_rn(x[2 * i + 1], sc), off), -d);
+                                y.x = __fadd_rn(__fadd_rn(__fmul_rn(x[2 * i], sc), off), LIFT - d);
+                                y.y = __fadd_rn(__fadd_rn(__fmul_rn(x[2 * i + 1], sc), off), LIFT - d);
                             }
                             const float2 e = make_float2(ex2(y.x), ex2(y.y));
                             s2[i >> 4] = fadd2(s2[i >> 4], e);
@@ -639,7 +646,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                         sum = make_float2(s2[0].x + s2[0].y, s2[1].x + s2[1].y);
                     };
                     pass(std::true_type());
-                    // below it every weight fits f16; past it some score is 2^9 above the reference
+                    // below it every weight fits f16; past it some score is above the reference
                     if (__any_sync(0xffffffffu, sum.x + sum.y >= TOO_LARGE || lower < 1.0f || (fabsf(m) > FAR && m != -INFINITY))) {
                         const float mx = fmaxf(m, largest());
                         if (!fresh) {
@@ -659,7 +666,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                             l *= f;
                         }
                         m = mx;
-                        pass(std::false_type());          // once: every weight of every row is 1 at most now
+                        pass(std::false_type());          // once: no score of any row is above the reference now
                     }
                     tmem_st32(th, pk);                    // over scores that are read
                     l = fmaf(sum.x, b0, fmaf(sum.y, b1, l));

@@ -266,3 +266,31 @@ def test_prefill_small_outputs_of_parts(cuda, hd):
     o = ref.attend(c, 0, q[1], n - 1, nHq)[0]
     assert torch.allclose(o, torch.full_like(o, 1.0 / n), rtol=1e-9)
     assert float((got[1] / o - 1).abs().max()) <= 2.0 ** -7
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n,t", [(8193, 3), (300, 290)])
+@pytest.mark.parametrize("gap", [6.0, 14.0, 20.0, 22.0, 24.5])
+def test_prefill_light_weights_beside_a_heavy_one(cuda, hd, n, t, gap):
+    """One first key with nearly all of the weight and V = 0, so the output is what the light keys, 2^-gap of
+    it each, give.  q and K's elements are multiples of 1/64 below 16 and exact in f16, V's are too, so what is
+    left is a weight's rounding: 2^-11 of itself where 2^(8 - gap) is normal in f16, and 2^-25 of 2^(8 - gap)
+    below (the exponential 2^-22); a part's output 2^-11, bf16 2^-8 (twice the half steps)."""
+    nKv, nHq, page = 1, 2, 16
+    c = ref.Cache(49, 1, n // page + 1, page, nKv, hd)
+    c.Ks[:] = 127.0 / 64
+    c.Vs[:] = 127.0 / 64
+    c.Kq[:] = 0
+    c.Vq[:] = (torch.arange(c.Vq.numel()).view(c.Vq.shape) % 50 + 60).to(torch.int8)
+    first = int(c.rows(0, 0))
+    c.Vq.view(-1, hd)[first] = 0
+    # score of the first key: 16 x k q_0 / sqrt(hd) = gap ln 2, to the nearest step of q in 1/64
+    c.Kq.view(-1, hd)[first, :16] = 64
+    q = torch.zeros(t, nHq * hd)
+    q.view(t, nHq, hd)[:, :, :16] = round(gap * 0.6931471805599453 * hd ** 0.5 / 16 * 64) / 64
+    got, _ = _prefill(c, q, [t], [n], nHq)
+    for i in sorted({1, t // 2, t - 1}):
+        o, _, _, _ = ref.attend(c, 0, q[i], n - t + i, nHq)
+        x = float(q[i, 0]) * 16 * hd ** -0.5 / 0.6931471805599453        # the gap as it is
+        tol = 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -11 + max(0.0, 2.0 ** (x - 33))
+        assert float(((got[i] - o) / o).abs().max()) <= tol, i
