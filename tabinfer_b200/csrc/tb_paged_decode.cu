@@ -714,7 +714,7 @@ __global__ void __launch_bounds__(256) k_paged_weights(const __grid_constant__ D
     for (int g = 0; g < GRP; g++) {
         const float2 ml = a.ML[(long long)b * a.nHq + h * GRP + g];
         m[g] = ml.x;
-        r[g] = ml.y > 0.0f ? 1.0f / ml.y : 0.0f;
+        r[g] = ml.y > 0.0f || ml.y != ml.y ? 1.0f / ml.y : 0.0f;     // a sum of no number leaves no weight one
     }
 #pragma unroll
     for (int i = 0; i < KEYS; i++) {

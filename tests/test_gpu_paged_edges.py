@@ -294,3 +294,24 @@ def test_prefill_light_weights_beside_a_heavy_one(cuda, hd, n, t, gap):
         x = float(q[i, 0]) * 16 * hd ** -0.5 / 0.6931471805599453        # the gap as it is
         tol = 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -11 + max(0.0, 2.0 ** (x - 33))
         assert float(((got[i] - o) / o).abs().max()) <= tol, i
+
+
+def test_decode_weights_of_no_number(cuda):
+    """a sequence whose scores hold no number (a query's NaN, a key's scale) has no weights either: every row
+    it sees becomes NaN, those outside its window and the other sequences' stay numbers"""
+    nKv, hd, nHq, lens, window, sinks = 2, 64, 4, [300, 77, 120], 100, 2
+    c = ref.Cache(48, 3, 20, 16, nKv, hd)
+    c.Ks.view(-1, nKv, 2)[int(c.rows(1, 40)), 0, 1] = float("nan")
+    q = torch.randn(3, nHq * hd, generator=c.g)
+    q.view(3, nHq, hd)[0, 1, 5] = float("nan")
+    w = torch.ones(3, nKv, c.cap, device="cuda")
+    tb.attention_decode_paged_q8(q.cuda(), c.dev(), c.table.cuda(), _ints(lens), nHq, nKv, hd, window=window,
+                                 sinks=sinks, weights=w)
+    for b, n in enumerate(lens):
+        ok = torch.zeros(c.cap, dtype=torch.bool)
+        ok[:n] = ref.seen(n, n - 1, window, sinks)
+        none = torch.zeros(nKv, c.cap, dtype=torch.bool)
+        if b < 2:
+            none[0] = ok
+        assert torch.equal(w[b].cpu().isnan(), none), b
+        assert (w[b].cpu()[:, ~ok] == 1).all()
