@@ -454,7 +454,10 @@ typedef struct tb_paged_kv {
  * pairs of a call are distinct).  q -> per-head RMSNorm + RoPE -> qr f32; k the
  * same and v as it is -> snorm int8 per 32 into the cache.  seq[t] < 0 marks a
  * padding row: nothing is written for it.  Norm and rotation are formed in 64 bits
- * and rounded to f32 once, so a cache byte does not depend on the call that wrote it. */
+ * and rounded to f32 once, so a cache byte does not depend on the call that wrote it.
+ * A NaN makes the scale of its 32 elements NaN, an infinity in v makes it infinite (the
+ * contiguous writers leave a NaN out); for the queries that see such a row the operators
+ * below give no number: in the 32 dimensions for V's, in the kv head's q heads for K's. */
 TB_API int tb_attn_prep_paged_q8(tb_ctx *ctx, const tb_paged_kv *kv, const float *q, const float *k,
                                  const float *v, const uint16_t *qw16, const uint16_t *kw16, float *qr,
                                  int64_t nHq, int64_t T, const int32_t *seq, const int32_t *slot,

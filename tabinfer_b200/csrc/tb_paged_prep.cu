@@ -45,13 +45,24 @@ __device__ __forceinline__ double shfl_xor_f64(double v, int m)
                             __shfl_xor_sync(0xffffffffu, __double2loint(v), m));
 }
 
-// x of one head (element l + 32 i in lane l) as snorm bytes with a scale a 32-group
+// the warp's largest |x|, NaN where one of them is
+__device__ __forceinline__ float redux_abs_nan(float x)
+{
+    float r;
+    asm volatile("redux.sync.max.abs.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+    return r;
+}
+// x of one head (element l + 32 i in lane l) as snorm bytes with a scale a 32-group.  A NaN among
+// the 32 makes the scale NaN, so that whoever reads the row meets it.
 template <int NW>
 __device__ __forceinline__ void store_q8(const float (&x)[NW], int8_t* dq, float* ds, int lane)
 {
     float m[NW];
 #pragma unroll
-    for (int i = 0; i < NW; i++) m[i] = fmaxf(1e-12f, redux_max(fabsf(x[i])));
+    for (int i = 0; i < NW; i++) {
+        const float r = redux_abs_nan(x[i]);
+        m[i] = r < 1e-12f ? 1e-12f : r;
+    }
 #pragma unroll
     for (int i = 0; i < NW; i++) dq[32 * i + lane] = snorm8(x[i], m[i], __fdividef(1.0f, m[i]));
     if (lane == 0) {

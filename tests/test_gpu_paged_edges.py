@@ -315,3 +315,46 @@ def test_decode_weights_of_no_number(cuda):
             none[0] = ok
         assert torch.equal(w[b].cpu().isnan(), none), b
         assert (w[b].cpu()[:, ~ok] == 1).all()
+
+
+@pytest.mark.parametrize("hd,T", [(128, 3), (64, 3), (128, 900)])
+def test_prep_keeps_what_is_not_a_number(cuda, hd, T):
+    """NaN in v: its 32-group's scale is NaN, so that every reader meets it; infinity in v: an infinite scale;
+    NaN in k: the head has no number after its norm, and every scale of it is NaN; infinity in k: x / sqrt(mean
+    x^2) is inf / inf in its place, so the rotation makes it and its partner hd / 2 away NaN, and 0 elsewhere.
+    Other groups, heads and rows are what they are without it."""
+    nKv, nHq, page = 3, 3, 16
+    c = ref.Cache(55, 1, T // page + 1, page, nKv, hd, fill=False)
+    g = torch.Generator().manual_seed(7)
+    q, k, v = (torch.randn(T, 3 * hd, generator=g) for _ in range(3))
+    w = torch.ones(hd, dtype=torch.float16, device="cuda")
+    at = torch.arange(T, dtype=torch.int32).cuda()
+
+    def run(k, v):
+        kv = c.dev()
+        tb.attn_prep_paged_q8(q.cuda(), k.cuda(), v.cuda(), w, w, kv, c.table.cuda(), torch.zeros_like(at), at, at, nHq,
+                              nKv, hd, 1e6, 1e-6)
+        r = c.rows(0, torch.arange(T))
+        return [t.cpu().view(-1, nKv, t.shape[-1] // nKv)[r] for t in kv]
+    clean = run(k, v)
+    k2, v2 = k.clone(), v.clone()
+    v2.view(T, nKv, hd)[1, 0, 40] = float("nan")
+    v2.view(T, nKv, hd)[T - 1, 2, 3] = float("-inf")
+    k2.view(T, nKv, hd)[0, 1, 5] = float("nan")
+    k2.view(T, nKv, hd)[T - 1, 0, 33] = float("inf")
+    Kq, Ks, Vq, Vs = run(k2, v2)
+    Kn = torch.zeros(T, nKv, hd // 32, dtype=torch.bool)
+    Kn[0, 1] = True
+    Kn[T - 1, 0, 1] = Kn[T - 1, 0, (33 + hd // 2) % hd // 32] = True
+    assert torch.equal(Ks.isnan(), Kn)
+    rest = ~Kn[T - 1, 0]
+    assert (Ks[T - 1, 0][rest] == 1e-12).all() and (Kq[T - 1, 0][rest.repeat_interleave(32)] == 0).all()
+    Kn[T - 1, 0] = True
+    Vn = torch.zeros(T, nKv, hd // 32, dtype=torch.bool)
+    Vn[1, 0, 1] = True
+    assert torch.equal(Vs.isnan(), Vn) and Vs[T - 1, 2, 0] == float("inf") and int(Vs.isinf().sum()) == 1
+    Vn[T - 1, 2, 0] = True
+    for bad, now, was in ((Kn, (Kq, Ks), clean[:2]), (Vn, (Vq, Vs), clean[2:])):
+        assert torch.equal(now[1][~bad], was[1][~bad])
+        ok = ~bad.repeat_interleave(32, 2)
+        assert torch.equal(now[0][ok], was[0][ok])
