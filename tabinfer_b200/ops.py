@@ -664,6 +664,7 @@ def _paged(kv, table, nKv, hd, index, what="kv"):
                      nKv, hd), r, B, most
 
 
+_F16 = (torch.float16, torch.int16, torch.uint16)
 _ws_sizes = {}
 
 
@@ -693,8 +694,8 @@ def attn_prep_paged_q8(q, k, v, qw16, kw16, kv, table, seq, slot, pos, nHq, nKv,
         op = qr.data_ptr()
     else:
         op = _arg(qr, "qr", f32, wide, d)
-    if qw16.dtype.itemsize != 2 or kw16.dtype.itemsize != 2:
-        raise TabInferError("the norm weights are f16 (16-bit patterns)")
+    if qw16.dtype not in _F16 or kw16.dtype not in _F16:
+        raise TabInferError("the norm weights are f16 (or its 16-bit patterns), not %s and %s" % (qw16.dtype, kw16.dtype))
     rc = LIB.tb_attn_prep_paged_q8(
         default_context(d).h, s, qp, kp, vp, _arg(qw16, "qw16", qw16.dtype, w16, d),
         _arg(kw16, "kw16", kw16.dtype, w16, d), op, nHq, T, _arg(seq, "seq", i32, (T,), d),

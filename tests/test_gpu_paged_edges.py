@@ -358,3 +358,20 @@ def test_prep_keeps_what_is_not_a_number(cuda, hd, T):
         assert torch.equal(now[1][~bad], was[1][~bad])
         ok = ~bad.repeat_interleave(32, 2)
         assert torch.equal(now[0][ok], was[0][ok])
+
+
+def test_prep_refuses_norm_weights_of_other_types(cuda):
+    """bf16 has as many bits as f16 and another meaning"""
+    c = ref.Cache(81, 2, 4, 16, 2, 64)
+    kv, table = c.dev(), c.table.cuda()
+    q = torch.randn(2, 256, device="cuda")
+    w, i = torch.ones(64, dtype=torch.float16, device="cuda"), _ints([0, 1])
+    kr = q[:, :128].contiguous()
+
+    def prep(qw, kw):
+        return tb.attn_prep_paged_q8(q, kr, kr, qw, kw, kv, table, i, i, i, 4, 2, 64, 1e6, 1e-6)
+    want = prep(w, w)
+    assert torch.equal(prep(w.view(torch.int16), w.view(torch.uint16)), want)      # the patterns of f16
+    for a, b in ((w.bfloat16(), w), (w, w.bfloat16()), (w.float(), w), (w, w.float())):
+        with pytest.raises(tb.TabInferError):
+            prep(a, b)
