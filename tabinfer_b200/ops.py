@@ -774,8 +774,8 @@ def kv_evict_paged_q8(kv, table, lens, weights, new_table, budget, sinks, recent
     wp = _arg(weights, "weights", torch.float32, (B, nKv, most * rows), d)
     if new_B != B:
         raise TabInferError("new_table must have %d rows" % B)
-    if budget < 0:
-        raise TabInferError("budget must not be negative")
+    if not 0 <= budget <= new_most * new_rows:          # before anything of its size is made
+        raise TabInferError("budget must be 0 .. %d, the rows of the new table (got %d)" % (new_most * new_rows, budget))
     kept, new_lens = lens.new_empty((B, int(budget))), torch.empty_like(lens)
     new_weights = weights.new_empty((B, nKv, new_most * new_rows))
     c = default_context(d)

@@ -375,3 +375,12 @@ def test_prep_refuses_norm_weights_of_other_types(cuda):
     for a, b in ((w.bfloat16(), w), (w, w.bfloat16()), (w.float(), w), (w, w.float())):
         with pytest.raises(tb.TabInferError):
             prep(a, b)
+
+
+def test_evict_refuses_a_budget_before_it_allocates(cuda):
+    c = ref.Cache(82, 2, 4, 16, 2, 64)
+    kv, weights = c.dev(), torch.zeros(2, 2, 64, device="cuda")
+    for budget in (17, 1 << 31, 1 << 45):
+        with pytest.raises(tb.TabInferError):
+            tb.kv_evict_paged_q8(kv, c.table.cuda(), _ints([10, 20]), weights, _ints([[8], [9]]), budget, 2, 3, 2, 64)
+    assert torch.cuda.memory_allocated() < 1 << 30
