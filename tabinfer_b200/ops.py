@@ -665,7 +665,8 @@ def _paged(kv, table, nKv, hd, index, what="kv"):
 
 
 _F16 = (torch.float16, torch.int16, torch.uint16)
-_ws_sizes = {}
+_ws_sizes = {}              # of the last calls' sizes: a server's prefills come at many row counts
+_WS_SIZES = 1024
 
 
 def _workspace(c, query, index, s, lens, *sizes):
@@ -677,6 +678,8 @@ def _workspace(c, query, index, s, lens, *sizes):
     if n is None:
         v = ctypes.c_size_t()
         c.check(getattr(LIB, query)(c.h, s, *sizes, ctypes.byref(v)), query)
+        if len(_ws_sizes) >= _WS_SIZES:
+            _ws_sizes.clear()
         n = _ws_sizes[key] = max(v.value + 3 & ~3, 256)
     return lens.new_empty(n >> 2), n
 
