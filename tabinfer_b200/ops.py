@@ -22,6 +22,11 @@ class TabInferError(RuntimeError):
     pass
 
 
+# a device's current stream as its handle alone (a Stream object takes 1.2 us more); not part of torch's
+# documented interface, so its absence is provided for
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 class Context:
     """One tb_ctx per (host thread, device): replaces the engine handle of
     engine/webgpu-engine.js:72 and the module scratch of models/qwen3.js."""
@@ -43,8 +48,11 @@ class Context:
         """Order the library's work on torch's current stream.  torch reports its
         default (legacy NULL) stream as handle 0, which the C ABI reads as "the
         context's own stream", so it is passed as cudaStreamLegacy (0x1)."""
-        torch.cuda.init()
-        s = torch._C._cuda_getCurrentRawStream(self.device)     # the handle alone: a Stream object takes 1.2 us
+        if _raw_stream is None:
+            s = torch.cuda.current_stream(self.device).cuda_stream
+        else:
+            torch.cuda.init()
+            s = _raw_stream(self.device)
         LIB.tb_ctx_set_stream(self.h, P(s if s else CUDA_STREAM_LEGACY))
 
     def own_stream(self):

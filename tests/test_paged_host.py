@@ -39,3 +39,21 @@ def test_workspace_sizes_are_bounded(monkeypatch):
     before = lib.queries
     ops._workspace(_Ctx(), "size", 0, kv, lens, 4999)
     assert lib.queries == before                              # the last size is known
+
+
+def test_current_stream_with_and_without_the_raw_handle(monkeypatch):
+    lib = _Lib()
+    monkeypatch.setattr(ops, "LIB", lib)
+    monkeypatch.setattr(torch.cuda, "init", lambda: None)
+
+    class Stream:
+        def __init__(self, device):
+            self.cuda_stream = 0 if device == 0 else 4000 + device
+    monkeypatch.setattr(torch.cuda, "current_stream", Stream)
+    for raw in (None, lambda device: Stream(device).cuda_stream):
+        monkeypatch.setattr(ops, "_raw_stream", raw)
+        for device in (0, 3):
+            c = object.__new__(ops.Context)
+            c.h, c.device = None, device
+            c.bind_stream()
+    assert lib.streams == [ops.CUDA_STREAM_LEGACY, 4003] * 2
