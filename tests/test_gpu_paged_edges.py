@@ -384,3 +384,38 @@ def test_evict_refuses_a_budget_before_it_allocates(cuda):
         with pytest.raises(tb.TabInferError):
             tb.kv_evict_paged_q8(kv, c.table.cuda(), _ints([10, 20]), weights, _ints([[8], [9]]), budget, 2, 3, 2, 64)
     assert torch.cuda.memory_allocated() < 1 << 30
+
+
+def _choose(w, n, budget, sinks, recent):
+    """ref.evict where scores may be NaN: those come before every number, the lower row first"""
+    if n <= budget:
+        return list(range(n))
+    score = w.double().sum(0)
+    rank = [(0, 0.0, j) if score[j].isnan() else (1, -float(score[j]), j) for j in range(sinks, n - recent)]
+    mid = [r[2] for r in sorted(rank)][:budget - sinks - recent]
+    return sorted(list(range(sinks)) + mid + list(range(n - recent, n)))
+
+
+@pytest.mark.parametrize("nKv,hd,lens,budget,page", [(2, 64, [300, 90, 40], 50, 16), (8, 128, [700, 1100], 300, 32),
+                                                      (8, 128, [20000], 5000, 256), (3, 64, [2500], 40, 16)])
+@pytest.mark.parametrize("few", [True, False])
+def test_evict_weights_of_no_number(cuda, nKv, hd, lens, budget, page, few):
+    """NaN of either sign, and NaN that is infinity less infinity over the heads, count as the largest score,
+    beside infinities; few of them, or more than the budget holds"""
+    c = ref.Cache(57, len(lens), -(-max(lens) // page), page, nKv, hd)
+    w = torch.exp(2 * torch.randn(c.B, nKv, c.cap, generator=c.g))
+    step = 29 if few else 3
+    w[:, 0, 1::step] = float("nan")
+    w[:, 1, 5::step] = -float("nan")
+    w[:, 0, 9::step], w[:, 1, 9::step] = float("inf"), float("-inf")
+    w[:, 1, 2::17] = float("inf")
+    _evict(c, lens, w, budget, 3, 6, _choose)
+
+
+def test_evict_more_heads_than_ctas(cuda):
+    """more (sequence, kv head) pairs than CTAs copy weights, and more kept rows than warps"""
+    B = 170
+    lens = [1 + (37 * b) % 96 for b in range(B)]
+    c = ref.Cache(58, B, 6, 16, 8, 128)
+    w = torch.rand(B, 8, c.cap, generator=c.g)
+    _evict(c, lens, w, 33, 2, 5)
