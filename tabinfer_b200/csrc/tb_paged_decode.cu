@@ -205,13 +205,13 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return ffma2(a, b, 
 // issue slots that the tile's share of the HBM rate leaves an SM; the form that converts V
 // and K to f32 takes 1180.
 // Measured with the join (bytes of the rows seen, their scales and the weights; 6.55 TB/s is
-// what a copy reaches): 131001 rows of 8 heads of 128, 302 MB, 60.8 us (5.0 TB/s: memory, and
-// a start of 6 us); 32 ragged sequences of 8192 rows and below with weights, 329 MB, 73.7 us
+// what a copy reaches): 131001 rows of 8 heads of 128, 302 MB, 59 us (5.1 TB/s: memory, and
+// a start of 6 us); 32 ragged sequences of 8192 rows and below with weights, 329 MB, 73.0 us
 // (4.5 TB/s: three kernels, and the scores pass through memory); 16 windows of 4096 rows of 8
-// heads of 64, 76 MB, 31 us (2.4 TB/s: a tile of half the bytes has as many steps behind one
-// another, 2100 cycles and 1000 for the next one's copies; 128 registers allow no more warps);
-// one sequence of 4096 rows 11.7 us, a chain of latencies: plan, page number, tile, products,
-// join.
+// heads of 64, 76 MB, 31.5 us (2.4 TB/s: a tile of half the bytes has as many steps behind one
+// another, 2100 cycles and 1000 for the next one's copies; the 128 registers of four CTAs an SM
+// hold no larger tile, and fewer CTAs with larger ones were not tried); one sequence of 4096
+// rows 11.6 us, a chain of latencies: plan, page number, tile, products, join.
 template <int HD, int GRP>
 __global__ void __launch_bounds__(NT, RingLayout<HD, GRP>::OCC) k_paged_decode(const __grid_constant__ DecArgs a)
 {

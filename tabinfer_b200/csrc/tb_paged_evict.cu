@@ -7,11 +7,11 @@
 //   then exact up to far below their own rounding, so the choice does not depend on the
 //   order of the sum); ties go to the lower row
 //
-// 16 sequences of 8192 rows and below to 2048 (8 heads of 128; 146 MB) take 52 us: scores 5,
-// selection 19, copy 27 (5.4 TB/s); one of 131072 rows to 16384 (80 MB) 41: scores 5,
-// selection 25, copy 10.  Slower: 16 CTAs a sequence (43 us for the long one), the scores
-// formed by the selecting clusters (one launch less, but 52, and 2 us more at 2048 rows),
-// 11-bit digits (61).
+// 16 sequences of 8192 rows and below to 2048 (8 heads of 128; 146 MB) take 51 us: scores 5,
+// selection 19, copy 27 (5.4 TB/s); one of 131072 rows to 16384 (80 MB) 41, of which scores 5,
+// selection 25, copy 10 (one call repeated, its weights in L2; calls over other inputs in turn
+// 54 and 48).  Slower: 16 CTAs a sequence (43 us for the long one), the scores formed by the
+// selecting clusters (one launch less, but 52, and 2 us more at 2048 rows), 11-bit digits (61).
 #include "tb_paged.cuh"
 
 namespace {
@@ -19,8 +19,9 @@ namespace {
 constexpr int ST = 1024;          // threads of a selecting CTA
 constexpr int DIGIT = 8, BINS = 1 << DIGIT;   // larger digits cost more in reading the other CTAs' counts than they save
 constexpr int MAX_CLUSTER = 8;    // CTAs a sequence (portable)
-// Table rows a CTA takes before a sequence gets another one (one CTA, and up to eight: 2048 rows 16.9 and 18.0
-// us for the whole call, 16384 rows 27.1 and 23.0, 131072 rows 136 and 42, 16 sequences of 8192 31.8 and 31.0).
+// Table rows a CTA takes before a sequence gets another one.  One CTA, and always eight, a call that keeps an eighth of
+// the rows, over 400 MB of inputs in turn: 2048 rows 19.9 and 21.0 us, 4096 22.6 and 22.5, 16384 30.3 and 25.5, 131072
+// 168 and 49; 16 sequences of up to 2048 24.5 and 26.8, of up to 8192 40.6 and 39.8; 32 of up to 4096 37.9 and 54.1.
 constexpr int SLOTS = 2048;
 constexpr int KEPT_KEYS = 16;     // keys a thread holds in registers; those beyond are read again each step
 

@@ -32,18 +32,24 @@
 // largest (2^-23).
 //
 // What bounds it.  Its operations at the bf16 rate a library product reaches (1679 TFLOP/s)
-// would take 164 us at 8192 rows (16 / 8 heads of 128); it takes 314 (876 TFLOP/s), 2048 rows
-// 48 (356), three chunks of up to 2001 rows under a window of 1024 (32 / 8 heads of 64) 147
-// (286).  A half of 64 keys takes a softmax warp about 2200 cycles, two of them sharing a
-// scheduler: 1100 to 1500 for its 64 exponentials with their sums and conversions (1024 of the
-// special function unit for both warps), the rest waits, TMEM loads and stores and the
-// barriers; the tensor cores are busy half of the time, so 64-wide heads, with half the
-// product for the same exponentials, come out at a third of the rate.  Short chunks (77 rows
-// behind 8192: 31 us) are the plan, the first tiles' latency and the join.
-// Measured and not kept: 16 softmax warps of 16 columns (362 us at 8192 rows), whole tiles of
-// 128 keys a softmax step (340), a quarter of the exponentials by polynomial (315), taking
-// turns at the exponentials (352), the next half's scores fetched ahead of the weights' store
-// (320), an MMA warp a row tile (323), raw bytes in registers (348).
+// would take 164 us at 8192 rows (16 / 8 heads of 128); it takes 310 alone (887 TFLOP/s;
+// 349, 787, call after call over other inputs, at the power cap), 2048 rows 51 (337), three
+// chunks of up to 2001 rows under a window of 1024 (32 / 8 heads of 64) 152 (276).  A half
+// of 64 keys takes a softmax warp about 2200 cycles, two of them sharing a scheduler: 1100
+// to 1500 for its 64 exponentials with their sums and conversions (1024 of the special
+// function unit for both warps), the rest waits, TMEM loads and stores and the barriers;
+// the tensor cores are busy half of the time, so 64-wide heads, with half the product for
+// the same exponentials, come out at a third of the rate (their exponentials alone are a
+// quarter of the time; the rest is the step's latency, and halves that no row of a tile
+// sees are worked through).  Short chunks (77 rows behind 8192: 32 us) are the plan, the
+// first tiles' latency and the join.  The powers of two, the lift and the marks cost 1 to
+// 2.5 us a call, most of it instructions that a short call runs through once (8192 rows:
+// nothing).
+// Measured and not kept (times of their day, beside 314 to 320 at 8192 rows): 16 softmax
+// warps of 16 columns (362 us at 8192 rows), whole tiles of 128 keys a softmax step (340),
+// a quarter of the exponentials by polynomial (315), taking turns at the exponentials
+// (352), the next half's scores fetched ahead of the weights' store (320), an MMA warp a
+// row tile (323), raw bytes in registers (348).
 // Every wait is bounded: one that gives up sets the error word and the CTA's abort flag, all
 // roles leave, the MMA thread waits for its last commit and TMEM is freed.
 #include <cuda_bf16.h>
@@ -61,8 +67,9 @@ constexpr int PROD = 128, W_MMA = 12;
 constexpr int NC = 4;                      // 16-byte chunks a producer thread takes at a time
 constexpr int KV_STAGES = 2;
 constexpr int MAX_BATCH = 4096;          // sequences a call (the plan keeps their sums in shared memory)
-// cycles by which row tile 1's softmax starts a part behind tile 0's (8192 rows 321 us with none, 318 with 300, 314
-// with 900 and 1200; three 2001-row chunks under a window 154, 149, 147, 149)
+// cycles by which row tile 1's softmax starts a part behind tile 0's (8192 rows 316 us with none, 318 with 450, 314
+// with 900; three 2001-row chunks under a window 158, 153, 151.6; 2048 rows 50.2, 50.2, 49.5; short ones too: 700 rows
+// 23.5, 23.2, 22.9, one row 12.6 with any)
 constexpr int STAGGER = 900;
 // Powers of two.  f16 holds 30 binades, so Q's rows and the K and V of 32 keys are brought to its upper end first:
 // x = x' 2^(e - TOP), the largest |x'| of K and of V in [2^11, 2^15), e a multiple of 4, so that a group's powers are
@@ -447,8 +454,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
             constexpr int C4 = HD / 4;                          // float4 columns a row
             auto load = [&](int i) {
                 const int ir = 128 * t + 32 * wq + i / C4, qi = ir / GRP;
-                return qi < p.nq ? __ldg(reinterpret_cast<const float4*>(a.q + ((long long)(p.row0 + qi) * a.nHq + h * GRP + ir % GRP) * HD) + i % C4)
-                                 : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                const float* src = a.q + ((long long)(p.row0 + qi) * a.nHq + h * GRP + ir % GRP) * HD;
+                return qi < p.nq ? __ldg(reinterpret_cast<const float4*>(src) + i % C4) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             };
             auto store = [&](int i, float4 v, float f) {
                 const int r = 32 * wq + i / C4, c = i % C4;
@@ -476,7 +483,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 }
                 // of the row of load i; of the rows 2 i (bit i) and 2 i + 1 (bit 16 + i)
                 has = __reduce_or_sync(0xffffffffu, C4 < 32 && lane >= 16 ? has << 16 : has);
-                const uint32_t all = C4 == 32 ? below(min(16, rows - i0 / C4)) : below(min(16, (rows + 1) / 2)) | below(min(16, rows / 2)) << 16;
+                const uint32_t all = C4 == 32 ? below(min(16, rows - i0 / C4))
+                                              : below(min(16, (rows + 1) / 2)) | below(min(16, rows / 2)) << 16;
                 fine = fine && (has & all) == all;
             }
             if (!__all_sync(0xffffffffu, fine && most < pow2(Q_E))) {
@@ -647,7 +655,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                     };
                     pass(std::true_type());
                     // below it every weight fits f16; past it some score is above the reference
-                    if (__any_sync(0xffffffffu, sum.x + sum.y >= TOO_LARGE || lower < 1.0f || (fabsf(m) > FAR && m != -INFINITY))) {
+                    const bool far = fabsf(m) > FAR && m != -INFINITY;
+                    if (__any_sync(0xffffffffu, sum.x + sum.y >= TOO_LARGE || lower < 1.0f || far)) {
                         const float mx = fmaxf(m, largest());
                         if (!fresh) {
                             // the half before: the last tile's second, or this tile's first
@@ -837,6 +846,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_paged_prefill(const __grid_const
                 marks[mat] = miss;
                 marks[mat + 2] = mk;
             }
+            // (a scale goes in as f16, one rounding more an element: as f32 the three tiles' scales take 6 KB more than
+            // the shared memory has left)
             scs[(2 * buf) * PK + pt] = make_uint2(pack_h2(ks[0] * fk, ks[1] * fk), pack_h2(ks[2] * fk, ks[3] * fk));
             scs[(2 * buf + 1) * PK + pt] = make_uint2(pack_h2(vs[0] * fv, vs[1] * fv), pack_h2(vs[2] * fv, vs[3] * fv));
         };

@@ -4,17 +4,21 @@
 //   y = x / sqrt(mean x^2 + eps) * w;  (y_i, y_{i+hd/2}) rotated by pos * theta^(-2i/hd)
 //   per 32 elements m = max(1e-12, max|x|), byte = floor(0.5 + 127 * x / m)
 //
-// The q / k rows are formed in 64 bits and rounded to f32 once, so a byte of the
-// cache does not depend on how a row's sum was split or in which call it was written
-// (f32 sums put a byte one step off wherever they differ next to a rounding border).
+// The q / k rows are formed in 64 bits and rounded to f32 once: the bytes are then those of
+// the definition, whatever the order of a sum (f32 sums put a byte one step off wherever they
+// differ next to a rounding border).  That a byte does not depend on the call that wrote it
+// comes from the fixed order of a head's sum, the same 32 lanes and tree for any R below.
 // 64-bit arithmetic runs at half the f32 rate, so it is kept short: the norm weight goes
 // into the rotation's coefficients (A = w_lo cos, B = w_hi sin, ...), formed once a row and
 // warp, a head then costs 4 multiply-adds a pair and one multiplication by 1/rms an
 // element, and the sums of four heads are reduced and inverted together.
 //
-// Four prompts of up to 2048 rows (16 / 8 heads of 128; 154 MB) take 46.6 us, 3.3 TB/s: the
-// 64-bit steps and the conversions to and from them bound it, not memory (23.5 us at a copy's
-// rate).  One row takes 5.8 us on the device, most of it the launch and the angles' sincos.
+// Four prompts of up to 2048 rows (16 / 8 heads of 128; 154 MB) take 46.9 us, 3.3 TB/s, against
+// 23.5 us at a copy's rate: the 64-bit steps, the conversions to and from them (an element is
+// converted for the sum and again for the rotation) and spills (32 bytes stored, 128 loaded at
+// the 64 registers of four CTAs an SM) lie between; sums in two f32 terms, with the 64-bit step
+// only beside a border, were not tried.  One row takes 5.7 us on the device, most of it the
+// launch and the angles' sincos.
 #include "tb_paged.cuh"
 
 namespace {
@@ -74,8 +78,9 @@ __device__ __forceinline__ void store_q8(const float (&x)[NW], int8_t* dq, float
 // R rows a CTA (8 warps): the angles of all of them first (one a thread at R = 4, hd 128), then
 // 8 / R warps a row, each with every (8 / R)-th head, NB heads at a time: their loads are in
 // flight together.  Lane l holds elements l + 32 i, a rotary partner hd / 64 registers away.
-// One row a CTA where there are fewer than five rows a SM (latency): 5.6 us for one row against
-// 9.3 at R = 4, 9.3 against 10.5 for 592 rows, 12.8 against 11.7 for 800, 51 against 35 for 4096.
+// One row a CTA where there are fewer than five rows a SM (latency): 5.2 us for one row against
+// 9.3 at R = 4, 9.4 against 12.3 for 592 rows, 13.8 against 13.6 for 740, 52 against 37 for 4096
+// (16 / 8 heads of 128, calls over 400 MB of inputs in turn).
 constexpr int NB = 4;
 template <int HD, int R>
 __global__ void __launch_bounds__(256, 4) k_paged_prep(const PrepArgs a, int T)
